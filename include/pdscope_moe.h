@@ -383,6 +383,83 @@ int pdscope_decode_run(const pdscope_decode_binding *binding, const void *x, voi
 void pdscope_decode_unbind(pdscope_decode_binding *binding);
 
 /*
+ * 4-bit expert blocks (microscaled floating point): e2m1 values with one e8m0
+ * scale 2^(byte - 127) per 32 consecutive inputs of a row, 17/32 byte a weight.
+ * No counterpart in the reference, whose experts are bf16 only.
+ *   quantize    experts [n, 3*I*H] bf16 (gate|up|down each) -> blocks
+ *               [n, pdscope_mxfp4_block_bytes(H, I)].  A block of 32 whose largest
+ *               magnitude is m has the scale 2^(floor(log2 m) - 2) (at least
+ *               2^-127), each value is rounded to the nearest of 0, 0.5, 1, 1.5, 2,
+ *               3, 4, 6 times that, ties to the even code, above 6 to 6.  32 values
+ *               with an infinity or NaN among them become NaN (byte 255).
+ *   dequantize  the values of blocks, as bf16 (exact).
+ *   pack        blocks of a checkpoint's tensors: codes [n, 3*I*H/2] (input 2i of
+ *               a row in the low half of byte i) and scales [n, 3*I*H/32], gate|up|
+ *               down row-major each; moves bytes only.
+ * The layout of a block is the one the matrix cores read (csrc/mxfp4.h); entry
+ * points that take 4-bit experts address blocks by the same slots tables as bf16
+ * ones.  Limits: H % 128 == 0 and I % 128 == 0 (block_bytes: else 0); every
+ * address 16-byte aligned; 1 <= n <= 65536.
+ */
+size_t pdscope_mxfp4_block_bytes(int H, int I);
+int pdscope_mxfp4_quantize(const void *experts, int n, int H, int I, void *blocks, void *stream);
+int pdscope_mxfp4_dequantize(const void *blocks, int n, int H, int I, void *experts, void *stream);
+int pdscope_mxfp4_pack(const void *codes, const void *scales, int n, int H, int I, void *blocks, void *stream);
+
+/*
+ * The whole layer for 1 to 16 tokens in three launches, over bf16 (mxfp4 == 0)
+ * or 4-bit expert blocks: replaces route (expertbench/adapters/qwen.py:140-152),
+ * the decode submissions (expertbench/pdscope_runtime.py:326-350) and the merge
+ * (pdscope_runtime.py:450-469) for a small batch.
+ *   logits  = bf16(x . gate^T), summed in 64 bits (pdscope_route_topk sums in 32)
+ *   ids, weights as pdscope_route_topk on these logits
+ *   out[t]  = bf16(add_in[t] + sum_s w[t,s] * down(bf16(silu(gate x_t) * up x_t)))
+ * with fp32 accumulation and no rounding between the down product and out
+ * (pdscope_swiglu_decode and the grouped path also round gate, up and each
+ * expert's row to bf16).  An expert without a copy (slots entry 0) adds nothing.
+ * x [T,H], gate [E,H], bias [E] fp32 or NULL, add_in [T,H] bf16 or NULL, logits
+ * [T,E] bf16, ids [T,k] int32, weights [T,k] bf16, out [T,H] bf16.
+ * workspace: pdscope_moe_few_workspace_size bytes, 16-byte aligned, any contents
+ * (0 bytes: outside the limits); calls that overlap in time need one each.
+ * Limits: 1 <= T <= 16, E <= 256, 1 <= k <= min(E, 16), H % 128 == 0, H <= 4096,
+ * I % 128 == 0 (pdscope_moe_few_supported).
+ */
+int pdscope_moe_few_supported(int T, int H, int I, int E, int k);
+size_t pdscope_moe_few_workspace_size(int T, int H, int I, int E, int k);
+int pdscope_moe_few(const void *x, const void *gate, const float *bias, int T, int H, int E, int k,
+                    int normalize, const void *const *slots, int mxfp4, int I, const void *add_in, void *logits,
+                    int32_t *ids, void *weights, void *out, void *workspace, void *stream);
+
+/*
+ * What stands between two blocks, in one launch: the norm after a block, its
+ * gate and residual scale, the residual sum and the norm before the next block.
+ * The reference leaves these to the model's torch modules around its layer hook
+ * (benchmarks/pdscope_compare.py:285-304).
+ *   a = block                                    [T,H] bf16
+ *   a = add_in + sum_s w[t,s] * y[row_of[t*k+s]] (merge_norm_residual: the merge of
+ *       pdscope_merge, in fp32 and not rounded; an entry of row_of outside
+ *       [0, y_rows) adds nothing; add_in [T,H] bf16 or NULL)
+ *   a = a * rsqrt(mean(a^2) + eps) * post_w      (post_w NULL: no norm)
+ *   r = resid + scale * gate * a                 -> out_resid
+ *   n = r * rsqrt(mean(r^2) + eps) * pre_w       -> out_norm (pre_w NULL: ones)
+ * in fp32, each result rounded once (n from the unrounded r).  resid and
+ * out_resid are [T,H] bf16, or fp32 when resid_f32; out_norm is [T,H] bf16; either
+ * output may be NULL, and out_resid may be resid.  post_w and pre_w [H] and gate
+ * are bf16, or fp32 when params_f32; gate (NULL: 1) has a value per token when
+ * gate_rows and per channel when gate_cols: [T,H], [T], [H] or one value.
+ * Limits: T >= 1, 1 <= H <= 16384 (16-byte accesses where H % 8 == 0 and every
+ * address is 16-byte aligned, single values otherwise).
+ */
+int pdscope_norm_residual(const void *block, const void *resid, int resid_f32, const void *post_w,
+                          const void *gate, int gate_rows, int gate_cols, float scale, const void *pre_w,
+                          int params_f32, float eps, int T, int H, void *out_resid, void *out_norm, void *stream);
+int pdscope_merge_norm_residual(const void *y, int64_t y_rows, const int32_t *row_of, const void *w, int k,
+                                const void *add_in, const void *resid, int resid_f32, const void *post_w,
+                                const void *gate, int gate_rows, int gate_cols, float scale, const void *pre_w,
+                                int params_f32, float eps, int T, int H, void *out_resid, void *out_norm,
+                                void *stream);
+
+/*
  * A7 demand staging: replaces the three per-projection non_blocking copies
  * (expertbench/executor.py:341-363).  One hipMemcpyAsync of `bytes` from
  * page-locked host memory into a cache or staging slot on `stream`, then

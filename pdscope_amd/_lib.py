@@ -14,6 +14,7 @@ _vp = ctypes.c_void_p
 _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
+_f32 = ctypes.c_float
 
 # name -> (argtypes, restype)
 SIGNATURES = {
@@ -59,6 +60,18 @@ SIGNATURES = {
                              _vp, ctypes.POINTER(_vp)], _i32),
     "pdscope_decode_run": ([_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp], _i32),
     "pdscope_decode_unbind": ([_vp], None),
+    "pdscope_mxfp4_block_bytes": ([_i32, _i32], _sz),
+    "pdscope_mxfp4_quantize": ([_vp, _i32, _i32, _i32, _vp, _vp], _i32),
+    "pdscope_mxfp4_dequantize": ([_vp, _i32, _i32, _i32, _vp, _vp], _i32),
+    "pdscope_mxfp4_pack": ([_vp, _vp, _i32, _i32, _i32, _vp, _vp], _i32),
+    "pdscope_moe_few_supported": ([_i32, _i32, _i32, _i32, _i32], _i32),
+    "pdscope_moe_few_workspace_size": ([_i32, _i32, _i32, _i32, _i32], _sz),
+    "pdscope_moe_few": ([_vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
+                         _vp], _i32),
+    "pdscope_norm_residual": ([_vp, _vp, _i32, _vp, _vp, _i32, _i32, _f32, _vp, _i32, _f32, _i32, _i32, _vp, _vp,
+                               _vp], _i32),
+    "pdscope_merge_norm_residual": ([_vp, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _f32, _vp, _i32,
+                                     _f32, _i32, _i32, _vp, _vp, _vp], _i32),
     "pdscope_stage_expert": ([_vp, _vp, _sz, _vp, _vp], _i32),
     "pdscope_stage_merge": ([_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp], _i32),
     "pdscope_dispatch_pack": ([_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp], _i32),

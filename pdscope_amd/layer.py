@@ -20,7 +20,7 @@ class MoEWorkspace:
     """Device buffers for up to ``max_tokens`` tokens of one layer shape."""
 
     def __init__(self, max_tokens: int, H: int, I: int, E: int, k: int, device, *, route_only: bool = False,
-                 shared_I: int | None = None):
+                 shared_I: int | None = None, few_tokens: bool = False):
         device = torch.device(device)
         n = max_tokens * k
         i32 = dict(dtype=torch.int32, device=device)
@@ -45,6 +45,13 @@ class MoEWorkspace:
         self.route_ws = ops.new_route_workspace(max_tokens, H, E, device)
         self.pack_ws = torch.empty(max(ops.pack_workspace_size(max_tokens, k, E), 4), dtype=torch.uint8,
                                    device=device)
+        # partial rows of moe_few (up to ops.FEW_MAX_TOKENS tokens of this shape)
+        self.few_ws = None
+        if few_tokens:
+            need = ops.moe_few_workspace_size(min(max_tokens, ops.FEW_MAX_TOKENS), H, I, E, k)
+            if need == 0:
+                raise ValueError("this layer shape is outside moe_few (ops.moe_few_supported)")
+            self.few_ws = torch.empty(need, dtype=torch.uint8, device=device)
         # always-on shared experts (one fused MLP of intermediate shared_I over every token)
         self.shared_I = shared_I
         if shared_I:
@@ -205,6 +212,21 @@ def grouped_ffn(x, packed, sel, bm, max_tiles, slots, ws: MoEWorkspace, *, max_t
     shared = None if shared_slot is None else (shared_slot, ws.shared_I, ws.h_shared, ws.y_shared)
     ops.swiglu_grouped_layer(x, perm, packed.offsets, order, tile_start, max_tiles, bm, tile_down, max_tiles_down, bmd,
                              slots, H, I, ws.h_ws, ws.y, shared=shared)
+
+
+def moe_few(x, gate, slots, ws: MoEWorkspace, *, normalize=True, bias=None, add_in=None, representation="bf16"):
+    """Full layer of 1 to 16 tokens in three launches over bf16 or 4-bit expert
+    blocks (pdscope_moe_few), for decode batches and drafted tokens: returns
+    (out, logits, ids, weights) as moe_forward does, in ws.  The workspace must
+    have been built with few_tokens=True."""
+    if ws.few_ws is None:
+        raise ValueError("moe_few needs a workspace built with few_tokens=True")
+    T = x.shape[0]
+    logits, ids, weights, _ = ws.views(T)
+    out = ws.out[:T]
+    ops.moe_few(x, gate, slots, ws.I, ws.k, normalize, bias=bias, add_in=add_in, representation=representation,
+                out=out, logits=logits, ids=ids, weights=weights, workspace=ws.few_ws)
+    return out, logits, ids, weights
 
 
 def moe_forward(x, gate, slots, ws: MoEWorkspace, *, normalize=True, bias=None, block_m=None, fused_decode=True,

@@ -33,6 +33,15 @@ def _stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _call_on(device, name, *args):
+    """An entry point on the current stream of `device`, which is made the
+    current device for the launch where it is another."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _lib.call(name, *args, _stream(device))
+    with torch.cuda.device(device):
+        return _lib.call(name, *args, _stream(device))
+
+
 def _need(t, name, dtype=None, ndim=None, device=None):
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor")
@@ -636,6 +645,212 @@ def merge(y, row_of, w, out, add_in=None, *, mode="fused"):
     name = "pdscope_merge_ordered" if merge_mode(mode) else "pdscope_merge"
     _lib.call(name, _p(y), _p(row_of), _p(w), T, k, H, _p(add_in), _p(out), _stream(dev))
     return out
+
+
+# ------------------------------------------------------------ 4-bit experts
+
+REPRESENTATIONS = ("bf16", "mxfp4")
+
+
+def is_mxfp4(representation: str) -> bool:
+    """Whether an expert representation is the 4-bit one ("mxfp4") rather than "bf16"."""
+    if representation not in REPRESENTATIONS:
+        raise ValueError(f"representation must be one of {REPRESENTATIONS}, got {representation!r}")
+    return representation == "mxfp4"
+
+
+def mxfp4_block_bytes(H: int, I: int) -> int:
+    """Bytes of one 4-bit expert block (17/32 of a byte per weight)."""
+    n = int(_lib.load().pdscope_mxfp4_block_bytes(int(H), int(I)))
+    if n == 0:
+        raise ValueError(f"4-bit experts need H % 128 == 0 and I % 128 == 0, got H={H}, I={I}")
+    return n
+
+
+def _mxfp4_out(out, E, width, dtype, dev):
+    if out is None:
+        return torch.empty((E, width), dtype=dtype, device=dev)
+    _need(out, "out", dtype, 2, dev)
+    if tuple(out.shape) != (E, width):
+        raise ValueError(f"out must be [{E}, {width}], got {tuple(out.shape)}")
+    return out
+
+
+def mxfp4_quantize(experts, H, I, out=None) -> torch.Tensor:
+    """4-bit blocks [E, mxfp4_block_bytes(H, I)] uint8 of bf16 expert blocks
+    [E, 3*I*H] (gate|up|down each; see pdscope_mxfp4_quantize for the rounding)."""
+    _need(experts, "experts", BF16, 2)
+    nbytes = mxfp4_block_bytes(H, I)
+    if experts.shape[1] != 3 * I * H or experts.shape[0] < 1:
+        raise ValueError(f"experts must be [E, 3*I*H] with E >= 1, got {tuple(experts.shape)}")
+    out = _mxfp4_out(out, experts.shape[0], nbytes, torch.uint8, experts.device)
+    _call_on(experts.device, "pdscope_mxfp4_quantize", _p(experts), experts.shape[0], H, I, _p(out))
+    return out
+
+
+def mxfp4_dequantize(blocks, H, I, out=None) -> torch.Tensor:
+    """The values of 4-bit blocks as bf16 blocks [E, 3*I*H] (exact)."""
+    _need(blocks, "blocks", torch.uint8, 2)
+    nbytes = mxfp4_block_bytes(H, I)
+    if blocks.shape[1] != nbytes or blocks.shape[0] < 1:
+        raise ValueError(f"blocks must be [E, {nbytes}] with E >= 1, got {tuple(blocks.shape)}")
+    out = _mxfp4_out(out, blocks.shape[0], 3 * I * H, BF16, blocks.device)
+    _call_on(blocks.device, "pdscope_mxfp4_dequantize", _p(blocks), blocks.shape[0], H, I, _p(out))
+    return out
+
+
+def mxfp4_pack(codes, scales, H, I, out=None) -> torch.Tensor:
+    """4-bit blocks of a checkpoint's tensors: codes uint8 [E, 3*I*H/2] (two
+    e2m1 values a byte, the first in the low half) and e8m0 scales uint8
+    [E, 3*I*H/32], row-major gate|up|down each."""
+    _need(codes, "codes", torch.uint8, 2)
+    _need(scales, "scales", torch.uint8, 2, codes.device)
+    nbytes = mxfp4_block_bytes(H, I)
+    E, n = codes.shape[0], 3 * I * H
+    if E < 1 or codes.shape[1] != n // 2 or tuple(scales.shape) != (E, n // 32):
+        raise ValueError(f"codes must be [E, {n // 2}] and scales [E, {n // 32}], got {tuple(codes.shape)} and "
+                         f"{tuple(scales.shape)}")
+    out = _mxfp4_out(out, E, nbytes, torch.uint8, codes.device)
+    _call_on(codes.device, "pdscope_mxfp4_pack", _p(codes), _p(scales), E, H, I, _p(out))
+    return out
+
+
+# --------------------------------------------------------- a few tokens' layer
+
+FEW_MAX_TOKENS = 16
+
+
+def moe_few_supported(T, H, I, E, k) -> bool:
+    """Whether moe_few runs T tokens of a layer shape (either representation)."""
+    return bool(_lib.load().pdscope_moe_few_supported(int(T), int(H), int(I), int(E), int(k)))
+
+
+def moe_few_workspace_size(T, H, I, E, k) -> int:
+    return int(_lib.load().pdscope_moe_few_workspace_size(int(T), int(H), int(I), int(E), int(k)))
+
+
+def moe_few(x, gate, slots, I, top_k, normalize, *, bias=None, add_in=None, representation="bf16", out, logits, ids,
+            weights, workspace):
+    """The whole layer of 1 to 16 tokens (router, top-k, SwiGLU experts, merge)
+    over the bf16 or 4-bit blocks in `slots`; see pdscope_moe_few.  add_in
+    [T, H] (shared experts' output) is added unweighted."""
+    _need(x, "inputs", BF16, 2)
+    dev = x.device
+    _need(gate, "gate", BF16, 2, dev)
+    T, H = x.shape
+    E = gate.shape[0]
+    mx = is_mxfp4(representation)
+    if gate.shape[1] != H:
+        raise ValueError("router input shape/dtype mismatch")
+    if type(top_k) is not int or not moe_few_supported(T, H, I, E, top_k):
+        raise ValueError(f"moe_few: unsupported shape T={T}, H={H}, I={I}, E={E}, k={top_k}")
+    _need(slots, "slots", torch.int64, 1, dev)
+    if slots.numel() < E:
+        raise ValueError("slots must hold one entry per expert")
+    if bias is not None:
+        _need(bias, "bias", torch.float32, 1, dev)
+        if bias.numel() != E:
+            raise ValueError("bias must have one entry per expert")
+    _need(ids, "ids", torch.int32, 2, dev)
+    for t, n, shape in ((logits, "logits", (T, E)), (weights, "weights", (T, top_k)), (out, "out", (T, H)),
+                        (ids, "ids", (T, top_k)), (add_in, "add_in", (T, H))):
+        if t is None and n == "add_in":
+            continue
+        _need(t, n, torch.int32 if n == "ids" else BF16, 2, dev)
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{n} must be {list(shape)}, got {list(t.shape)}")
+    _need(workspace, "workspace", torch.uint8, 1, dev)
+    if workspace.numel() < moe_few_workspace_size(T, H, I, E, top_k):
+        raise ValueError("moe_few workspace too small for this token count")
+    _call_on(dev, "pdscope_moe_few", _p(x), _p(gate), _p(bias), T, H, E, top_k, int(bool(normalize)), _p(slots),
+             int(mx), I, _p(add_in), _p(logits), _p(ids), _p(weights), _p(out), _p(workspace))
+    return out
+
+
+# ------------------------------------------------------ between two blocks
+
+def _norm_args(T, H, dev, resid, post_weight, gate, pre_weight, out_resid, out_norm, want_resid):
+    """Checks of norm_residual / merge_norm_residual and their allocated outputs."""
+    _need(resid, "resid", None, 2, dev)
+    if resid.dtype not in (BF16, torch.float32):
+        raise ValueError(f"resid must be bf16 or fp32, got {resid.dtype}")
+    if tuple(resid.shape) != (T, H):
+        raise ValueError(f"resid must be [{T}, {H}], got {list(resid.shape)}")
+    given = [(t, n) for t, n in ((post_weight, "post_weight"), (gate, "gate"), (pre_weight, "pre_weight"))
+             if t is not None]
+    P = given[0][0].dtype if given and isinstance(given[0][0], torch.Tensor) else BF16
+    if P not in (BF16, torch.float32):
+        raise ValueError(f"{given[0][1]} must be bf16 or fp32, got {P}")
+    for t, n in given:
+        _need(t, n, P, None, dev)
+        if n != "gate" and tuple(t.shape) != (H,):
+            raise ValueError(f"{n} must be [{H}], got {list(t.shape)}")
+    rows = cols = 0
+    if gate is not None:
+        if tuple(gate.shape) not in ((H,), (1, H), (T, 1), (T, H)):
+            raise ValueError(f"gate must be [H], [1, H], [T, 1] or [T, H], got {list(gate.shape)}")
+        rows = int(gate.ndim == 2 and gate.shape[0] == T)
+        cols = int(gate.ndim == 1 or gate.shape[1] == H)
+    if out_resid is not None:
+        _need(out_resid, "out_resid", resid.dtype, 2, dev)
+        if tuple(out_resid.shape) != (T, H):
+            raise ValueError(f"out_resid must be [{T}, {H}], got {list(out_resid.shape)}")
+    elif want_resid:
+        out_resid = torch.empty_like(resid)
+    if out_norm is None:
+        out_norm = torch.empty((T, H), dtype=BF16, device=dev)
+    else:
+        _need(out_norm, "out_norm", BF16, 2, dev)
+        if tuple(out_norm.shape) != (T, H):
+            raise ValueError(f"out_norm must be [{T}, {H}], got {list(out_norm.shape)}")
+    return int(resid.dtype == torch.float32), rows, cols, int(P == torch.float32), out_resid, out_norm
+
+
+def norm_residual(block, resid, *, post_weight=None, gate=None, scale=1.0, pre_weight=None, eps=1e-6, out_resid=None,
+                  out_norm=None, want_resid=True):
+    """The norm after a block (post_weight [H]; None: none), its gate and
+    residual scale, the residual sum and the norm before the next block
+    (pre_weight [H]; None: ones) in one launch: returns (resid + scale * gate *
+    norm(block), its RMS norm as bf16).  block [T, H] bf16; resid [T, H] bf16
+    or fp32 (the sum has its type; out_resid may be resid); weights and gate
+    ([H], [T, 1] or [T, H]) bf16 or fp32, all alike.  want_resid=False without
+    out_resid computes the norm alone and returns None for the sum."""
+    _need(block, "block", BF16, 2)
+    T, H = block.shape
+    f32, rows, cols, p32, out_resid, out_norm = _norm_args(T, H, block.device, resid, post_weight, gate, pre_weight,
+                                                           out_resid, out_norm, want_resid)
+    _call_on(block.device, "pdscope_norm_residual", _p(block), _p(resid), f32, _p(post_weight), _p(gate), rows, cols,
+             float(scale), _p(pre_weight), p32, float(eps), T, H, _p(out_resid), _p(out_norm))
+    return out_resid, out_norm
+
+
+def merge_norm_residual(y, row_of, w, resid, *, add_in=None, post_weight=None, gate=None, scale=1.0, pre_weight=None,
+                        eps=1e-6, out_resid=None, out_norm=None, want_resid=True):
+    """norm_residual of the experts' weighted merge, which is summed in the same
+    launch (as merge(y, row_of, w, add_in=add_in) in mode 'fused', and not rounded):
+    y [rows, H] grouped expert rows, row_of [T*k] int32 (an entry outside
+    [0, rows) adds nothing), w [T, k] bf16, add_in [T, H] bf16 or None."""
+    _need(w, "weights", BF16, 2)
+    dev = w.device
+    T, k = w.shape
+    _need(resid, "resid", None, 2, dev)
+    H = resid.shape[1]
+    _need(y, "y", BF16, None, dev)
+    _need(row_of, "row_of", torch.int32, 1, dev)
+    if row_of.numel() != T * k:
+        raise ValueError(f"row_of must hold T*k = {T * k} entries, got {row_of.numel()}")
+    if H < 1 or y.numel() < H or y.numel() % H:
+        raise ValueError(f"y must hold rows of {H} values")
+    if add_in is not None:
+        _need(add_in, "add_in", BF16, 2, dev)
+        if tuple(add_in.shape) != (T, H):
+            raise ValueError(f"add_in must be [{T}, {H}], got {list(add_in.shape)}")
+    f32, rows, cols, p32, out_resid, out_norm = _norm_args(T, H, dev, resid, post_weight, gate, pre_weight, out_resid,
+                                                           out_norm, want_resid)
+    _call_on(dev, "pdscope_merge_norm_residual", _p(y), y.numel() // H, _p(row_of), _p(w), k, _p(add_in), _p(resid),
+             f32, _p(post_weight), _p(gate), rows, cols, float(scale), _p(pre_weight), p32, float(eps), T, H,
+             _p(out_resid), _p(out_norm))
+    return out_resid, out_norm
 
 
 def stage_expert(dst, src, *, event=None, stream=None):
