@@ -407,6 +407,22 @@ int pdscope_mxfp4_dequantize(const void *blocks, int n, int H, int I, void *expe
 int pdscope_mxfp4_pack(const void *codes, const void *scales, int n, int H, int I, void *blocks, void *stream);
 
 /*
+ * pdscope_swiglu_grouped over 4-bit expert blocks (same arguments; slots hold the
+ * addresses of pdscope_mxfp4_quantize's or _pack's blocks):
+ *   h[r] = bf16(silu(x . gate_e^T) * (x . up_e^T)),  y[r] = bf16(h[r] . down_e^T)
+ * on the weights' exact values, bf16 activations, fp32 accumulation (gate and up
+ * are not rounded, unlike the bf16 path's).  block_m: 32, 64 or 128, the row tile
+ * of the schedule (pdscope_grouped_mxfp4_block_m picks it from the mean rows per
+ * selected expert).  Rows of an expert without a copy keep what y holds.
+ * Limits: H % 128 == 0 and I % 128 == 0; x, h_ws and y 16-byte aligned.
+ */
+int pdscope_grouped_mxfp4_block_m(int rows_hint);
+int pdscope_swiglu_grouped_mxfp4(const void *x, const int32_t *perm_token, const int32_t *offsets,
+                                 const int32_t *sel, int nsel, const int32_t *tile_start, int max_tiles,
+                                 int block_m, const void *const *slots, int H, int I, void *h_ws, void *y,
+                                 void *stream);
+
+/*
  * The whole layer for 1 to 16 tokens in three launches, over bf16 (mxfp4 == 0)
  * or 4-bit expert blocks: replaces route (expertbench/adapters/qwen.py:140-152),
  * the decode submissions (expertbench/pdscope_runtime.py:326-350) and the merge

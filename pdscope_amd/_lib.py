@@ -64,6 +64,8 @@ SIGNATURES = {
     "pdscope_mxfp4_quantize": ([_vp, _i32, _i32, _i32, _vp, _vp], _i32),
     "pdscope_mxfp4_dequantize": ([_vp, _i32, _i32, _i32, _vp, _vp], _i32),
     "pdscope_mxfp4_pack": ([_vp, _vp, _i32, _i32, _i32, _vp, _vp], _i32),
+    "pdscope_grouped_mxfp4_block_m": ([_i32], _i32),
+    "pdscope_swiglu_grouped_mxfp4": ([_vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp], _i32),
     "pdscope_moe_few_supported": ([_i32, _i32, _i32, _i32, _i32], _i32),
     "pdscope_moe_few_workspace_size": ([_i32, _i32, _i32, _i32, _i32], _sz),
     "pdscope_moe_few": ([_vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp,

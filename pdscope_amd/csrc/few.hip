@@ -70,7 +70,7 @@ __global__ __launch_bounds__(256) void few_router_kernel(const uint16_t *__restr
         const uint4 w = ld_g(gate + (size_t)e * H + 8 * c);
 #pragma unroll
         for (int t0 = 0; t0 < kFewMaxT; t0 += 4) {
-            if (t0 >= T) break;
+            if (t0 >= T) continue;
             uint4 v[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) v[q] = ld_g(x + (size_t)min(t0 + q, T - 1) * H + 8 * c);
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(256) void few_router_kernel(const uint16_t *__restr
     }
 #pragma unroll
     for (int t = 0; t < kFewMaxT; ++t) {
-        if (t >= T) break;
+        if (t >= T) continue;
 #pragma unroll
         for (int d = 32; d; d >>= 1) acc[t] += __shfl_xor(acc[t], d);
         if (lane == 0) s_sum[wave][t] = acc[t];

@@ -146,17 +146,31 @@ def shared_forward(x, shared_slot, ws: MoEWorkspace):
 
 
 def experts_resident(x, ids, weights, slots, ws: MoEWorkspace, out=None, *, block_m=None, add_in=None,
-                     merge="fused", before_merge=None, shared_slot=None):
+                     merge="fused", before_merge=None, shared_slot=None, representation="bf16"):
     """K4 (T == 1) or K2+K3+K5 (T > 1) over experts that are all addressable in `slots`.
     add_in [T, H] bf16 (shared-expert output) is added unweighted in the merge;
     before_merge() runs right before the merge is enqueued (to order add_in's producer).
     shared_slot (int64 [1], T > 1, shared_in_grouped(ws)): shared experts run as
     further tiles of the grouped launches, into ws.y_shared, and are added in the merge.
     merge: 'fused' (fp32 sum, one rounding) or 'reference' (bf16 adds in
-    ascending expert id, the reference runtime's default merge)."""
+    ascending expert id, the reference runtime's default merge).
+    representation: what `slots` addresses, "bf16" or "mxfp4" blocks (4-bit, any
+    T: K2, their grouped launches, K5; shared experts' output comes through add_in)."""
     T = x.shape[0]
     H, I, E, k = ws.H, ws.I, ws.E, ws.k
     out = ws.out[:T] if out is None else out
+    if ops.is_mxfp4(representation):
+        if shared_slot is not None:
+            raise ValueError("shared experts join 4-bit routed experts through add_in")
+        _, _, _, packed = ws.views(T)
+        bm = block_m or ops.grouped_mxfp4_block_m((T * k) // E)
+        ops.pack(ids, E, out=packed, workspace=ws.pack_ws, schedule=(ws.sel_all, bm, ws.sel_order, ws.tile_start))
+        ops.swiglu_grouped_mxfp4(x, packed.perm_token, packed.offsets, ws.sel_order, ws.tile_start,
+                                 (T * k + bm - 1) // bm + E, bm, slots, H, I, ws.h_ws, ws.y)
+        if before_merge is not None:
+            before_merge()
+        ops.merge(ws.y, packed.row_of, weights, out, add_in=add_in, mode=merge)
+        return out
     if T == 1 and add_in is None and shared_slot is None:
         ops.swiglu_decode(x, ids, weights, slots, H, I, ws.h_ws, out, merge=merge)
         return out
@@ -230,7 +244,7 @@ def moe_few(x, gate, slots, ws: MoEWorkspace, *, normalize=True, bias=None, add_
 
 
 def moe_forward(x, gate, slots, ws: MoEWorkspace, *, normalize=True, bias=None, block_m=None, fused_decode=True,
-                shared_slot=None, merge="fused", next_gate=None, pred_out=None):
+                shared_slot=None, merge="fused", next_gate=None, pred_out=None, representation="bf16"):
     """Full layer: returns (out [T,H] bf16, logits, ids int32 [T,k], weights bf16 [T,k]).
 
     merge: 'fused' (each token's k weighted rows summed in fp32, one
@@ -245,8 +259,27 @@ def moe_forward(x, gate, slots, ws: MoEWorkspace, *, normalize=True, bias=None, 
     next_gate / pred_out (T == 1 on the single-launch kernel only, see
     ops.decode_chained_supported): the next layer's gate-fallback prediction,
     top-k of next_gate . x, is written to pred_out [k] int32 by the same launch.
+    representation: what `slots` addresses, "bf16" or "mxfp4" blocks.  4-bit
+    experts take up to 16 tokens through moe_few where the workspace was built
+    with few_tokens=True and merge is 'fused', and more through route (K1) and
+    their grouped launches; shared experts stay bf16 (one MLP, read once for all tokens).
     """
     T = x.shape[0]
+    if ops.is_mxfp4(representation):
+        if next_gate is not None or pred_out is not None:
+            raise ValueError("the fused next-layer prediction needs bf16 experts")
+        y_shared = None
+        if shared_slot is not None:
+            if not ws.shared_I:
+                raise ValueError("shared experts need a workspace built with shared_I")
+            y_shared = shared_forward(x, shared_slot, ws)
+        if T <= ops.FEW_MAX_TOKENS and ws.few_ws is not None and not ops.merge_mode(merge) and block_m is None:
+            return moe_few(x, gate, slots, ws, normalize=normalize, bias=bias, add_in=y_shared,
+                           representation=representation)
+        logits, ids, weights = route(x, gate, ws, normalize=normalize, bias=bias)
+        out = experts_resident(x, ids, weights, slots, ws, block_m=block_m, add_in=y_shared, merge=merge,
+                               representation=representation)
+        return out, logits, ids, weights
     if shared_slot is not None:
         if not ws.shared_I:
             raise ValueError("shared experts need a workspace built with shared_I")

@@ -715,6 +715,31 @@ def mxfp4_pack(codes, scales, H, I, out=None) -> torch.Tensor:
     return out
 
 
+def grouped_mxfp4_block_m(rows_hint: int) -> int:
+    """Row tile of swiglu_grouped_mxfp4 for rows_hint mean rows per expert."""
+    return int(_lib.load().pdscope_grouped_mxfp4_block_m(int(rows_hint)))
+
+
+def swiglu_grouped_mxfp4(x, perm_token, offsets, sel, tile_start, max_tiles, block_m, slots, H, I, h_ws, y):
+    """swiglu_grouped over the 4-bit blocks in `slots`; block_m 32, 64 or 128."""
+    _need(x, "inputs", BF16, 2)
+    dev = x.device
+    for t, n in ((perm_token, "perm_token"), (offsets, "offsets"), (sel, "sel"), (tile_start, "tile_start")):
+        _need(t, n, torch.int32, 1, dev)
+    _need(slots, "slots", torch.int64, 1, dev)
+    _need(h_ws, "h_ws", BF16, None, dev)
+    _need(y, "y", BF16, None, dev)
+    if x.shape[1] != H:
+        raise ValueError(f"inputs must be [T, {H}], got {list(x.shape)}")
+    if h_ws.numel() < perm_token.numel() * I or y.numel() < perm_token.numel() * H:
+        raise ValueError("h_ws / y workspaces are smaller than rows x I / rows x H")
+    if tile_start.numel() < sel.numel() + 1 or offsets.numel() < slots.numel() + 1:
+        raise ValueError("tile_start must hold one entry more than sel, offsets one more than slots")
+    _call_on(dev, "pdscope_swiglu_grouped_mxfp4", _p(x), _p(perm_token), _p(offsets), _p(sel), sel.numel(),
+             _p(tile_start), int(max_tiles), int(block_m), _p(slots), H, I, _p(h_ws), _p(y))
+    return y
+
+
 # --------------------------------------------------------- a few tokens' layer
 
 FEW_MAX_TOKENS = 16
