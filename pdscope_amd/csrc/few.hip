@@ -54,51 +54,76 @@ struct FewArgs {
 
 // ---------------------------------------------------------------- router
 
-// One workgroup per expert.  Products of two bf16 values are exact in fp32; the
-// sums are kept in fp64, so the logits are the exactly rounded ones (but for a
-// double rounding by way of fp32, as a conversion from fp64 to bf16 goes) and the
-// selection does not depend on the order of the sum.
+// The same double of lane l ^ 32 / l ^ 16 (in one of the two results; the other
+// is the lane's own) and of a lane N further around its row of 16.
+__device__ __forceinline__ double sum_swap32(double v) {
+    const uint64_t u = __double_as_longlong(v);
+    const auto lo = __builtin_amdgcn_permlane32_swap((uint32_t)u, (uint32_t)u, false, false);
+    const auto hi = __builtin_amdgcn_permlane32_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+    return __longlong_as_double((uint64_t)hi[0] << 32 | lo[0]) + __longlong_as_double((uint64_t)hi[1] << 32 | lo[1]);
+}
+__device__ __forceinline__ double sum_swap16(double v) {
+    const uint64_t u = __double_as_longlong(v);
+    const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+    return __longlong_as_double((uint64_t)hi[0] << 32 | lo[0]) + __longlong_as_double((uint64_t)hi[1] << 32 | lo[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ double sum_ror(double v) {
+    const uint64_t u = __double_as_longlong(v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xf, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+    return v + __longlong_as_double((uint64_t)hi << 32 | lo);
+}
+// Sum over the wave, in every lane (the steps of wave_sum, on doubles).
+__device__ __forceinline__ double wave_sum64(double v) {
+    v = sum_swap16(sum_swap32(v));
+    v = sum_ror<0x124>(sum_ror<0x128>(v));     // row_ror 8, 4
+    return sum_ror<0x121>(sum_ror<0x122>(v));  // row_ror 2, 1
+}
+
+// One workgroup per expert and four tokens.  Products of two bf16 values are
+// exact in fp32; the sums are kept in fp64, so the logits are the exactly rounded
+// ones (but for a double rounding by way of fp32, as a conversion from fp64 to
+// bf16 goes) and the selection does not depend on the order of the sum.  Bound by
+// latency: one load of the gate row's piece and of each token's, the sums
+// (fp64 runs at the rate of fp32 here), a store.
+constexpr int kRouterT = 4;
 __global__ __launch_bounds__(256) void few_router_kernel(const uint16_t *__restrict__ x,
                                                          const uint16_t *__restrict__ gate, int T, int H, int E,
                                                          uint16_t *__restrict__ logits) {
-    __shared__ double s_sum[4][kFewMaxT];
-    const int e = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    double acc[kFewMaxT];
-#pragma unroll
-    for (int t = 0; t < kFewMaxT; ++t) acc[t] = 0.0;
+    __shared__ double s_sum[4][kRouterT];
+    const int e = blockIdx.x, t0 = blockIdx.y * kRouterT, tid = threadIdx.x, wave = tid >> 6;
+    const int nt = min(kRouterT, T - t0);  // uniform
+    double acc[kRouterT] = {};
     for (int c = tid; c < H / 8; c += 256) {
         const uint4 w = ld_g(gate + (size_t)e * H + 8 * c);
+        uint4 v[kRouterT];
 #pragma unroll
-        for (int t0 = 0; t0 < kFewMaxT; t0 += 4) {
-            if (t0 >= T) continue;
-            uint4 v[4];
+        for (int q = 0; q < kRouterT; ++q)
+            if (q < nt) v[q] = ld_g(x + (size_t)(t0 + q) * H + 8 * c);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = ld_g(x + (size_t)min(t0 + q, T - 1) * H + 8 * c);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                double s = acc[t0 + q];
-                s += (double)(lo_bf(v[q].x) * lo_bf(w.x));
-                s += (double)(hi_bf(v[q].x) * hi_bf(w.x));
-                s += (double)(lo_bf(v[q].y) * lo_bf(w.y));
-                s += (double)(hi_bf(v[q].y) * hi_bf(w.y));
-                s += (double)(lo_bf(v[q].z) * lo_bf(w.z));
-                s += (double)(hi_bf(v[q].z) * hi_bf(w.z));
-                s += (double)(lo_bf(v[q].w) * lo_bf(w.w));
-                s += (double)(hi_bf(v[q].w) * hi_bf(w.w));
-                acc[t0 + q] = s;
+        for (int q = 0; q < kRouterT; ++q)
+            if (q < nt) {
+                acc[q] += (double)(lo_bf(v[q].x) * lo_bf(w.x));
+                acc[q] += (double)(hi_bf(v[q].x) * hi_bf(w.x));
+                acc[q] += (double)(lo_bf(v[q].y) * lo_bf(w.y));
+                acc[q] += (double)(hi_bf(v[q].y) * hi_bf(w.y));
+                acc[q] += (double)(lo_bf(v[q].z) * lo_bf(w.z));
+                acc[q] += (double)(hi_bf(v[q].z) * hi_bf(w.z));
+                acc[q] += (double)(lo_bf(v[q].w) * lo_bf(w.w));
+                acc[q] += (double)(hi_bf(v[q].w) * hi_bf(w.w));
             }
+    }
+#pragma unroll
+    for (int q = 0; q < kRouterT; ++q)
+        if (q < nt) {
+            acc[q] = wave_sum64(acc[q]);
+            if ((tid & 63) == 0) s_sum[wave][q] = acc[q];
         }
-    }
-#pragma unroll
-    for (int t = 0; t < kFewMaxT; ++t) {
-        if (t >= T) continue;
-#pragma unroll
-        for (int d = 32; d; d >>= 1) acc[t] += __shfl_xor(acc[t], d);
-        if (lane == 0) s_sum[wave][t] = acc[t];
-    }
     __syncthreads();
-    if (tid < T)
-        logits[(size_t)tid * E + e] =
+    if (tid < nt)
+        logits[(size_t)(t0 + tid) * E + e] =
             (uint16_t)f2bf((float)((s_sum[0][tid] + s_sum[1][tid]) + (s_sum[2][tid] + s_sum[3][tid])));
 }
 
@@ -119,11 +144,11 @@ struct FewStage {
 template <bool MX, int KQ>
 __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
     __shared__ __attribute__((aligned(16))) float s_part[8 * 4 * 64 * 4];  // 32 KB; the logits before that
-    __shared__ __attribute__((aligned(16))) uint16_t s_h[kFewMaxT * 40];   // rows of 32, 80 bytes apart
+    __shared__ __attribute__((aligned(16))) uint16_t s_h[2 * kFewMaxT * 40];  // h and its rest; rows of 32, 80 bytes apart
     __shared__ TopkScratch s_tk[8];
-    __shared__ int s_id[256], s_row[256], s_list[256], s_pos[256], s_mask[256];
+    __shared__ int s_id[256], s_first[256], s_mask[256];
     __shared__ float s_w[256];
-    __shared__ int s_cnt[4], s_seg[4];
+    __shared__ int s_rows[4];
     __shared__ const uint8_t *s_base[256];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int T = a.T, H = a.H, E = a.E, k = a.k, I = a.I;
@@ -143,9 +168,13 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
                                                                 32 * jj + 8 * g);
         }
 
-    // ---- routing, by every workgroup for itself
+    // ---- routing, by every workgroup for itself (everything it reads was asked
+    // for above or here at once; one barrier before and one behind the selection)
     for (int i = tid; i < T * E; i += 512) s_part[i] = bf2f(a.logits[i]);
-    if (tid < 256) s_mask[tid] = 0;
+    if (tid < 256) {
+        s_mask[tid] = 0;
+        s_base[tid] = tid < E ? a.slots[tid] : nullptr;
+    }
     __syncthreads();
     for (int t = wave; t < T; t += 8) {
         TopkScratch *sc = s_tk + wave;
@@ -160,6 +189,7 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
             const uint16_t w = sc->selw[lane];
             s_id[t * k + lane] = id;
             s_w[t * k + lane] = bf2f(w);
+            if (s_base[id]) atomicOr(&s_mask[id], 1 << t);  // the tokens of each expert that has a copy
             if (blockIdx.x == 0) {
                 a.ids[t * k + lane] = id;
                 a.weights[t * k + lane] = w;
@@ -168,51 +198,73 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
         wave_lds_sync();  // before the next token overwrites the scratch
     }
     __syncthreads();
-    // tokens of each expert that has a copy; the list of these experts in order
-    if (tid < T * k && a.slots[s_id[tid]]) atomicOr(&s_mask[s_id[tid]], 1 << (tid / k));
-    __syncthreads();
-    const bool hit = tid < 256 && s_mask[tid] != 0;
-    const unsigned long long hits = __ballot(hit);
-    if (tid < 256 && lane == 0) s_cnt[wave] = __popcll(hits);
-    __syncthreads();
-    if (hit) {
-        int pos = __popcll(hits & ((1ull << lane) - 1));
-        for (int w = 0; w < wave; ++w) pos += s_cnt[w];
-        s_list[pos] = tid;
-        s_pos[tid] = pos;
-        s_base[pos] = a.slots[tid];
+    // The list: these experts in ascending order, as four 64-bit masks that every
+    // wave holds.
+    uint64_t hits[4];
+    int total = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        hits[j] = __ballot(s_mask[64 * j + lane] != 0);
+        total += __popcll(hits[j]);
     }
-    __syncthreads();
-    const int ns = I / kFewChunk;
-    const int n = __builtin_amdgcn_readfirstlane(s_cnt[0] + s_cnt[1] + s_cnt[2] + s_cnt[3]) * ns;
+    auto expert_at = [&](int u) __attribute__((always_inline)) {  // the u-th of the list
+        int e = 0, before = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int rank = before + __builtin_amdgcn_mbcnt_hi((uint32_t)(hits[j] >> 32),
+                                                                __builtin_amdgcn_mbcnt_lo((uint32_t)hits[j], 0));
+            const uint64_t at = __ballot((hits[j] >> lane & 1) && rank == u);
+            if (at) e = 64 * j + __builtin_ctzll(at);
+            before += __popcll(hits[j]);
+        }
+        return __builtin_amdgcn_readfirstlane(e);
+    };
+    auto place_of = [&](int e) __attribute__((always_inline)) {  // and the reverse
+        int pos = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int below = e - 64 * j;
+            pos += __popcll(below >= 64 ? hits[j] : below > 0 ? hits[j] & ((1ull << below) - 1) : 0);
+        }
+        return pos;
+    };
+    const int ns = I / kFewChunk, n = __builtin_amdgcn_readfirstlane(total) * ns;
     const int G = min((int)gridDim.x, n);  // pieces: every one has a chunk
     // piece b takes chunks [b n / G, (b + 1) n / G); the piece of chunk c:
     auto piece_of = [&](int c) { return (int)(((int64_t)(c + 1) * G - 1) / n); };
-    // a partial row for every token, expert of it and piece of that expert, in
-    // the order of the (token, slot) pairs
-    int rows = 0;
-    if (tid < T * k && (s_mask[s_id[tid]] != 0)) {
-        const int u = s_pos[s_id[tid]];
-        rows = piece_of((u + 1) * ns - 1) - piece_of(u * ns) + 1;
-    }
-    int incl = rows;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(incl, d);
-        if (lane >= d) incl += v;
-    }
-    if (tid < 256 && lane == 63) s_seg[wave] = incl;
-    __syncthreads();
-    if (tid < 256) {
-        int first = incl - rows;
-        for (int w = 0; w < wave; ++w) first += s_seg[w];
-        s_row[tid] = first;
-        if (blockIdx.x == 0) {
-            if (tid < T * k && tid % k == 0) a.row_base[tid / k] = first;
-            if (tid == T * k - 1) a.row_base[T] = first + rows;
+    // A partial row for every token, expert of it and piece of that expert, in
+    // the order of the (token, slot) pairs: s_first counts within 64 pairs, s_rows
+    // the 64s.  Read behind the barriers of the first chunk.
+    auto count_rows = [&]() __attribute__((always_inline)) {
+        if (tid >= 256) return;
+        int rows = 0;
+        if (tid < T * k && s_mask[s_id[tid]] != 0) {
+            const int u = place_of(s_id[tid]);
+            rows = piece_of((u + 1) * ns - 1) - piece_of(u * ns) + 1;
         }
+        int incl = rows;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int v = __shfl_up(incl, d);
+            if (lane >= d) incl += v;
+        }
+        s_first[tid] = incl - rows;
+        if (lane == 63) s_rows[wave] = incl;
+    };
+    auto first_row = [&](int p) __attribute__((always_inline)) {
+        int v = s_first[p];
+        for (int w = 0; w < p >> 6; ++w) v += s_rows[w];
+        return v;
+    };
+    auto write_rows = [&]() __attribute__((always_inline)) {  // for the merge
+        if (tid < T) a.row_base[tid] = first_row(tid * k);
+        if (tid == T) a.row_base[T] = s_rows[0] + s_rows[1] + s_rows[2] + s_rows[3];
+    };
+    if (G == 0 && blockIdx.x == 0) {  // no expert has a copy
+        count_rows();
+        __syncthreads();
+        write_rows();
     }
-    __syncthreads();
     if ((int)blockIdx.x >= G) return;
     const int c0 = (int)((int64_t)blockIdx.x * n / G), c1 = (int)((int64_t)(blockIdx.x + 1) * n / G);
 
@@ -227,10 +279,10 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
     // load is one lane offset from it) and its place in the expert
     struct Chunk {
         const uint8_t *base;
-        int u, j;
+        int e, u, j;  // expert, its place in the list, the chunk's in the expert
     };
-    auto block_of = [&](int u) __attribute__((always_inline)) {
-        const uint64_t p = reinterpret_cast<uint64_t>(s_base[u]);
+    auto block_of = [&](int e) __attribute__((always_inline)) {
+        const uint64_t p = reinterpret_cast<uint64_t>(s_base[e]);
         // readfirstlane returns an int: unsigned before it is widened
         const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)p);
         const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
@@ -285,7 +337,7 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
 
     auto chunk = [&](const Chunk &c, const Chunk &next, bool more) __attribute__((always_inline)) {
         f32x4_t acc1[4] = {};
-        bf16x8_t hf = {};
+        bf16x8_t hf[2] = {};
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             if (s == NS1) {
@@ -302,45 +354,57 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
                     gs += s_part[w * 1024 + tid];
                     us += s_part[w * 1024 + 512 + tid];
                 }
-                // h is rounded to bf16, the matrix cores' input
-                s_h[((tid >> 2) & 15) * 40 + (tid >> 8) * 16 + ((tid >> 6) & 3) * 4 + (tid & 3)] =
-                    (uint16_t)f2bf(silu_fast(gs) * us);
+                // h as the sum of two bf16 values (16 bits of it): the matrix cores
+                // take bf16, and a second product per weight costs nothing beside
+                // the stream, so h adds no rounding that out would show
+                const float h = silu_fast(gs) * us;
+                const uint32_t h0 = f2bf(h);
+                const float rest = (h0 & 0x7f80u) == 0x7f80u ? 0.0f : h - bf2f(h0);  // none of an infinity
+                const int at = ((tid >> 2) & 15) * 40 + (tid >> 8) * 16 + ((tid >> 6) & 3) * 4 + (tid & 3);
+                s_h[at] = (uint16_t)h0;
+                s_h[kFewMaxT * 40 + at] = (uint16_t)f2bf(rest);
                 __syncthreads();
-                hf = *reinterpret_cast<const bf16x8_t *>(s_h + r * 40 + 8 * g);
+                hf[0] = *reinterpret_cast<const bf16x8_t *>(s_h + r * 40 + 8 * g);
+                hf[1] = *reinterpret_cast<const bf16x8_t *>(s_h + kFewMaxT * 40 + r * 40 + 8 * g);
             }
             FewStage<MX> &d = st[s % R];
-            if (MX) {
-                if (s < NS1) {
+            auto mfma = [](bf16x8_t w, bf16x8_t v, f32x4_t c) {
+                return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, v, c, 0, 0, 0);
+            };
+            if (s < NS1) {
 #pragma unroll
-                    for (int jj = 0; jj < 4; ++jj) {
+                for (int jj = 0; jj < (MX ? 4 : 2); ++jj) {
+                    const bf16x8_t v = MX ? xf[s < KQ ? s : 0][jj] : xf[s / 2 < KQ ? s / 2 : 0][2 * (s & 1) + (jj & 1)];
+                    if (MX) {
                         const uint32_t sw = jj == 0 ? d.v[4].x : jj == 1 ? d.v[4].y : jj == 2 ? d.v[4].z : d.v[4].w;
-                        acc1[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode(d.v[jj].x, mx_scale<0>(sw)), xf[s < NS1 ? s : 0][jj], acc1[0], 0, 0, 0);
-                        acc1[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode(d.v[jj].y, mx_scale<1>(sw)), xf[s < NS1 ? s : 0][jj], acc1[1], 0, 0, 0);
-                        acc1[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode(d.v[jj].z, mx_scale<2>(sw)), xf[s < NS1 ? s : 0][jj], acc1[2], 0, 0, 0);
-                        acc1[3] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode(d.v[jj].w, mx_scale<3>(sw)), xf[s < NS1 ? s : 0][jj], acc1[3], 0, 0, 0);
-                    }
-                } else {
+                        acc1[0] = mfma(mx_decode(d.v[jj].x, mx_scale<0>(sw)), v, acc1[0]);
+                        acc1[1] = mfma(mx_decode(d.v[jj].y, mx_scale<1>(sw)), v, acc1[1]);
+                        acc1[2] = mfma(mx_decode(d.v[jj].z, mx_scale<2>(sw)), v, acc1[2]);
+                        acc1[3] = mfma(mx_decode(d.v[jj].w, mx_scale<3>(sw)), v, acc1[3]);
+                    } else {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        f32x4_t *o = acc2[2 * (s - NS1) + h];
-                        const uint32_t sw = h == 0 ? d.v[2].x : d.v[2].y;
-                        o[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode(d.v[h].x, mx_scale<0>(sw)), hf, o[0], 0, 0, 0);
-                        o[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode(d.v[h].y, mx_scale<1>(sw)), hf, o[1], 0, 0, 0);
-                        o[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode(d.v[h].z, mx_scale<2>(sw)), hf, o[2], 0, 0, 0);
-                        o[3] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode(d.v[h].w, mx_scale<3>(sw)), hf, o[3], 0, 0, 0);
+                        for (int i = 0; i < 4; ++i)
+                            acc1[i] = mfma(__builtin_bit_cast(bf16x8_t, d.v[4 * jj + i]), v, acc1[i]);
                     }
                 }
             } else {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h) {
+                    f32x4_t *o = acc2[2 * (s - NS1) + h];
+                    bf16x8_t w[4];
+                    if (MX) {
+                        const uint32_t sw = h == 0 ? d.v[2].x : d.v[2].y;
+                        w[0] = mx_decode(d.v[h].x, mx_scale<0>(sw));
+                        w[1] = mx_decode(d.v[h].y, mx_scale<1>(sw));
+                        w[2] = mx_decode(d.v[h].z, mx_scale<2>(sw));
+                        w[3] = mx_decode(d.v[h].w, mx_scale<3>(sw));
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bf16x8_t w = __builtin_bit_cast(bf16x8_t, d.v[4 * h + i]);
-                        if (s < NS1)
-                            acc1[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xf[s < NS1 ? s >> 1 : 0][2 * (s & 1) + h], acc1[i], 0, 0, 0);
-                        else
-                            acc2[2 * (s - NS1) + h][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, hf, acc2[2 * (s - NS1) + h][i], 0, 0, 0);
+                        for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(bf16x8_t, d.v[4 * h + i]);
                     }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = mfma(w[i], hf[1], mfma(w[i], hf[0], o[i]));
+                }
             }
             // the slot is free: the stage R further on, in this chunk or the next
             if (s + R < NS) load(c, s + R, d);
@@ -348,12 +412,11 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
         }
     };
     // the sums of a piece's columns of one expert leave as one row per token
-    auto flush = [&](int u) __attribute__((always_inline)) {
-        const int e = s_list[u], seg = (int)blockIdx.x - piece_of(u * ns);
-        if (s_mask[e] >> r & 1) {
+    auto flush = [&](const Chunk &c) __attribute__((always_inline)) {
+        if (s_mask[c.e] >> r & 1) {
             int p = r * k;
-            while (s_id[p] != e) ++p;
-            float *row = a.partial + (size_t)(s_row[p] + seg) * H;
+            while (s_id[p] != c.e) ++p;
+            float *row = a.partial + (size_t)(first_row(p) + (int)blockIdx.x - piece_of(c.u * ns)) * H;
             const float w = s_w[p];
 #pragma unroll
             for (int q = 0; q < 2 * KQ; ++q) {
@@ -373,50 +436,59 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
             for (int i = 0; i < 4; ++i) acc2[q][i] = f32x4_t{};
     };
 
-    Chunk cur{nullptr, c0 / ns, c0 % ns};
-    cur.base = block_of(cur.u);
+    Chunk cur{nullptr, 0, c0 / ns, c0 % ns};
+    cur.e = expert_at(cur.u);
+    cur.base = block_of(cur.e);
 #pragma unroll
     for (int s = 0; s < R; ++s) load(cur, s, st[s]);
+    count_rows();
     for (int c = c0; c + 1 < c1; ++c) {
-        Chunk next{cur.base, cur.u, cur.j + 1};
-        if (next.j == ns) next = Chunk{block_of(cur.u + 1), cur.u + 1, 0};
+        Chunk next{cur.base, cur.e, cur.u, cur.j + 1};
+        if (next.j == ns) {
+            next = Chunk{nullptr, expert_at(cur.u + 1), cur.u + 1, 0};
+            next.base = block_of(next.e);
+        }
         chunk(cur, next, true);
-        if (next.u != cur.u) flush(cur.u);
+        if (next.u != cur.u) flush(cur);
         cur = next;
     }
     chunk(cur, cur, false);
-    flush(cur.u);
+    flush(cur);
+    if (blockIdx.x == 0) write_rows();
 }
 
 // ---------------------------------------------------------------- merge
 
-// One workgroup per token and 256 columns; eight waves take its rows in turn.
+// One workgroup per token and 64 columns: 32 quarter-waves take its rows in turn,
+// 16 bytes a lane, and are summed in order.  Bound by latency (1.6 MB of rows at
+// T = 1, 192 of them).
 __global__ __launch_bounds__(512) void few_merge_kernel(const float *__restrict__ partial,
                                                         const int32_t *__restrict__ row_base,
                                                         const uint16_t *__restrict__ add_in, int H,
                                                         uint16_t *__restrict__ out) {
-    __shared__ __attribute__((aligned(16))) float s_sum[8][256];
-    const int t = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int col = blockIdx.x * 256 + 4 * lane;
+    __shared__ float s_sum[32][65];
+    const int t = blockIdx.y, q = threadIdx.x >> 4, l = threadIdx.x & 15;
+    const int col = blockIdx.x * 64 + 4 * l;
     const int r0 = row_base[t], r1 = row_base[t + 1];
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (col < H) {
-#pragma unroll 4
-        for (int r = r0 + wave; r < r1; r += 8) {
-            const float4 p = *reinterpret_cast<const float4 *>(partial + (size_t)r * H + col);
-            v.x += p.x;
-            v.y += p.y;
-            v.z += p.z;
-            v.w += p.w;
-        }
+#pragma unroll 6
+    for (int r = r0 + q; r < r1; r += 32) {
+        const float4 p = *reinterpret_cast<const float4 *>(partial + (size_t)r * H + col);
+        v.x += p.x;
+        v.y += p.y;
+        v.z += p.z;
+        v.w += p.w;
     }
-    *reinterpret_cast<float4 *>(&s_sum[wave][4 * lane]) = v;
+    s_sum[q][4 * l] = v.x;
+    s_sum[q][4 * l + 1] = v.y;
+    s_sum[q][4 * l + 2] = v.z;
+    s_sum[q][4 * l + 3] = v.w;
     __syncthreads();
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (threadIdx.x < 256 && c < H) {
+    if (threadIdx.x < 64) {
+        const int c = blockIdx.x * 64 + threadIdx.x;
         float s = add_in ? bf2f(add_in[(size_t)t * H + c]) : 0.0f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) s += s_sum[w][threadIdx.x];
+        for (int w = 0; w < 32; ++w) s += s_sum[w][threadIdx.x];
         out[(size_t)t * H + c] = (uint16_t)f2bf(s);
     }
 }
@@ -467,7 +539,7 @@ PD_API int pdscope_moe_few(const void *x, const void *gate, const float *bias, i
     if (err == hipSuccess) err = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
     if (err != hipSuccess) return fail(kEHip, std::string("moe_few: ") + hipGetErrorString(err));
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    few_router_kernel<<<E, 256, 0, s>>>((const uint16_t *)x, (const uint16_t *)gate, T, H, E, (uint16_t *)logits);
+    few_router_kernel<<<dim3(E, (T + kRouterT - 1) / kRouterT), 256, 0, s>>>((const uint16_t *)x, (const uint16_t *)gate, T, H, E, (uint16_t *)logits);
     int rc = check_launch("few_router_kernel");
     if (rc) return rc;
     const FewArgs a{(const uint16_t *)x, (const uint16_t *)logits, bias, T, H, E, k, normalize, I,
@@ -475,7 +547,7 @@ PD_API int pdscope_moe_few(const void *x, const void *gate, const float *bias, i
                     (float *)((char *)workspace + 256)};
     rc = mxfp4 ? few_launch_experts<true>(a, cus, s) : few_launch_experts<false>(a, cus, s);
     if (rc) return rc;
-    few_merge_kernel<<<dim3((H + 255) / 256, T), 512, 0, s>>>(a.partial, a.row_base, (const uint16_t *)add_in, H,
+    few_merge_kernel<<<dim3(H / 64, T), 512, 0, s>>>(a.partial, a.row_base, (const uint16_t *)add_in, H,
                                                              (uint16_t *)out);
     return check_launch("few_merge_kernel");
 }
