@@ -411,7 +411,7 @@ int pdscope_mxfp4_pack(const void *codes, const void *scales, int n, int H, int 
  * addresses of pdscope_mxfp4_quantize's or _pack's blocks):
  *   h[r] = bf16(silu(x . gate_e^T) * (x . up_e^T)),  y[r] = bf16(h[r] . down_e^T)
  * on the weights' exact values, bf16 activations, fp32 accumulation (gate and up
- * are not rounded, unlike the bf16 path's).  block_m: 32, 64 or 128, the row tile
+ * are not rounded, unlike the bf16 path's).  block_m: 32 or 64, the row tile
  * of the schedule (pdscope_grouped_mxfp4_block_m picks it from the mean rows per
  * selected expert).  Rows of an expert without a copy keep what y holds.
  * Limits: H % 128 == 0 and I % 128 == 0; x, h_ws and y 16-byte aligned.

@@ -5,14 +5,28 @@
 //   gate/up : h[r,i] = bf16(silu(x_r . gate_i) * (x_r . up_i))
 //   down    : y[r,n] = bf16(h_r . down_n)
 //
-// Weights are the first operand of v_mfma_f32_16x16x32_bf16 and never enter LDS: a
-// wave's four waves' worth of a tile is four 64-row groups, one per wave, and a
-// group's 4352 bytes for 128 inputs go from memory to the registers that hold
-// them until they are decoded (16 conversions per lane and 16-row tile, used for
-// every token tile).  Activation rows are the second operand, shared by the four
+// Weights are the first operand of v_mfma_f32_16x16x32_bf16 and never enter LDS:
+// each wave of a tile has a 64-row group of them to itself, whose 4352 bytes for
+// 128 inputs go from memory to the registers that hold them until they are
+// decoded (16 conversions per lane and 16-row tile, used for every token tile).  Activation rows are the second operand, shared by the four
 // waves: they stream into an LDS ring by direct-to-LDS loads, gathered through
 // perm_token, in 256-byte rows whose 16-byte chunk c lies in slot c ^ (row % 16),
 // so that the 16 rows of a fragment read lie in 16 bank groups.
+//
+// Thin experts are bound by HBM (Qwen shape T=33, gate/up 6.1 TB/s).  Long
+// prompts reach 1.19 PFLOP/s in gate/up and 1.02 in down (Qwen shape T=4096, 173
+// and 101 us; a 128-row tile 185 and 108): there the matrix cores are busy for
+// 63% of the CUs' cycles, LDS for 17%, and a quarter of the waves' time is waits.
+// Measured on the 128-row tile and not kept: direct-to-LDS loads through buffer
+// descriptors, which need no address arithmetic (1-3%, and 4 GiB of activations
+// at most); weights two steps ahead (216 us); eight waves to a tile, which read
+// the activations half as often (212); the products' order fixed by scheduling
+// barriers (208).  On 64 rows: weight registers reloaded piece by piece, for a
+// third workgroup per CU (the layer 336 us against 314).
+//
+// h, and each expert's row of y before the merge, are rounded to bf16: h is the
+// matrix cores' input, and y in fp32 would be a quarter of the traffic of a long
+// prompt on top (out is off by three bf16 roundings in all, 0.3% of its norm).
 #include <type_traits>
 
 #include "mxfp4.h"
@@ -30,21 +44,21 @@ struct MxGrouped {
     uint16_t *out;  // gate/up: h [rows, I]; down: y [rows, H]
 };
 
-// bytes of a staged output row: 128 columns of h or 256 of y, off the bank line
-template <bool GATEUP>
-constexpr int kMxOutRow = (GATEUP ? 256 : 512) + 16;
-template <int BM, int S, bool GATEUP>
-constexpr int kMxLds = S * BM * 256 > BM * kMxOutRow<GATEUP> ? S * BM * 256 : BM * kMxOutRow<GATEUP>;
+// bytes of a staged output row: 32 columns of h or 64 of y per wave, off the bank line
+template <int NW, bool GATEUP>
+constexpr int kMxOutRow = NW * (GATEUP ? 64 : 128) + 16;
+template <int BM, int NW, bool GATEUP>
+constexpr int kMxLds = 2 * BM * 256 > BM * kMxOutRow<NW, GATEUP> ? 2 * BM * 256 : BM * kMxOutRow<NW, GATEUP>;
 
-// BM rows x four groups (128 h columns or 256 y columns), K in steps of 128, S
-// stages of activations.
-template <int BM, int S, bool GATEUP, int OCC>
-__global__ __launch_bounds__(256, OCC) void mx_grouped_kernel(MxGrouped p) {
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[kMxLds<BM, S, GATEUP>];
-    constexpr int TM = BM / 16, PF = 2;
+// BM rows x four groups (128 h columns or 256 y columns), K in steps of 128, two
+// stages of activations; OCC workgroups per CU.
+template <int BM, int NW, bool GATEUP, int OCC>
+__global__ __launch_bounds__(64 * NW, OCC * NW / 4) void mx_grouped_kernel(MxGrouped p) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kMxLds<BM, NW, GATEUP>];
+    constexpr int TM = BM / 16;
     const int H = p.H, I = p.I;
     const int K = GATEUP ? H : I, KT = K / kGroupIn;
-    const int groups = GATEUP ? I / 32 : H / kGroupRows, NT = (groups + 3) / 4;
+    const int groups = GATEUP ? I / 32 : H / kGroupRows, NT = (groups + NW - 1) / NW;
 
     // ---- tile: eight contiguous pieces of the list, one per XCD, columns fastest
     const int total = p.tile_start[p.nsel] * NT;
@@ -68,18 +82,20 @@ __global__ __launch_bounds__(256, OCC) void mx_grouped_kernel(MxGrouped p) {
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
-    const int rg = nt * 4 + wave;             // this wave's row group
+    const int rg = nt * NW + wave;            // this wave's row group
     const int rg_in = min(rg, groups - 1);    // past the end: read the last one, store nothing
     const uint8_t *const wbase =
         base + ((GATEUP ? 0 : mx_gateup_groups(H, I)) + (size_t)rg_in * KT) * kGroupBytes;
 
-    // ---- activation loads: load q of wave w fills rows 16 q + 4 w .. + 3; lane l
+    // ---- activation loads: load q of wave w fills rows 4 (NW q + w) .. + 3; lane l
     // takes row + l / 16 and the chunk that belongs in its slot
-    uint32_t arow[TM];
-    const uint32_t achunk = (uint32_t)((lane & 15) ^ (4 * wave + (lane >> 4)));
+    constexpr int RQ = 4 * NW, AL = BM / RQ;  // rows per load of all waves, loads of a wave
+    static_assert(RQ % 16 == 0 && AL * RQ == BM, "activation loads");
+    uint32_t arow[AL];
+    const uint32_t achunk = (uint32_t)((lane & 15) ^ ((4 * wave + (lane >> 4)) & 15));
 #pragma unroll
-    for (int q = 0; q < TM; ++q) {
-        const int row = min(m0 + 16 * q + 4 * wave + (lane >> 4), row_end - 1);
+    for (int q = 0; q < AL; ++q) {
+        const int row = min(m0 + RQ * q + 4 * wave + (lane >> 4), row_end - 1);
         arow[q] = (uint32_t)(GATEUP ? p.perm_token[row] : row) * (uint32_t)(K / 8) + achunk;
     }
     const uint8_t *const abase = reinterpret_cast<const uint8_t *>(p.a);
@@ -92,86 +108,75 @@ __global__ __launch_bounds__(256, OCC) void mx_grouped_kernel(MxGrouped p) {
 
     auto kloop = [&](auto live) __attribute__((always_inline)) {
         constexpr int L = decltype(live)::value;  // token tiles with rows of the expert
-        // loads that follow those of stage kt by the time it is needed: the weights
-        // of its own step (all PF of them for the first stages, whose steps lie in
-        // the prologue), and both kinds of the S - 2 steps between
-        constexpr int YOUNGER = (S - 2) * L + 5 * (S - 1 < PF ? S - 1 : PF);
         auto issue_a = [&](int kt) __attribute__((always_inline)) {
-            uint8_t *st = smem + (kt % S) * (BM * 256);
+            uint8_t *st = smem + (kt & 1) * (BM * 256);
 #pragma unroll
-            for (int q = 0; q < L; ++q) {
+            for (int q = 0; q < (16 * L + RQ - 1) / RQ; ++q) {
                 uint32_t o = arow[q];
                 opaque(o);
                 load_lds16(reinterpret_cast<const uint16_t *>(abase + kt * 256 + (size_t)o * 16),
-                           st + (16 * q + 4 * wave) * 256);
+                           st + (RQ * q + 4 * wave) * 256);
             }
         };
-        uint4 w[PF][5];
         auto issue_w = [&](int kt, uint4 (&d)[5]) __attribute__((always_inline)) {
             const uint8_t *b = wbase + (size_t)kt * kGroupBytes;
 #pragma unroll
             for (int jj = 0; jj < 4; ++jj) d[jj] = ld_g(b + jj * 1024 + lane * 16);
             d[4] = ld_g(b + kGroupScales + r * 16);
         };
-        auto step = [&](int kt, uint4 (&d)[5], auto steady) __attribute__((always_inline)) {
-            constexpr bool STEADY = decltype(steady)::value;
-            // this wave's share of stage kt has landed; with the barrier, everyone's
-            if (STEADY) wait_vm<YOUNGER>();
-            else wait_vm<0>();
+        // Step kt: everything asked for in step kt - 1 has landed (the one wait of
+        // the step: loads to registers and to LDS complete in one order that the
+        // compiler does not count through, so any wait of its own would be for
+        // all of them, and here none is younger than a whole step); then ask for
+        // kt + 1 and run the products of kt from d.
+        auto step = [&](int kt, uint4 (&d)[5], uint4 (&next)[5]) __attribute__((always_inline)) {
+            wait_vm<0>();
             ring_barrier();
-            if (STEADY || kt + S - 1 < KT) issue_a(kt + S - 1);
-            // the count above needs these loads ahead of the weights' that follow
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
-            const uint8_t *st = smem + (kt % S) * (BM * 256);
+            if (kt + 1 < KT) {
+                issue_a(kt + 1);
+                issue_w(kt + 1, next);
+            }
+            const uint8_t *st = smem + (kt & 1) * (BM * 256) + r * 256;
+            bf16x8_t x[2][L];
+            auto read_piece = [&](int jj) __attribute__((always_inline)) {
+#pragma unroll
+                for (int m = 0; m < L; ++m)
+                    x[jj & 1][m] = *reinterpret_cast<const bf16x8_t *>(st + m * 4096 + (((4 * jj + g) ^ r) << 4));
+            };
+            read_piece(0);
 #pragma unroll
             for (int jj = 0; jj < 4; ++jj) {
+                if (jj < 3) read_piece(jj + 1);
                 const uint32_t sw = jj == 0 ? d[4].x : jj == 1 ? d[4].y : jj == 2 ? d[4].z : d[4].w;
-                const bf16x8_t w0 = mx_decode(d[jj].x, mx_scale<0>(sw)), w1 = mx_decode(d[jj].y, mx_scale<1>(sw));
-                const bf16x8_t w2 = mx_decode(d[jj].z, mx_scale<2>(sw)), w3 = mx_decode(d[jj].w, mx_scale<3>(sw));
+                const bf16x8_t w[4] = {mx_decode(d[jj].x, mx_scale<0>(sw)), mx_decode(d[jj].y, mx_scale<1>(sw)),
+                                       mx_decode(d[jj].z, mx_scale<2>(sw)), mx_decode(d[jj].w, mx_scale<3>(sw))};
 #pragma unroll
-                for (int m = 0; m < L; ++m) {
-                    const bf16x8_t x =
-                        *reinterpret_cast<const bf16x8_t *>(st + (16 * m + r) * 256 + (((4 * jj + g) ^ r) << 4));
-                    acc[0][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w0, x, acc[0][m], 0, 0, 0);
-                    acc[1][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w1, x, acc[1][m], 0, 0, 0);
-                    acc[2][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w2, x, acc[2][m], 0, 0, 0);
-                    acc[3][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w3, x, acc[3][m], 0, 0, 0);
-                }
+                for (int m = 0; m < L; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[i][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i], x[jj & 1][m], acc[i][m], 0, 0, 0);
             }
-            if (STEADY || kt + PF < KT) issue_w(kt + PF, d);
         };
-#pragma unroll
-        for (int s = 0; s < S - 1; ++s)
-            if (s < KT) issue_a(s);
-#pragma unroll
-        for (int s = 0; s < PF; ++s)
-            if (s < KT) issue_w(s, w[s]);
-        int kt = 0;
-        for (; kt + 1 + (S - 1 > PF ? S - 1 : PF) < KT; kt += 2) {
-            step(kt, w[0], std::true_type{});
-            step(kt + 1, w[1], std::true_type{});
-        }
-        for (; kt < KT; kt += 2) {
-            step(kt, w[0], std::false_type{});
-            if (kt + 1 < KT) step(kt + 1, w[1], std::false_type{});
+        uint4 w0[5], w1[5];
+        issue_w(0, w0);
+        issue_a(0);
+        for (int kt = 0; kt < KT; kt += 2) {
+            step(kt, w0, w1);
+            if (kt + 1 < KT) step(kt + 1, w1, w0);
         }
     };
-    // whole quarters of the tile that hold rows
+    // one straight-line loop for each number of 16-row tiles that hold rows
     const int live = (min(BM, row_end - m0) + 15) / 16;
-    if constexpr (TM >= 4) {
-        if (4 * live <= TM) kloop(std::integral_constant<int, TM / 4>{});
-        else if (2 * live <= TM) kloop(std::integral_constant<int, TM / 2>{});
-        else if (4 * live <= 3 * TM) kloop(std::integral_constant<int, 3 * TM / 4>{});
-        else kloop(std::integral_constant<int, TM>{});
-    } else {
-        if (live == 1) kloop(std::integral_constant<int, 1>{});
-        else kloop(std::integral_constant<int, TM>{});
+    if (live == 1) kloop(std::integral_constant<int, 1>{});
+    else if (live == 2) kloop(std::integral_constant<int, 2>{});
+    else if constexpr (TM == 4) {
+        if (live == 3) kloop(std::integral_constant<int, 3>{});
+        else kloop(std::integral_constant<int, 4>{});
     }
 
     // ---- epilogue: a lane holds token row r of each tile and weight rows 4 g ..
     // + 3 of each 16-row tile; through LDS, out in whole-row 16-byte stores
-    constexpr int OB = kMxOutRow<GATEUP>;
+    constexpr int OB = kMxOutRow<NW, GATEUP>;
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
@@ -188,10 +193,10 @@ __global__ __launch_bounds__(256, OCC) void mx_grouped_kernel(MxGrouped p) {
         }
     }
     __syncthreads();
-    constexpr int CO = GATEUP ? 128 : 256, CH = CO / 8;
+    constexpr int CO = NW * (GATEUP ? 32 : 64), CH = CO / 8;
     const int ldo = GATEUP ? I : H, cols = min(CO, ldo - nt * CO);  // cols % 64 == 0
     const int rows = min(BM, row_end - m0);
-    for (int c = tid; c < rows * CH; c += 256) {
+    for (int c = tid; c < rows * CH; c += 64 * NW) {
         const int row = c / CH, ch = c % CH;
         if (ch * 8 < cols)
             st_through(p.out + (size_t)(m0 + row) * ldo + nt * CO + ch * 8,
@@ -209,14 +214,15 @@ struct MxCall {
     hipStream_t s;
 };
 
-template <int BM, int S, int OCC>
+// NWG / NWD waves and OCCG / OCCD workgroups per CU of the gate/up and down halves
+template <int BM, int NWG, int OCCG, int NWD, int OCCD>
 static int mx_grouped_launch(const MxCall &c, const uint16_t *x, const int32_t *perm, uint16_t *h, uint16_t *y) {
     auto grid = [&](int nt) { return (unsigned)(((size_t)c.max_tiles * nt + 7) / 8 * 8); };
-    mx_grouped_kernel<BM, S, true, OCC><<<grid(c.I / 128), 256, 0, c.s>>>(
+    mx_grouped_kernel<BM, NWG, true, OCCG><<<grid((c.I / 32 + NWG - 1) / NWG), 64 * NWG, 0, c.s>>>(
         MxGrouped{x, perm, c.offsets, c.sel, c.nsel, c.tile_start, c.slots, c.H, c.I, h});
     const int rc = check_launch("mx_grouped_kernel<gateup>");
     if (rc) return rc;
-    mx_grouped_kernel<BM, S, false, OCC><<<grid((c.H / kGroupRows + 3) / 4), 256, 0, c.s>>>(
+    mx_grouped_kernel<BM, NWD, false, OCCD><<<grid((c.H / kGroupRows + NWD - 1) / NWD), 64 * NWD, 0, c.s>>>(
         MxGrouped{h, nullptr, c.offsets, c.sel, c.nsel, c.tile_start, c.slots, c.H, c.I, y});
     return check_launch("mx_grouped_kernel<down>");
 }
@@ -225,7 +231,12 @@ static int mx_grouped_launch(const MxCall &c, const uint16_t *x, const int32_t *
 
 using namespace pd;
 
-PD_API int pdscope_grouped_mxfp4_block_m(int rows_hint) { return rows_hint <= 16 ? 32 : rows_hint <= 44 ? 64 : 128; }
+// Layers of the Qwen shape on 32 and 64 rows: 2 mean rows 66.0 and 69.1 us, 16
+// 78.5 and 81.3, 32 105.0 and 90.0, 64 129 and 121, 256 347 and 299 (DeepSeek-V2-
+// Lite shape, 3 mean rows 68.5 and 66.4, 24 81.0 and 75.3).  A 128-row tile, whose
+// weights are decoded once for twice the rows, is no faster anywhere (256 mean
+// rows 322 against 314 then).
+PD_API int pdscope_grouped_mxfp4_block_m(int rows_hint) { return rows_hint <= 16 ? 32 : 64; }
 
 PD_API int pdscope_swiglu_grouped_mxfp4(const void *x, const int32_t *perm_token, const int32_t *offsets,
                                         const int32_t *sel, int nsel, const int32_t *tile_start, int max_tiles,
@@ -235,8 +246,7 @@ PD_API int pdscope_swiglu_grouped_mxfp4(const void *x, const int32_t *perm_token
         return fail(kEInval, "grouped_mxfp4: null pointer");
     if (nsel < 1 || max_tiles < 1 || max_tiles > (1 << 22))
         return fail(kEInval, "grouped_mxfp4: need nsel >= 1 and 1 <= max_tiles <= 4194304");
-    if (block_m != 32 && block_m != 64 && block_m != 128)
-        return fail(kEInval, "grouped_mxfp4: block_m must be 32, 64 or 128");
+    if (block_m != 32 && block_m != 64) return fail(kEInval, "grouped_mxfp4: block_m must be 32 or 64");
     if (!mx_shape_ok(H, I) || H > 65536 || I > 65536)
         return fail(kEInval, "grouped_mxfp4: need H % 128 == 0 and I % 128 == 0 (at most 65536)");
     for (const void *p : {x, (const void *)h_ws, (const void *)y})
@@ -245,7 +255,11 @@ PD_API int pdscope_swiglu_grouped_mxfp4(const void *x, const int32_t *perm_token
                    reinterpret_cast<hipStream_t>(stream)};
     auto *xs = (const uint16_t *)x;
     auto *h = (uint16_t *)h_ws, *out = (uint16_t *)y;
-    if (block_m == 32) return mx_grouped_launch<32, 4, 2>(c, xs, perm_token, h, out);
-    if (block_m == 64) return mx_grouped_launch<64, 3, 2>(c, xs, perm_token, h, out);
-    return mx_grouped_launch<128, 2, 2>(c, xs, perm_token, h, out);
+    // 32 rows: bound by the weight stream.  gate/up on four waves, four workgroups
+    // per CU; down (a short K loop) on eight, two per CU: fewer, wider workgroups
+    // read each expert's h fewer times (Qwen shape T=33, gate/up 31.0 us = 6.1
+    // TB/s, eight waves 32.8; down 17.5, four waves 20.6).  64 rows: four waves,
+    // two workgroups per CU, whose steps interleave.
+    if (block_m == 32) return mx_grouped_launch<32, 4, 4, 8, 2>(c, xs, perm_token, h, out);
+    return mx_grouped_launch<64, 4, 2, 4, 2>(c, xs, perm_token, h, out);
 }

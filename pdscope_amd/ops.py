@@ -721,7 +721,7 @@ def grouped_mxfp4_block_m(rows_hint: int) -> int:
 
 
 def swiglu_grouped_mxfp4(x, perm_token, offsets, sel, tile_start, max_tiles, block_m, slots, H, I, h_ws, y):
-    """swiglu_grouped over the 4-bit blocks in `slots`; block_m 32, 64 or 128."""
+    """swiglu_grouped over the 4-bit blocks in `slots`; block_m 32 or 64."""
     _need(x, "inputs", BF16, 2)
     dev = x.device
     for t, n in ((perm_token, "perm_token"), (offsets, "offsets"), (sel, "sel"), (tile_start, "tile_start")):

@@ -45,7 +45,7 @@ def test_experts_of_a_prompt(T, H, I, E, k):
     check(out, x, ids, w, blocks, H, I)
 
 
-@pytest.mark.parametrize("block_m", [32, 64, 128])
+@pytest.mark.parametrize("block_m", [32, 64])
 @pytest.mark.parametrize("T,used", [(5, 2), (130, 2), (257, 5), (515, 9)])
 def test_every_row_tile_and_merge(block_m, T, used):
     """Experts of 1 to several hundred rows on each tile height: full tiles, every fill of
@@ -64,7 +64,7 @@ def test_every_row_tile_and_merge(block_m, T, used):
 def test_rows_counts_of_one_expert():
     """One expert with every count of rows around the tiles' edges."""
     H, I = 256, 128
-    for block_m in (32, 64, 128):
+    for block_m in (32, 64):
         for T in (1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 97, 113, 127, 128, 129):
             x, ids, w, blocks, slots = make(T, H, I, 1, 1, seed=T)
             ws = layer.MoEWorkspace(T, H, I, 1, 1, DEV)
@@ -169,7 +169,7 @@ def test_refusals():
     with pytest.raises(ValueError, match="representation"):
         layer.experts_resident(x, ids, w, slots, ws, representation="fp8")
     with pytest.raises(ValueError, match="block_m"):
-        layer.experts_resident(x, ids, w, slots, ws, block_m=256, representation="mxfp4")
+        layer.experts_resident(x, ids, w, slots, ws, block_m=128, representation="mxfp4")
     with pytest.raises(ValueError, match="add_in"):
         layer.experts_resident(x, ids, w, slots, ws, shared_slot=slots[:1], representation="mxfp4")
     with pytest.raises(ValueError, match="H % 128"):
