@@ -17,6 +17,9 @@
 // tokens, which goes to memory in fp32 (a row per token, expert and piece:
 // 1.6 MB against 21 MB of 4-bit weights at T = 1) and is summed in a fixed order
 // by the merge.
+#include <algorithm>
+#include <type_traits>
+
 #include "mxfp4.h"
 #include "topk.h"
 
@@ -26,7 +29,7 @@ constexpr int kFewMaxT = 16;
 constexpr int kFewMaxE = 256;
 constexpr int kFewMaxK = 16;
 constexpr int kFewMaxH = 4096;
-constexpr int kFewChunk = 32;  // I columns of a chunk: one 64-row group of gate/up
+constexpr int kFewChunk = 32;  // I columns of a chunk: one 64-row group of gate/up (I % 128 == 0: an even number of them)
 
 // 16 bytes at a uniform address plus a lane's offset (one scalar pair and one
 // register for the address), not kept in the caches: weights are read once.
@@ -42,8 +45,8 @@ __device__ __forceinline__ uint4 ld_keep(const uint8_t *base, uint32_t off) {
 }
 
 struct FewArgs {
-    const uint16_t *x, *logits;
-    const float *bias;
+    const uint16_t *x;
+    const int *keys;  // [T, E] order_key of logit + bias
     int T, H, E, k, normalize, I;
     const uint8_t *const *slots;
     int32_t *ids;
@@ -53,6 +56,17 @@ struct FewArgs {
 };
 
 // ---------------------------------------------------------------- router
+
+// An integer in the order of v (-0 is 0).  A NaN comes last, so that a token of NaN
+// takes experts 0 .. k-1 (with NaN weights); kNoKey is behind every value.
+constexpr int kNoKey = (int)0x80000000, kNanKey = kNoKey + 1;
+__device__ __forceinline__ int order_key(float v) {
+    const int bits = __float_as_int(v + 0.0f);
+    return v == v ? bits ^ ((bits >> 31) & 0x7fffffff) : kNanKey;
+}
+__device__ __forceinline__ float key_value(int key) {
+    return key == kNanKey ? __int_as_float(0x7fc00000) : __int_as_float(key ^ ((key >> 31) & 0x7fffffff));
+}
 
 // The same double of lane l ^ 32 / l ^ 16 (in one of the two results; the other
 // is the lane's own) and of a lane N further around its row of 16.
@@ -90,8 +104,9 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // (fp64 runs at the rate of fp32 here), a store.
 constexpr int kRouterT = 4;
 __global__ __launch_bounds__(256) void few_router_kernel(const uint16_t *__restrict__ x,
-                                                         const uint16_t *__restrict__ gate, int T, int H, int E,
-                                                         uint16_t *__restrict__ logits) {
+                                                         const uint16_t *__restrict__ gate,
+                                                         const float *__restrict__ bias, int T, int H, int E,
+                                                         uint16_t *__restrict__ logits, int *__restrict__ keys) {
     __shared__ double s_sum[4][kRouterT];
     const int e = blockIdx.x, t0 = blockIdx.y * kRouterT, tid = threadIdx.x, wave = tid >> 6;
     const int nt = min(kRouterT, T - t0);  // uniform
@@ -122,12 +137,22 @@ __global__ __launch_bounds__(256) void few_router_kernel(const uint16_t *__restr
             if ((tid & 63) == 0) s_sum[wave][q] = acc[q];
         }
     __syncthreads();
-    if (tid < nt)
-        logits[(size_t)(t0 + tid) * E + e] =
-            (uint16_t)f2bf((float)((s_sum[0][tid] + s_sum[1][tid]) + (s_sum[2][tid] + s_sum[3][tid])));
+    if (tid < nt) {
+        const uint32_t v = f2bf((float)((s_sum[0][tid] + s_sum[1][tid]) + (s_sum[2][tid] + s_sum[3][tid])));
+        logits[(t0 + tid) * E + e] = (uint16_t)v;
+        keys[(t0 + tid) * E + e] = order_key(bf2f(v) + (bias ? bias[e] : 0.0f));
+    }
 }
 
 // ---------------------------------------------------------------- experts
+
+// a / b for 0 <= a < 2^22, 0 < b: the quotient in floats is off by one at most.
+__device__ __forceinline__ int small_div(int a, int b) {
+    int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+    const int rest = a - q * b;
+    q += rest >= b;
+    return q - (rest < 0);
+}
 
 // One stage of a wave's weight stream.  4-bit: a 64 x 128 group of gate/up (four
 // pieces of codes and their scales) or one 32-input piece of two groups of
@@ -145,7 +170,6 @@ template <bool MX, int KQ>
 __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
     __shared__ __attribute__((aligned(16))) float s_part[8 * 4 * 64 * 4];  // 32 KB; the logits before that
     __shared__ __attribute__((aligned(16))) uint16_t s_h[2 * kFewMaxT * 40];  // h and its rest; rows of 32, 80 bytes apart
-    __shared__ TopkScratch s_tk[8];
     __shared__ int s_id[256], s_first[256], s_mask[256];
     __shared__ float s_w[256];
     __shared__ int s_rows[4];
@@ -154,7 +178,16 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
     const int T = a.T, H = a.H, E = a.E, k = a.k, I = a.I;
     const int r = lane & 15, g = lane >> 4;
 
-    // ---- the tokens' activations as the second operand of every gate/up product
+    // ---- everything the routing reads, then the tokens' activations as the second
+    // operand of every gate/up product (loads complete in order: these are waited
+    // for where they are used, behind the routing)
+    int *const s_key = reinterpret_cast<int *>(s_part);
+    const int n_keys = T * E;
+    uint4 key4[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (4 * (tid + 512 * i) < n_keys) key4[i] = ld_g(a.keys + 4 * (tid + 512 * i));
+    const uint8_t *slot = tid < E ? a.slots[tid] : nullptr;
     const int KG = H / kGroupIn, HG = H / kGroupRows;
     bf16x8_t xf[KQ][4];
 #pragma unroll
@@ -164,38 +197,70 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
             const int kg = wave + 8 * q;
             xf[q][jj] = bf16x8_t{};
             if (kg < KG)
-                xf[q][jj] = *reinterpret_cast<const bf16x8_t *>(a.x + (size_t)min(r, T - 1) * H + kg * kGroupIn +
-                                                                32 * jj + 8 * g);
+                xf[q][jj] = *reinterpret_cast<const bf16x8_t *>(a.x + (uint32_t)(min(r, T - 1) * H + kg * kGroupIn +
+                                                                                 32 * jj + 8 * g));
         }
-
-    // ---- routing, by every workgroup for itself (everything it reads was asked
-    // for above or here at once; one barrier before and one behind the selection)
-    for (int i = tid; i < T * E; i += 512) s_part[i] = bf2f(a.logits[i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (4 * (tid + 512 * i) < n_keys) *reinterpret_cast<uint4 *>(s_key + 4 * (tid + 512 * i)) = key4[i];
     if (tid < 256) {
         s_mask[tid] = 0;
-        s_base[tid] = tid < E ? a.slots[tid] : nullptr;
+        s_base[tid] = slot;
     }
     __syncthreads();
-    for (int t = wave; t < T; t += 8) {
-        TopkScratch *sc = s_tk + wave;
-        if (E <= 64) topk_token<1>(s_part + t * E, a.bias, E, k, a.normalize, t, nullptr, nullptr, nullptr, sc);
-        else if (E <= 128) topk_token<2>(s_part + t * E, a.bias, E, k, a.normalize, t, nullptr, nullptr, nullptr, sc);
-        else topk_token<4>(s_part + t * E, a.bias, E, k, a.normalize, t, nullptr, nullptr, nullptr, sc);
-        if (lane < k) {
-            // a token whose largest logit is not finite has no probabilities
-            // (all NaN): it takes experts 0 .. k-1 with NaN weights
-            const float p = sc->selp[lane];
-            const int id = p == p ? sc->seli[lane] : lane;
-            const uint16_t w = sc->selw[lane];
-            s_id[t * k + lane] = id;
-            s_w[t * k + lane] = bf2f(w);
-            if (s_base[id]) atomicOr(&s_mask[id], 1 << t);  // the tokens of each expert that has a copy
-            if (blockIdx.x == 0) {
-                a.ids[t * k + lane] = id;
-                a.weights[t * k + lane] = w;
+
+    // ---- selection, by every workgroup for itself: the k largest keys of a token,
+    // equal ones by their expert
+    auto picked = [&](int t, int rank, int e) __attribute__((always_inline)) {
+        s_id[t * k + rank] = e;
+        if (s_base[e]) atomicOr(&s_mask[e], 1 << t);  // the tokens of each expert that has a copy
+    };
+    if (n_keys <= 512) {
+        // A lane (or up to eight neighbouring ones) per token and expert counts the
+        // experts ahead of it: no step waits for another.  One token of 128
+        // experts: SEL_RANK against SEL_ROUNDS by rounds.
+        int parts = 1;
+        int shift = 0;
+        while (parts < 8 && 2 * parts * n_keys <= 512) parts *= 2, ++shift;
+        const int pair = min(tid >> shift, n_keys - 1), part = tid & (parts - 1);
+        const int t = small_div(pair, E), e = pair - t * E;
+        const int *row = s_key + t * E;
+        const int mine = row[e];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = part; j < E; j += parts) rank += row[j] >= mine + (j >= e);
+        if (parts > 1) rank += __builtin_amdgcn_mov_dpp(rank, 0xb1, 0xf, 0xf, true);   // lanes ^ 1
+        if (parts > 2) rank += __builtin_amdgcn_mov_dpp(rank, 0x4e, 0xf, 0xf, true);   // lanes ^ 2
+        if (parts > 4) rank += __builtin_amdgcn_mov_dpp(rank, 0x141, 0xf, 0xf, true);  // lane i with 7 - i
+        if (tid < n_keys * parts && part == 0 && rank < k) picked(t, rank, e);
+    } else {
+        // a wave per token: the largest of those left, k times
+        auto rounds = [&](auto j_c) __attribute__((always_inline)) {
+            constexpr int J = decltype(j_c)::value;
+            for (int t = wave; t < T; t += 8) {
+                int key[J];
+#pragma unroll
+                for (int j = 0; j < J; ++j) key[j] = 64 * j + lane < E ? s_key[t * E + 64 * j + lane] : kNoKey;
+                for (int i = 0; i < k; ++i) {
+                    int most = key[0];
+#pragma unroll
+                    for (int j = 1; j < J; ++j) most = max(most, key[j]);
+                    most = dpp_max_i32(most);
+                    int e = -1;
+#pragma unroll
+                    for (int j = 0; j < J; ++j) {
+                        const uint64_t at = __ballot(key[j] == most);
+                        if (e < 0 && at) e = 64 * j + __builtin_ctzll(at);
+                    }
+#pragma unroll
+                    for (int j = 0; j < J; ++j) key[j] = 64 * j + lane == e ? kNoKey : key[j];
+                    if (lane == 0) picked(t, i, e);
+                }
             }
-        }
-        wave_lds_sync();  // before the next token overwrites the scratch
+        };
+        if (E <= 64) rounds(std::integral_constant<int, 1>{});
+        else if (E <= 128) rounds(std::integral_constant<int, 2>{});
+        else rounds(std::integral_constant<int, 4>{});
     }
     __syncthreads();
     // The list: these experts in ascending order, as four 64-bit masks that every
@@ -228,11 +293,22 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
         }
         return pos;
     };
-    const int ns = I / kFewChunk, n = __builtin_amdgcn_readfirstlane(total) * ns;
-    const int G = min((int)gridDim.x, n);  // pieces: every one has a chunk
-    // piece b takes chunks [b n / G, (b + 1) n / G); the piece of chunk c:
-    auto piece_of = [&](int c) { return (int)(((int64_t)(c + 1) * G - 1) / n); };
-    // A partial row for every token, expert of it and piece of that expert, in
+    // n pairs of chunks (ns of them an expert) in G pieces, each for the two
+    // workgroups of one XCD that stand next to each other there (block b runs on
+    // XCD b % 8): one takes the first chunk of every pair and the other the
+    // second, at about the same time, so that the 128-byte lines of the down
+    // matrix that hold both (bf16: 64 bytes of a row each) come from HBM once.
+    const int ns = I / (2 * kFewChunk), n = __builtin_amdgcn_readfirstlane(total) * ns;
+    const int b = blockIdx.x, pairs = gridDim.x / 2, G = min(pairs, n);
+    const bool by_xcd = gridDim.x % 16 == 0;
+    const int piece = by_xcd ? (b & 7) + 8 * (b >> 4) : b >> 1, second = by_xcd ? b >> 3 & 1 : b & 1;
+    // the first `longer` pieces take per + 1 pairs, the others per
+    const int per = n >= pairs ? __builtin_amdgcn_readfirstlane(small_div(n, pairs)) : 1, longer = n - per * G;
+    auto piece_of = [&](int c) {  // of pair c
+        const int in_longer = longer * (per + 1);
+        return c < in_longer ? small_div(c, per + 1) : longer + small_div(c - in_longer, per);
+    };
+    // A partial row for every token, expert of it and workgroup of that expert, in
     // the order of the (token, slot) pairs: s_first counts within 64 pairs, s_rows
     // the 64s.  Read behind the barriers of the first chunk.
     auto count_rows = [&]() __attribute__((always_inline)) {
@@ -240,7 +316,7 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
         int rows = 0;
         if (tid < T * k && s_mask[s_id[tid]] != 0) {
             const int u = place_of(s_id[tid]);
-            rows = piece_of((u + 1) * ns - 1) - piece_of(u * ns) + 1;
+            rows = 2 * (piece_of((u + 1) * ns - 1) - piece_of(u * ns) + 1);
         }
         int incl = rows;
 #pragma unroll
@@ -256,17 +332,40 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
         for (int w = 0; w < p >> 6; ++w) v += s_rows[w];
         return v;
     };
+    // One wave per token: the softmax's sum over the chosen experts (or all of
+    // them) and the weights of its slots.
+    auto weigh = [&]() __attribute__((always_inline)) {
+        for (int t = wave; t < T; t += 8) {
+            const int *row = s_key + t * E;
+            const float top = key_value(row[s_id[t * k]]);
+            const float ex = lane < k ? expf(key_value(row[s_id[t * k + lane]]) - top) : 0.0f;
+            float sum = ex;
+            if (!a.normalize) {
+                sum = 0.0f;
+                for (int e = lane; e < E; e += 64) sum += expf(key_value(row[e]) - top);
+            }
+            const uint16_t w = (uint16_t)f2bf(ex / wave_sum_dpp(sum));
+            if (lane < k) {
+                s_w[t * k + lane] = bf2f(w);
+                if (b == 0) {
+                    a.ids[t * k + lane] = s_id[t * k + lane];
+                    a.weights[t * k + lane] = w;
+                }
+            }
+        }
+    };
     auto write_rows = [&]() __attribute__((always_inline)) {  // for the merge
         if (tid < T) a.row_base[tid] = first_row(tid * k);
         if (tid == T) a.row_base[T] = s_rows[0] + s_rows[1] + s_rows[2] + s_rows[3];
     };
-    if (G == 0 && blockIdx.x == 0) {  // no expert has a copy
+    if (n == 0 && b == 0) {  // no expert has a copy
+        weigh();
         count_rows();
         __syncthreads();
         write_rows();
     }
-    if ((int)blockIdx.x >= G) return;
-    const int c0 = (int)((int64_t)blockIdx.x * n / G), c1 = (int)((int64_t)(blockIdx.x + 1) * n / G);
+    if (piece >= G) return;
+    const int c0 = piece * per + min(piece, longer), c1 = c0 + per + (piece < longer);
 
     // ---- the weight stream: per chunk NS1 stages of gate/up, then KQ of down, in
     // a ring of R; R divides the stages of a chunk, so that every register is
@@ -288,42 +387,42 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
         const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
         return reinterpret_cast<const uint8_t *>((uint64_t)hi << 32 | lo);
     };
+    // Offsets in a block (32 bits: the launch refuses larger ones): a lane's part,
+    // this wave's groups, and per chunk one product.
     const uint32_t lane16 = lane * 16, row16 = r * 16;
     const uint32_t in_gu = ((uint32_t)r * H + 8 * g) * 2, in_down = ((uint32_t)r * I + 8 * g) * 2;
+    const uint32_t gu_chunk = MX ? (uint32_t)KG * kGroupBytes : 64u * H;  // between chunks of gate/up
+    const uint32_t down0 = MX ? (uint32_t)mx_gateup_groups(H, I) * kGroupBytes : 4u * I * H;
+    const uint32_t down_group = MX ? (uint32_t)(I / kGroupIn) * kGroupBytes : 128u * I;
     auto load = [&](const Chunk &c, int s, FewStage<MX> &d) __attribute__((always_inline)) {
-        if (MX) {
-            if (s < NS1) {
-                const uint8_t *p = c.base + ((size_t)c.j * KG + min(wave + 8 * s, KG - 1)) * kGroupBytes;
+        if (s < NS1) {
+            const uint32_t kg = min(wave + 8 * (MX ? s : s >> 1), KG - 1);
+            const uint8_t *p = c.base + (c.j * gu_chunk + kg * (MX ? kGroupBytes : 2 * kGroupIn));
+            if (MX) {
 #pragma unroll
                 for (int jj = 0; jj < 4; ++jj) d.v[jj] = ld_stream(p + jj * 1024, lane16);
                 d.v[4] = ld_stream(p + kGroupScales, row16);
             } else {
-                const uint8_t *down = c.base + mx_gateup_groups(H, I) * kGroupBytes;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int grp = min(wave + 8 * (2 * (s - NS1) + h), HG - 1);
-                    const uint8_t *p = down + ((size_t)grp * (I / kGroupIn) + (c.j >> 2)) * kGroupBytes;
+                for (int i = 0; i < 4; ++i) {
+                    const uint8_t *q = p + ((uint32_t)(i >> 1) * I + 16 * (i & 1)) * 2u * H + 128 * (s & 1);
+                    d.v[i] = ld_stream(q, in_gu);
+                    d.v[4 + i] = ld_stream(q + 64, in_gu);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t grp = min(wave + 8 * (2 * (s - NS1) + h), HG - 1);
+                const uint8_t *p = c.base + (down0 + grp * down_group + (MX ? (c.j >> 2) * kGroupBytes : 64 * c.j));
+                if (MX) {
                     d.v[h] = ld_stream(p + (c.j & 3) * 1024, lane16);
                     const uint32_t w = *(const __attribute__((address_space(1))) uint32_t *)((const g_u8_t *)(p + kGroupScales + (c.j & 3) * 4) + row16);
                     if (h == 0) d.v[2].x = w;
                     else d.v[2].y = w;
-                }
-            }
-        } else {
-            if (s < NS1) {
-                const uint8_t *p = c.base + ((size_t)32 * c.j * H + min(wave + 8 * (s >> 1), KG - 1) * kGroupIn) * 2;
+                } else {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        d.v[4 * h + i] = ld_stream(p + ((size_t)((i >> 1) * I + 16 * (i & 1)) * H + 32 * (2 * (s & 1) + h)) * 2, in_gu);
-            } else {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int grp = min(wave + 8 * (2 * (s - NS1) + h), HG - 1);
-                    const uint8_t *p = c.base + ((size_t)2 * I * H + (size_t)grp * 64 * I + 32 * c.j) * 2;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) d.v[4 * h + i] = ld_keep(p + (size_t)32 * i * I, in_down);
+                    for (int i = 0; i < 4; ++i) d.v[4 * h + i] = ld_keep(p + (uint32_t)(32 * i) * I, in_down);
                 }
             }
         }
@@ -411,13 +510,21 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
             else if (more) load(next, s + R - NS, d);
         }
     };
-    // the sums of a piece's columns of one expert leave as one row per token
-    auto flush = [&](const Chunk &c) __attribute__((always_inline)) {
+    // The sums of a workgroup's columns of one expert leave as one row per token.
+    // Where to is looked up (seek) before the last chunk of them is consumed.
+    float *row = nullptr;
+    float weight = 0.0f;
+    auto seek = [&](const Chunk &c) __attribute__((always_inline)) {
+        row = nullptr;
         if (s_mask[c.e] >> r & 1) {
-            int p = r * k;
-            while (s_id[p] != c.e) ++p;
-            float *row = a.partial + (size_t)(first_row(p) + (int)blockIdx.x - piece_of(c.u * ns)) * H;
-            const float w = s_w[p];
+            int p = 0;
+            for (int i = 0; i < k; ++i) p = s_id[r * k + i] == c.e ? r * k + i : p;
+            row = a.partial + (size_t)(first_row(p) + 2 * (piece - piece_of(c.u * ns)) + second) * H + 4 * g;
+            weight = s_w[p];
+        }
+    };
+    auto flush = [&]() __attribute__((always_inline)) {
+        if (row) {
 #pragma unroll
             for (int q = 0; q < 2 * KQ; ++q) {
                 const int grp = wave + 8 * q;
@@ -425,8 +532,8 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const f32x4_t v = acc2[q][i];
-                        *reinterpret_cast<float4 *>(row + grp * 64 + 16 * i + 4 * g) =
-                            make_float4(v[0] * w, v[1] * w, v[2] * w, v[3] * w);
+                        *reinterpret_cast<float4 *>(row + grp * 64 + 16 * i) =
+                            make_float4(v[0] * weight, v[1] * weight, v[2] * weight, v[3] * weight);
                     }
             }
         }
@@ -436,25 +543,30 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
             for (int i = 0; i < 4; ++i) acc2[q][i] = f32x4_t{};
     };
 
-    Chunk cur{nullptr, 0, c0 / ns, c0 % ns};
+    Chunk cur{nullptr, 0, __builtin_amdgcn_readfirstlane(small_div(c0, ns)), 0};
+    cur.j = 2 * (c0 - cur.u * ns) + second;
     cur.e = expert_at(cur.u);
     cur.base = block_of(cur.e);
 #pragma unroll
     for (int s = 0; s < R; ++s) load(cur, s, st[s]);
+    weigh();
     count_rows();
+    __syncthreads();
     for (int c = c0; c + 1 < c1; ++c) {
-        Chunk next{cur.base, cur.e, cur.u, cur.j + 1};
-        if (next.j == ns) {
-            next = Chunk{nullptr, expert_at(cur.u + 1), cur.u + 1, 0};
+        Chunk next{cur.base, cur.e, cur.u, cur.j + 2};
+        if (next.j >= 2 * ns) {
+            next = Chunk{nullptr, expert_at(cur.u + 1), cur.u + 1, second};
             next.base = block_of(next.e);
+            seek(cur);
         }
         chunk(cur, next, true);
-        if (next.u != cur.u) flush(cur);
+        if (next.u != cur.u) flush();
         cur = next;
     }
+    seek(cur);
     chunk(cur, cur, false);
-    flush(cur);
-    if (blockIdx.x == 0) write_rows();
+    flush();
+    if (b == 0) write_rows();
 }
 
 // ---------------------------------------------------------------- merge
@@ -503,6 +615,9 @@ static bool few_shape_ok(int T, int H, int I, int E, int k) {
 // the partial rows: of each (token, slot) pair at most one per chunk
 static size_t few_rows(int T, int k, int I) { return (size_t)T * k * (I / kFewChunk); }
 
+// the workspace: row_base, the keys, the partial rows
+constexpr size_t kFewKeysAt = 256, kFewRowsAt = kFewKeysAt + kFewMaxT * kFewMaxE * sizeof(int);
+
 template <bool MX>
 static int few_launch_experts(const FewArgs &a, int cus, hipStream_t s) {
     switch ((a.H / kGroupIn + 7) / 8) {
@@ -521,7 +636,7 @@ using namespace pd;
 PD_API int pdscope_moe_few_supported(int T, int H, int I, int E, int k) { return few_shape_ok(T, H, I, E, k); }
 
 PD_API size_t pdscope_moe_few_workspace_size(int T, int H, int I, int E, int k) {
-    return few_shape_ok(T, H, I, E, k) ? 256 + few_rows(T, k, I) * H * sizeof(float) : 0;
+    return few_shape_ok(T, H, I, E, k) ? kFewRowsAt + few_rows(T, k, I) * H * sizeof(float) : 0;
 }
 
 PD_API int pdscope_moe_few(const void *x, const void *gate, const float *bias, int T, int H, int E, int k,
@@ -538,13 +653,17 @@ PD_API int pdscope_moe_few(const void *x, const void *gate, const float *bias, i
     hipError_t err = hipGetDevice(&dev);
     if (err == hipSuccess) err = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
     if (err != hipSuccess) return fail(kEHip, std::string("moe_few: ") + hipGetErrorString(err));
+    cus = std::min(cus, 1024) & ~1;  // an even grid, one workgroup a CU
+    if (cus < 2) return fail(kEHip, "moe_few: no compute units");
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    few_router_kernel<<<dim3(E, (T + kRouterT - 1) / kRouterT), 256, 0, s>>>((const uint16_t *)x, (const uint16_t *)gate, T, H, E, (uint16_t *)logits);
+    char *ws = (char *)workspace;
+    int *keys = (int *)(ws + kFewKeysAt);
+    few_router_kernel<<<dim3(E, (T + kRouterT - 1) / kRouterT), 256, 0, s>>>(
+        (const uint16_t *)x, (const uint16_t *)gate, bias, T, H, E, (uint16_t *)logits, keys);
     int rc = check_launch("few_router_kernel");
     if (rc) return rc;
-    const FewArgs a{(const uint16_t *)x, (const uint16_t *)logits, bias, T, H, E, k, normalize, I,
-                    (const uint8_t *const *)slots, ids, (uint16_t *)weights, (int32_t *)workspace,
-                    (float *)((char *)workspace + 256)};
+    const FewArgs a{(const uint16_t *)x, keys, T, H, E, k, normalize, I, (const uint8_t *const *)slots, ids,
+                    (uint16_t *)weights, (int32_t *)ws, (float *)(ws + kFewRowsAt)};
     rc = mxfp4 ? few_launch_experts<true>(a, cus, s) : few_launch_experts<false>(a, cus, s);
     if (rc) return rc;
     few_merge_kernel<<<dim3(H / 64, T), 512, 0, s>>>(a.partial, a.row_base, (const uint16_t *)add_in, H,
