@@ -428,7 +428,9 @@ int pdscope_swiglu_grouped_mxfp4(const void *x, const int32_t *perm_token, const
  * the decode submissions (expertbench/pdscope_runtime.py:326-350) and the merge
  * (pdscope_runtime.py:450-469) for a small batch.
  *   logits  = bf16(x . gate^T), summed in 64 bits (pdscope_route_topk sums in 32)
- *   ids, weights as pdscope_route_topk on these logits
+ *   ids     = the k experts of the largest logit + bias, equal ones by ascending id,
+ *             NaN after everything else; weights the softmax of those (normalize) or
+ *             their share of the softmax over all E, as pdscope_route_topk has them
  *   out[t]  = bf16(add_in[t] + sum_s w[t,s] * down(bf16(silu(gate x_t) * up x_t)))
  * with fp32 accumulation and no rounding between the down product and out
  * (pdscope_swiglu_decode and the grouped path also round gate, up and each
