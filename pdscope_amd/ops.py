@@ -794,41 +794,53 @@ def moe_few(x, gate, slots, I, top_k, normalize, *, bias=None, add_in=None, repr
 
 # ------------------------------------------------------ between two blocks
 
+def _fits(t, dtype, shape, dev) -> bool:
+    """Whether _need(t, ..., dtype, len(shape), dev) passes and t has this shape
+    (the checks of a call of 3 us on the GPU: one expression instead of a call
+    and four comparisons each)."""
+    return (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is dtype and t.device == dev
+            and t.is_contiguous())
+
+
+def _refuse(t, name, dtype, shape, dev):
+    _need(t, name, dtype, None, dev)
+    raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+
+
 def _norm_args(T, H, dev, resid, post_weight, gate, pre_weight, out_resid, out_norm, want_resid):
     """Checks of norm_residual / merge_norm_residual and their allocated outputs."""
-    _need(resid, "resid", None, 2, dev)
-    if resid.dtype not in (BF16, torch.float32):
-        raise ValueError(f"resid must be bf16 or fp32, got {resid.dtype}")
-    if tuple(resid.shape) != (T, H):
-        raise ValueError(f"resid must be [{T}, {H}], got {list(resid.shape)}")
-    given = [(t, n) for t, n in ((post_weight, "post_weight"), (gate, "gate"), (pre_weight, "pre_weight"))
-             if t is not None]
-    P = given[0][0].dtype if given and isinstance(given[0][0], torch.Tensor) else BF16
-    if P not in (BF16, torch.float32):
-        raise ValueError(f"{given[0][1]} must be bf16 or fp32, got {P}")
-    for t, n in given:
-        _need(t, n, P, None, dev)
-        if n != "gate" and tuple(t.shape) != (H,):
-            raise ValueError(f"{n} must be [{H}], got {list(t.shape)}")
+    shape = (T, H)
+    R = resid.dtype if isinstance(resid, torch.Tensor) else None
+    if R is not BF16 and R is not torch.float32:
+        _need(resid, "resid", None, 2, dev)
+        raise ValueError(f"resid must be bf16 or fp32, got {R}")
+    if not _fits(resid, R, shape, dev):
+        _refuse(resid, "resid", R, shape, dev)
+    first = post_weight if post_weight is not None else gate if gate is not None else pre_weight
+    P = first.dtype if isinstance(first, torch.Tensor) else BF16
+    if P is not BF16 and P is not torch.float32:
+        raise ValueError(f"post_weight, gate and pre_weight must be bf16 or fp32, got {P}")
+    if post_weight is not None and not _fits(post_weight, P, (H,), dev):
+        _refuse(post_weight, "post_weight", P, (H,), dev)
+    if pre_weight is not None and not _fits(pre_weight, P, (H,), dev):
+        _refuse(pre_weight, "pre_weight", P, (H,), dev)
     rows = cols = 0
     if gate is not None:
-        if tuple(gate.shape) not in ((H,), (1, H), (T, 1), (T, H)):
+        _need(gate, "gate", P, None, dev)
+        if gate.shape not in ((H,), (1, H), (T, 1), shape):
             raise ValueError(f"gate must be [H], [1, H], [T, 1] or [T, H], got {list(gate.shape)}")
         rows = int(gate.ndim == 2 and gate.shape[0] == T)
         cols = int(gate.ndim == 1 or gate.shape[1] == H)
     if out_resid is not None:
-        _need(out_resid, "out_resid", resid.dtype, 2, dev)
-        if tuple(out_resid.shape) != (T, H):
-            raise ValueError(f"out_resid must be [{T}, {H}], got {list(out_resid.shape)}")
+        if not _fits(out_resid, R, shape, dev):
+            _refuse(out_resid, "out_resid", R, shape, dev)
     elif want_resid:
         out_resid = torch.empty_like(resid)
     if out_norm is None:
-        out_norm = torch.empty((T, H), dtype=BF16, device=dev)
-    else:
-        _need(out_norm, "out_norm", BF16, 2, dev)
-        if tuple(out_norm.shape) != (T, H):
-            raise ValueError(f"out_norm must be [{T}, {H}], got {list(out_norm.shape)}")
-    return int(resid.dtype == torch.float32), rows, cols, int(P == torch.float32), out_resid, out_norm
+        out_norm = torch.empty_like(resid, dtype=BF16)
+    elif not _fits(out_norm, BF16, shape, dev):
+        _refuse(out_norm, "out_norm", BF16, shape, dev)
+    return int(R is torch.float32), rows, cols, int(P is torch.float32), out_resid, out_norm
 
 
 def norm_residual(block, resid, *, post_weight=None, gate=None, scale=1.0, pre_weight=None, eps=1e-6, out_resid=None,
