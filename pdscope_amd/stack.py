@@ -33,7 +33,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import layer as LY
-from . import synthetic
+from . import ops, synthetic
 from .cache import ExpertKey
 from .executor import masters_from_block
 from .pdscope_runtime import PDScopeCudaRuntime
@@ -41,9 +41,12 @@ from .pdscope_runtime import PDScopeCudaRuntime
 GIB = 1 << 30
 
 
-def rms_residual(out, x, eps=1e-6):
+def rms_residual(out, x, eps=1e-6, *, fused=False):
     """Next block's input: attention is the identity, so h = x + moe(x),
-    then RMSNorm with weight 1, in fp32, rounded to bf16."""
+    then RMSNorm with weight 1, in fp32, rounded to bf16.  fused: in one launch
+    (ops.norm_residual; the fp32 sum of squares runs in another order)."""
+    if fused:
+        return ops.norm_residual(out, x, eps=eps, want_resid=False)[1]
     h = out.float() + x.float()
     return (h * torch.rsqrt(h.pow(2).mean(-1, keepdim=True) + eps)).to(torch.bfloat16)
 
@@ -133,12 +136,14 @@ class StackBudget:
 
 @dataclass
 class StackSession:
-    """One runtime over a StackModel under a StackBudget."""
+    """One runtime over a StackModel under a StackBudget.  fused_norm: what stands
+    between two blocks runs as one launch."""
     model: StackModel
     device: torch.device
     budget: StackBudget = field(default_factory=StackBudget)
     resident_graphs: bool = True
     diagnostics: bool = False
+    fused_norm: bool = False
 
     def __post_init__(self):
         m = self.model
@@ -196,7 +201,7 @@ class StackSession:
             if observe is not None:
                 observe(LayerCall(step, l, x, out, routing, row))
             rows.append(row)
-            x = rms_residual(out, x)
+            x = rms_residual(out, x, fused=self.fused_norm)
         return x, rows
 
     def run(self, T_prefill=2048, n_decode=64, observe=None, observe_steps=None):
@@ -212,7 +217,7 @@ class StackSession:
         x = synthetic.make_tokens(T_prefill, m.H, seed=m.seed0 + 30002, device=dev)
         # the residual block's torch kernels load on their first call: call
         # it once outside the timed passes
-        rms_residual(x, x)
+        rms_residual(x, x, fused=self.fused_norm)
         torch.cuda.synchronize(dev)
         st0 = Counter(rt.cache.stats())
         t0 = time.perf_counter()

@@ -8,7 +8,7 @@ are rounded once.
 import pytest
 import torch
 
-from pdscope_amd import ops
+from pdscope_amd import ops, stack
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -220,3 +220,25 @@ def test_refusals():
         ops.merge_norm_residual(m["y"].flatten()[:-1], m["row_of"], m["w"], m["resid"])
     with pytest.raises(ValueError, match="add_in"):
         ops.merge_norm_residual(m["y"], m["row_of"], m["w"], m["resid"], add_in=m["resid"][:2])
+
+
+def test_stack_with_the_fused_norm():
+    """Every block's input in a session with fused_norm is the norm of the block
+    before: the sum and its norm in 64 bits, within (H + 8) / 2 + 4 roundings of fp32
+    and the one to bf16."""
+    model = stack.build_stack(3, torch.device(DEV, 0), hot_per_layer=6, calib_tokens=64, H=512, I=256, E=32, k=4)
+    session = stack.StackSession(model, torch.device(DEV, 0), stack.StackBudget(demand_slots=4), fused_norm=True)
+    try:
+        for step, T in enumerate((5, 1)):
+            calls = []
+            x = torch.randn(T, model.H, device=DEV, generator=torch.Generator(DEV).manual_seed(step)).to(BF16)
+            last, _ = session.run_pass(x, step, lambda c: calls.append((c.x.clone(), c.out.clone())))
+            torch.cuda.synchronize()
+            assert torch.equal(calls[0][0], x)
+            for (xin, out), got in zip(calls, [c[0] for c in calls[1:]] + [last]):
+                h = xin.double() + out.double()
+                want = h * torch.rsqrt(h.square().mean(1, keepdim=True) + 1e-6)
+                bound = want.abs() * (((model.H + 8) / 2 + 4) * U + 2.0 ** -8) + 2.0 ** -133
+                assert ((got.double() - want).abs() <= bound).all()
+    finally:
+        session.close()
