@@ -414,7 +414,8 @@ int pdscope_mxfp4_pack(const void *codes, const void *scales, int n, int H, int 
  * are not rounded, unlike the bf16 path's).  block_m: 32 or 64, the row tile
  * of the schedule (pdscope_grouped_mxfp4_block_m picks it from the mean rows per
  * selected expert).  Rows of an expert without a copy keep what y holds.
- * Limits: H % 128 == 0 and I % 128 == 0; x, h_ws and y 16-byte aligned.
+ * Limits: H % 128 == 0 and I % 128 == 0, at most 65536 each; x, h_ws and y
+ * 16-byte aligned; fewer than 2^35 values in x and in h_ws.
  */
 int pdscope_grouped_mxfp4_block_m(int rows_hint);
 int pdscope_swiglu_grouped_mxfp4(const void *x, const int32_t *perm_token, const int32_t *offsets,
@@ -465,7 +466,8 @@ int pdscope_moe_few(const void *x, const void *gate, const float *bias, int T, i
  * output may be NULL, and out_resid may be resid.  post_w and pre_w [H] and gate
  * are bf16, or fp32 when params_f32; gate (NULL: 1) has a value per token when
  * gate_rows and per channel when gate_cols: [T,H], [T], [H] or one value.
- * Limits: T >= 1, 1 <= H <= 16384 (16-byte accesses where H % 8 == 0 and every
+ * out_norm may be block (not y) or a bf16 resid; nothing else may overlap an output.
+ * Limits: 1 <= T < 2^22, 1 <= H <= 16384 (16-byte accesses where H % 8 == 0 and every
  * address is 16-byte aligned, single values otherwise).
  */
 int pdscope_norm_residual(const void *block, const void *resid, int resid_f32, const void *post_w,

@@ -27,6 +27,7 @@
 // h, and each expert's row of y before the merge, are rounded to bf16: h is the
 // matrix cores' input, and y in fp32 would be a quarter of the traffic of a long
 // prompt on top (out is off by three bf16 roundings in all, 0.3% of its norm).
+#include <algorithm>
 #include <type_traits>
 
 #include "mxfp4.h"
@@ -251,6 +252,10 @@ PD_API int pdscope_swiglu_grouped_mxfp4(const void *x, const int32_t *perm_token
         return fail(kEInval, "grouped_mxfp4: need H % 128 == 0 and I % 128 == 0 (at most 65536)");
     for (const void *p : {x, (const void *)h_ws, (const void *)y})
         if (reinterpret_cast<uintptr_t>(p) % 16) return fail(kEInval, "grouped_mxfp4: x, h_ws and y need 16-byte alignment");
+    // a launch has fewer than 2^32 threads: at least 128 columns of h or 256 of y a workgroup
+    // of 256, or 512 of y one of 512
+    if ((int64_t)max_tiles * ((std::max(I, H / 2) + 127) / 128) * 256 > ((int64_t)1 << 32) - 8192)
+        return fail(kEInval, "grouped_mxfp4: too many tiles for one launch");
     const MxCall c{offsets, sel, nsel, tile_start, max_tiles, (const uint8_t *const *)slots, H, I,
                    reinterpret_cast<hipStream_t>(stream)};
     auto *xs = (const uint16_t *)x;

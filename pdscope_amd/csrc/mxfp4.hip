@@ -161,8 +161,8 @@ static int mx_check(const char *what, const void *a, const void *b, const void *
         return fail(kEInval, std::string(what) + ": need H % 128 == 0 and I % 128 == 0 (at most 65536)");
     for (const void *p : {a, b, c})
         if (reinterpret_cast<uintptr_t>(p) % 16) return fail(kEInval, std::string(what) + ": addresses need 16-byte alignment");
-    // one wave per group, four to a workgroup, in one grid dimension
-    if ((int64_t)n * (int64_t)(mx_block_bytes(H, I) / kGroupBytes) > (int64_t)4 * 0x7fffffff)
+    // one wave per group, in one grid dimension of fewer than 2^32 threads
+    if ((int64_t)n * (int64_t)(mx_block_bytes(H, I) / kGroupBytes) > ((int64_t)1 << 26) - 4)
         return fail(kEInval, std::string(what) + ": too many weights for one call");
     return kOk;
 }

@@ -207,7 +207,9 @@ static void norm_launch(const NormArgs &a, int T, hipStream_t s) {
 }
 
 static int norm_call(const char *what, const NormArgs &a, int resid_f32, int params_f32, int T, void *stream) {
-    if (T < 1 || a.H < 1 || a.H > kNormMaxH) return fail(kEInval, std::string(what) + ": need T >= 1 and 1 <= H <= 16384");
+    // a row of up to 1024 threads: fewer than 2^32 in a launch
+    if (T < 1 || T >= (1 << 22) || a.H < 1 || a.H > kNormMaxH)
+        return fail(kEInval, std::string(what) + ": need T >= 1 and below 2^22, and 1 <= H <= 16384");
     if (!a.block || !a.resid || (!a.out_resid && !a.out_norm)) return fail(kEInval, std::string(what) + ": null pointer");
     if (!(a.eps >= 0.0f)) return fail(kEInval, std::string(what) + ": eps must not be negative");
     bool vec = a.H % 8 == 0;

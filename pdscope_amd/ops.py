@@ -735,6 +735,8 @@ def swiglu_grouped_mxfp4(x, perm_token, offsets, sel, tile_start, max_tiles, blo
         raise ValueError("h_ws / y workspaces are smaller than rows x I / rows x H")
     if tile_start.numel() < sel.numel() + 1 or offsets.numel() < slots.numel() + 1:
         raise ValueError("tile_start must hold one entry more than sel, offsets one more than slots")
+    if max(x.numel(), perm_token.numel() * I) >= 1 << 35:
+        raise ValueError("swiglu_grouped_mxfp4 addresses fewer than 2^35 activations")
     _call_on(dev, "pdscope_swiglu_grouped_mxfp4", _p(x), _p(perm_token), _p(offsets), _p(sel), sel.numel(),
              _p(tile_start), int(max_tiles), int(block_m), _p(slots), H, I, _p(h_ws), _p(y))
     return y

@@ -156,6 +156,19 @@ def test_the_same_call_gives_the_same_bits():
             assert all(torch.equal(a, b) for a, b in zip(lay.run(), want))
 
 
+@pytest.mark.parametrize("T", [1, 7, 16])
+@pytest.mark.parametrize("rep", ["mxfp4", "bf16"])
+def test_the_layer_over_its_own_output(rep, T):
+    """A step whose activations (and the shared experts' sum) lie where the layer's
+    output goes, as a stack that keeps one buffer has it."""
+    lay = Layer(T, 512, 256, 16, 4, rep)
+    want = [t.clone() for t in layer.moe_few(lay.x, lay.gate, lay.slots, lay.ws, add_in=lay.x, representation=rep)]
+    x = lay.ws.out[:T]
+    x.copy_(lay.x)
+    got = layer.moe_few(x, lay.gate, lay.slots, lay.ws, add_in=x, representation=rep)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_refusals():
     lay = Layer(4, 256, 128, 8, 2, "bf16")
     x17 = torch.zeros((17, 256), dtype=torch.bfloat16, device=DEV)

@@ -126,6 +126,18 @@ def test_outputs_in_place_and_the_norm_alone():
         assert torch.equal(r, want[0]) and torch.equal(n, want[1])
 
 
+@pytest.mark.parametrize("H", [1032, 2048, 10240])
+def test_the_norm_over_its_own_input(H):
+    """out_norm in the place of block or of resid, both rows read before they are written."""
+    c = make(37, H)
+    want = call(c)
+    for name in ("block", "resid"):
+        own = {**c, name: c[name].clone()}
+        got = call(own, out_norm=own[name])
+        assert got[1] is own[name]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_rows_of_an_expert_computed_elsewhere_add_nothing():
     c = make(5, 256, k=4, seed=5)
     c["row_of"][[0, 7]] = -1
