@@ -399,7 +399,7 @@ void pdscope_decode_unbind(pdscope_decode_binding *binding);
  * The layout of a block is the one the matrix cores read (csrc/mxfp4.h); entry
  * points that take 4-bit experts address blocks by the same slots tables as bf16
  * ones.  Limits: H % 128 == 0 and I % 128 == 0 (block_bytes: else 0); every
- * address 16-byte aligned; 1 <= n <= 65536.
+ * address 16-byte aligned; 1 <= n <= 65536, fewer than 2^37 weights in a call.
  */
 size_t pdscope_mxfp4_block_bytes(int H, int I);
 int pdscope_mxfp4_quantize(const void *experts, int n, int H, int I, void *blocks, void *stream);

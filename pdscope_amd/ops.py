@@ -7,6 +7,7 @@ Tensors are borrowed; nothing here allocates unless an output is omitted.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -33,10 +34,13 @@ def _stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _call_on(device, name, *args):
-    """An entry point on the current stream of `device`, which is made the
-    current device for the launch where it is another."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    """An entry point on the current stream of `device` (a tensor's), which is
+    made the current device for the launch where it is another."""
+    if device.index == _current_device():
         return _lib.call(name, *args, _stream(device))
     with torch.cuda.device(device):
         return _lib.call(name, *args, _stream(device))
@@ -659,6 +663,7 @@ def is_mxfp4(representation: str) -> bool:
     return representation == "mxfp4"
 
 
+@functools.lru_cache(maxsize=None)
 def mxfp4_block_bytes(H: int, I: int) -> int:
     """Bytes of one 4-bit expert block (17/32 of a byte per weight)."""
     n = int(_lib.load().pdscope_mxfp4_block_bytes(int(H), int(I)))
@@ -829,10 +834,17 @@ def _norm_args(T, H, dev, resid, post_weight, gate, pre_weight, out_resid, out_n
     rows = cols = 0
     if gate is not None:
         _need(gate, "gate", P, None, dev)
-        if gate.shape not in ((H,), (1, H), (T, 1), shape):
-            raise ValueError(f"gate must be [H], [1, H], [T, 1] or [T, H], got {list(gate.shape)}")
-        rows = int(gate.ndim == 2 and gate.shape[0] == T)
-        cols = int(gate.ndim == 1 or gate.shape[1] == H)
+        at = gate.shape
+        if at == (H,):
+            cols = 1
+        elif at == shape:
+            rows = cols = 1
+        elif at == (T, 1):
+            rows = 1
+        elif at == (1, H):
+            cols = 1
+        else:
+            raise ValueError(f"gate must be [H], [1, H], [T, 1] or [T, H], got {list(at)}")
     if out_resid is not None:
         if not _fits(out_resid, R, shape, dev):
             _refuse(out_resid, "out_resid", R, shape, dev)
