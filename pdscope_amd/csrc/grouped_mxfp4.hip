@@ -8,15 +8,17 @@
 // Weights are the first operand of v_mfma_f32_16x16x32_bf16 and never enter LDS:
 // each wave of a tile has a 64-row group of them to itself, whose 4352 bytes for
 // 128 inputs go from memory to the registers that hold them until they are
-// decoded (16 conversions per lane and 16-row tile, used for every token tile).  Activation rows are the second operand, shared by the four
-// waves: they stream into an LDS ring by direct-to-LDS loads, gathered through
-// perm_token, in 256-byte rows whose 16-byte chunk c lies in slot c ^ (row % 16),
-// so that the 16 rows of a fragment read lie in 16 bank groups.
+// decoded (16 conversions per lane and 16-row tile, used for every token tile).
+// Activation rows are the second operand, shared by the waves: they stream into
+// an LDS ring by direct-to-LDS loads, gathered through perm_token, in 256-byte
+// rows whose 16-byte chunk c lies in slot c ^ (row % 16), so that the 16 rows of a
+// fragment read lie in 16 bank groups.
 //
 // Thin experts are bound by HBM (Qwen shape T=33, gate/up 6.1 TB/s).  Long
 // prompts reach 1.19 PFLOP/s in gate/up and 1.02 in down (Qwen shape T=4096, 173
 // and 101 us; a 128-row tile 185 and 108): there the matrix cores are busy for
-// 63% of the CUs' cycles, LDS for 17%, and a quarter of the waves' time is waits.
+// 59% and 47% of the time, and 23% and 32% of the waves' time is waits (barriers and
+// loads: a step's loads have one step of three workgroups to land).
 // Measured on the 128-row tile and not kept: direct-to-LDS loads through buffer
 // descriptors, which need no address arithmetic (1-3%, and 4 GiB of activations
 // at most); weights two steps ahead (216 us); eight waves to a tile, which read
@@ -52,7 +54,7 @@ template <int BM, int NW, bool GATEUP>
 constexpr int kMxLds = 2 * BM * 256 > BM * kMxOutRow<NW, GATEUP> ? 2 * BM * 256 : BM * kMxOutRow<NW, GATEUP>;
 
 // BM rows x four groups (128 h columns or 256 y columns), K in steps of 128, two
-// stages of activations; OCC workgroups per CU.
+// stages of activations; at least OCC workgroups per CU.
 template <int BM, int NW, bool GATEUP, int OCC>
 __global__ __launch_bounds__(64 * NW, OCC * NW / 4) void mx_grouped_kernel(MxGrouped p) {
     __shared__ __attribute__((aligned(1024))) uint8_t smem[kMxLds<BM, NW, GATEUP>];
@@ -263,8 +265,8 @@ PD_API int pdscope_swiglu_grouped_mxfp4(const void *x, const int32_t *perm_token
     // 32 rows: bound by the weight stream.  gate/up on four waves, four workgroups
     // per CU; down (a short K loop) on eight, two per CU: fewer, wider workgroups
     // read each expert's h fewer times (Qwen shape T=33, gate/up 31.0 us = 6.1
-    // TB/s, eight waves 32.8; down 17.5, four waves 20.6).  64 rows: four waves,
-    // two workgroups per CU, whose steps interleave.
+    // TB/s, eight waves 32.8; down 17.5, four waves 20.6).  64 rows: four waves;
+    // three workgroups fit a CU (166 registers), whose steps interleave.
     if (block_m == 32) return mx_grouped_launch<32, 4, 4, 8, 2>(c, xs, perm_token, h, out);
     return mx_grouped_launch<64, 4, 2, 4, 2>(c, xs, perm_token, h, out);
 }
