@@ -156,6 +156,63 @@ def test_the_same_call_gives_the_same_bits():
             assert all(torch.equal(a, b) for a, b in zip(lay.run(), want))
 
 
+@pytest.mark.parametrize("rep", ["mxfp4", "bf16"])
+@pytest.mark.parametrize("masked", [float("-inf"), torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("T,E,k,left", [(1, 32, 4, 5), (5, 160, 4, 4), (16, 96, 6, 3), (2, 8, 8, 1)])
+@pytest.mark.parametrize("normalize", [True, False])
+def test_a_bias_that_masks_experts(T, E, k, left, masked, normalize, rep):
+    """All but `left` experts masked, in one case fewer than k: masked ones are then picked by
+    ascending id, with weight 0."""
+    lay = Layer(T, 256, 128, E, k, rep, bias=True, seed=12)
+    keep = torch.randperm(E, generator=torch.Generator().manual_seed(13))[:left].to(DEV)
+    bias = torch.full((E,), masked, device=DEV)
+    bias[keep] = lay.bias[keep]
+    lay.bias = bias
+    got = lay.run(normalize)
+    lay.check(got, normalize)
+    assert torch.isin(got[2][:, :min(k, left)].long(), keep).all() and not got[3][:, left:].any()
+
+
+def test_two_calls_at_once_and_graphs_that_share_a_workspace():
+    """Two streams with a workspace each; then two captured calls of different sizes on one
+    workspace, replayed in turn."""
+    a, b = Layer(16, 1024, 256, 64, 6, "mxfp4", seed=14), Layer(7, 1024, 512, 64, 4, "bf16", seed=15)
+    want = [[t.clone() for t in lay.run()] for lay in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for lay, s in zip((a, b), streams):
+            with torch.cuda.stream(s):
+                lay.run()
+    torch.cuda.synchronize()
+    for lay, w in zip((a, b), want):
+        assert torch.equal(lay.ws.out[:lay.T], w[0]) and torch.equal(lay.ws.ids[:lay.T], w[2])
+
+    ws = torch.empty(max(lay.ws.few_ws.numel() for lay in (a, b)), dtype=torch.uint8, device=DEV)
+    graphs, outs = [], []
+    for lay, w in zip((a, b), want):
+        o = [torch.empty_like(t) for t in w]
+
+        def call(lay=lay, o=o):
+            ops.moe_few(lay.x, lay.gate, lay.slots, lay.I, lay.k, True, representation=lay.rep, out=o[0], logits=o[1],
+                        ids=o[2], weights=o[3], workspace=ws)
+
+        call()
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call()
+        outs.append(o)
+    for _ in range(4):
+        for g, o, w in zip(graphs, outs, want):
+            for t in o:
+                t.zero_()
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(t, v) for t, v in zip(o, w))
+
+
 @pytest.mark.parametrize("T", [1, 7, 16])
 @pytest.mark.parametrize("rep", ["mxfp4", "bf16"])
 def test_the_layer_over_its_own_output(rep, T):
