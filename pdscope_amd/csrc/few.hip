@@ -250,12 +250,16 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
         const int t = small_div(pair, EK), e = pair - t * EK;
         const int *row = s_key + t * EK;
         const int mine = row[e];
-        int rank = 0;
+        // equal keys count where their expert is lower: those of the groups of four
+        // before e's own, and of that group the first e % 4
+        const int4 own = *reinterpret_cast<const int4 *>(row + (e & ~3));
+        int rank = part ? 0 : (own.x == mine && (e & 3) > 0) + (own.y == mine && (e & 3) > 1) +
+                                  (own.z == mine && (e & 3) > 2);
 #pragma unroll 8
         for (int j = 4 * part; j < EK; j += 4 * parts) {
             const int4 o = *reinterpret_cast<const int4 *>(row + j);
-            rank += (o.x >= mine + (j >= e)) + (o.y >= mine + (j + 1 >= e)) + (o.z >= mine + (j + 2 >= e)) +
-                    (o.w >= mine + (j + 3 >= e));
+            const int least = mine + (j >= (e & ~3));
+            rank += (o.x >= least) + (o.y >= least) + (o.z >= least) + (o.w >= least);
         }
         if (parts > 1) rank += __builtin_amdgcn_mov_dpp(rank, 0xb1, 0xf, 0xf, true);   // lanes ^ 1
         if (parts > 2) rank += __builtin_amdgcn_mov_dpp(rank, 0x4e, 0xf, 0xf, true);   // lanes ^ 2
@@ -269,6 +273,7 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
                 int key[J];
 #pragma unroll
                 for (int j = 0; j < J; ++j) key[j] = 64 * j + lane < E ? s_key[t * EK + 64 * j + lane] : kNoKey;
+                int mine = 0;  // lane i: the expert of rank i
                 for (int i = 0; i < k; ++i) {
                     int most = key[0];
 #pragma unroll
@@ -282,8 +287,9 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
                     }
 #pragma unroll
                     for (int j = 0; j < J; ++j) key[j] = 64 * j + lane == e ? kNoKey : key[j];
-                    if (lane == 0) picked(t, i, e);
+                    mine = lane == i ? e : mine;
                 }
+                if (lane < k) picked(t, lane, mine);
             }
         };
         if (E <= 64) rounds(std::integral_constant<int, 1>{});
