@@ -242,7 +242,7 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
     if (n_keys <= 512) {
         // A lane (or up to eight neighbouring ones) per token and expert counts the
         // experts ahead of it: no step waits for another.  One token of 128
-        // experts: 1.3 us from the keys to the weights, against 1.8 by rounds.
+        // experts: 2.3 thousand cycles from the keys to the picks, against 3.1 by rounds.
         int parts = 1;
         int shift = 0;
         while (parts < 8 && 2 * parts * n_keys <= 512) parts *= 2, ++shift;
@@ -630,13 +630,24 @@ __global__ __launch_bounds__(512) void few_merge_kernel(const float *__restrict_
     const int col = blockIdx.x * 64 + 4 * l;
     const int r0 = row_base[t], r1 = row_base[t + 1];
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 6
-    for (int r = r0 + q; r < r1; r += 32) {
-        const float4 p = *reinterpret_cast<const float4 *>(partial + (size_t)r * H + col);
-        v.x += p.x;
-        v.y += p.y;
-        v.z += p.z;
-        v.w += p.w;
+    // six rows at a time, the missing ones as zeros: a loop of the compiler's own
+    // takes the rows behind a multiple one after the other (T=4 26.7 us a layer
+    // against 26.4)
+    constexpr int U = 6;
+    for (int r = r0 + q; r < r1; r += 32 * U) {
+        float4 p[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            p[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (r + 32 * u < r1) p[u] = *reinterpret_cast<const float4 *>(partial + (size_t)(r + 32 * u) * H + col);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v.x += p[u].x;
+            v.y += p[u].y;
+            v.z += p[u].z;
+            v.w += p[u].w;
+        }
     }
     s_sum[q][4 * l] = v.x;
     s_sum[q][4 * l + 1] = v.y;
