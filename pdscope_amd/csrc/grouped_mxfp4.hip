@@ -109,8 +109,9 @@ __global__ __launch_bounds__(64 * NW, OCC * NW / 4) void mx_grouped_kernel(MxGro
 #pragma unroll
         for (int m = 0; m < TM; ++m) acc[i][m] = f32x4_t{};
 
-    auto kloop = [&](auto live) __attribute__((always_inline)) {
+    auto kloop = [&](auto live, auto once) __attribute__((always_inline)) {
         constexpr int L = decltype(live)::value;  // token tiles with rows of the expert
+        auto ld = [](const uint8_t *q) { return decltype(once)::value ? ld_nt(q) : ld_g(q); };
         auto issue_a = [&](int kt) __attribute__((always_inline)) {
             uint8_t *st = smem + (kt & 1) * (BM * 256);
 #pragma unroll
@@ -124,8 +125,8 @@ __global__ __launch_bounds__(64 * NW, OCC * NW / 4) void mx_grouped_kernel(MxGro
         auto issue_w = [&](int kt, uint4 (&d)[5]) __attribute__((always_inline)) {
             const uint8_t *b = wbase + (size_t)kt * kGroupBytes;
 #pragma unroll
-            for (int jj = 0; jj < 4; ++jj) d[jj] = ld_g(b + jj * 1024 + lane * 16);
-            d[4] = ld_g(b + kGroupScales + r * 16);
+            for (int jj = 0; jj < 4; ++jj) d[jj] = ld(b + jj * 1024 + lane * 16);
+            d[4] = ld(b + kGroupScales + r * 16);
         };
         // Step kt: everything asked for in step kt - 1 has landed (the one wait of
         // the step: loads to registers and to LDS complete in one order that the
@@ -168,14 +169,21 @@ __global__ __launch_bounds__(64 * NW, OCC * NW / 4) void mx_grouped_kernel(MxGro
             if (kt + 1 < KT) step(kt + 1, w1, w0);
         }
     };
-    // one straight-line loop for each number of 16-row tiles that hold rows
+    // one straight-line loop for each number of 16-row tiles that hold rows, and for
+    // weights that no other tile reads, which are not kept in the caches
+    // (the layer of the Qwen shape at T=33 66 -> 60 us, T=64 72 -> 64, T=512 95 -> 88;
+    // all weights read so, T=4096 takes 335 against 315)
     const int live = (min(BM, row_end - m0) + 15) / 16;
-    if (live == 1) kloop(std::integral_constant<int, 1>{});
-    else if (live == 2) kloop(std::integral_constant<int, 2>{});
-    else if constexpr (TM == 4) {
-        if (live == 3) kloop(std::integral_constant<int, 3>{});
-        else kloop(std::integral_constant<int, 4>{});
-    }
+    auto run = [&](auto once) __attribute__((always_inline)) {
+        if (live == 1) kloop(std::integral_constant<int, 1>{}, once);
+        else if (live == 2) kloop(std::integral_constant<int, 2>{}, once);
+        else if constexpr (TM == 4) {
+            if (live == 3) kloop(std::integral_constant<int, 3>{}, once);
+            else kloop(std::integral_constant<int, 4>{}, once);
+        }
+    };
+    if (row_end - p.offsets[e] <= BM) run(std::true_type{});
+    else run(std::false_type{});
 
     // ---- epilogue: a lane holds token row r of each tile and weight rows 4 g ..
     // + 3 of each 16-row tile; through LDS, out in whole-row 16-byte stores
@@ -234,9 +242,9 @@ static int mx_grouped_launch(const MxCall &c, const uint16_t *x, const int32_t *
 
 using namespace pd;
 
-// Layers of the Qwen shape on 32 and 64 rows: 2 mean rows 66.0 and 69.1 us, 16
-// 78.5 and 81.3, 32 105.0 and 90.0, 64 129 and 121, 256 347 and 299 (DeepSeek-V2-
-// Lite shape, 3 mean rows 68.5 and 66.4, 24 81.0 and 75.3).  A 128-row tile, whose
+// Layers of the Qwen shape on 32 and 64 rows: 6 mean rows 68.0 and 71.9 us, 16
+// 73.5 and 75.5, 24 89.0 and 82.4, 32 100.7 and 86.8, 44 113 and 103 (DeepSeek-V2-
+// Lite shape, 6 mean rows 64.4 and 64.1, 24 75.8 and 71.6). A 128-row tile, whose
 // weights are decoded once for twice the rows, is no faster anywhere (256 mean
 // rows 322 against 314 then).
 PD_API int pdscope_grouped_mxfp4_block_m(int rows_hint) { return rows_hint <= 16 ? 32 : 64; }
