@@ -14,7 +14,7 @@
 // rows whose 16-byte chunk c lies in slot c ^ (row % 16), so that the 16 rows of a
 // fragment read lie in 16 bank groups.
 //
-// Thin experts are bound by HBM (Qwen shape T=33, gate/up 6.1 TB/s).  Long
+// Thin experts are bound by HBM (Qwen shape T=33, gate/up 6.2 TB/s).  Long
 // prompts reach 1.19 PFLOP/s in gate/up and 1.02 in down (Qwen shape T=4096, 173
 // and 101 us; a 128-row tile 185 and 108): there the matrix cores are busy for
 // 59% and 47% of the time, and 23% and 32% of the waves' time is waits (barriers and
@@ -23,8 +23,9 @@
 // descriptors, which need no address arithmetic (1-3%, and 4 GiB of activations
 // at most); weights two steps ahead (216 us); eight waves to a tile, which read
 // the activations half as often (212); the products' order fixed by scheduling
-// barriers (208).  On 64 rows: weight registers reloaded piece by piece, for a
-// third workgroup per CU (the layer 336 us against 314).
+// barriers (208).  On 64 rows: weight registers reloaded piece by piece (the layer 336
+// us against 314); activation fragments read two or three ahead (the same); 32x32x16
+// products (361 against 317).
 //
 // h, and each expert's row of y before the merge, are rounded to bf16: h is the
 // matrix cores' input, and y in fp32 would be a quarter of the traffic of a long
