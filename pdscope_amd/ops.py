@@ -41,7 +41,10 @@ def _call_on(device, name, *args):
     """An entry point on the current stream of `device` (a tensor's), which is
     made the current device for the launch where it is another."""
     if device.index == _current_device():
-        return _lib.call(name, *args, _stream(device))
+        rc = getattr(_lib.load(), name)(*args, _stream(device))
+        if rc:
+            _lib.raise_for(name, rc)
+        return rc
     with torch.cuda.device(device):
         return _lib.call(name, *args, _stream(device))
 
@@ -833,7 +836,8 @@ def _norm_args(T, H, dev, resid, post_weight, gate, pre_weight, out_resid, out_n
         _refuse(pre_weight, "pre_weight", P, (H,), dev)
     rows = cols = 0
     if gate is not None:
-        _need(gate, "gate", P, None, dev)
+        if not (isinstance(gate, torch.Tensor) and gate.dtype is P and gate.device == dev and gate.is_contiguous()):
+            _need(gate, "gate", P, None, dev)
         at = gate.shape
         if at == (H,):
             cols = 1
