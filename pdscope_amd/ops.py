@@ -675,10 +675,10 @@ def mxfp4_block_bytes(H: int, I: int) -> int:
     return n
 
 
-def _mxfp4_out(out, E, width, dtype, dev):
+def _mxfp4_out(out, E, width, dtype, src):
     if out is None:
-        return torch.empty((E, width), dtype=dtype, device=dev)
-    _need(out, "out", dtype, 2, dev)
+        return src.new_empty((E, width), dtype=dtype)
+    _need(out, "out", dtype, 2, src.device)
     if tuple(out.shape) != (E, width):
         raise ValueError(f"out must be [{E}, {width}], got {tuple(out.shape)}")
     return out
@@ -689,10 +689,11 @@ def mxfp4_quantize(experts, H, I, out=None) -> torch.Tensor:
     [E, 3*I*H] (gate|up|down each; see pdscope_mxfp4_quantize for the rounding)."""
     _need(experts, "experts", BF16, 2)
     nbytes = mxfp4_block_bytes(H, I)
-    if experts.shape[1] != 3 * I * H or experts.shape[0] < 1:
+    E, n = experts.shape
+    if n != 3 * I * H or E < 1:
         raise ValueError(f"experts must be [E, 3*I*H] with E >= 1, got {tuple(experts.shape)}")
-    out = _mxfp4_out(out, experts.shape[0], nbytes, torch.uint8, experts.device)
-    _call_on(experts.device, "pdscope_mxfp4_quantize", _p(experts), experts.shape[0], H, I, _p(out))
+    out = _mxfp4_out(out, E, nbytes, torch.uint8, experts)
+    _call_on(experts.device, "pdscope_mxfp4_quantize", _p(experts), E, H, I, _p(out))
     return out
 
 
@@ -700,10 +701,11 @@ def mxfp4_dequantize(blocks, H, I, out=None) -> torch.Tensor:
     """The values of 4-bit blocks as bf16 blocks [E, 3*I*H] (exact)."""
     _need(blocks, "blocks", torch.uint8, 2)
     nbytes = mxfp4_block_bytes(H, I)
-    if blocks.shape[1] != nbytes or blocks.shape[0] < 1:
+    E, n = blocks.shape
+    if n != nbytes or E < 1:
         raise ValueError(f"blocks must be [E, {nbytes}] with E >= 1, got {tuple(blocks.shape)}")
-    out = _mxfp4_out(out, blocks.shape[0], 3 * I * H, BF16, blocks.device)
-    _call_on(blocks.device, "pdscope_mxfp4_dequantize", _p(blocks), blocks.shape[0], H, I, _p(out))
+    out = _mxfp4_out(out, E, 3 * I * H, BF16, blocks)
+    _call_on(blocks.device, "pdscope_mxfp4_dequantize", _p(blocks), E, H, I, _p(out))
     return out
 
 
@@ -718,7 +720,7 @@ def mxfp4_pack(codes, scales, H, I, out=None) -> torch.Tensor:
     if E < 1 or codes.shape[1] != n // 2 or tuple(scales.shape) != (E, n // 32):
         raise ValueError(f"codes must be [E, {n // 2}] and scales [E, {n // 32}], got {tuple(codes.shape)} and "
                          f"{tuple(scales.shape)}")
-    out = _mxfp4_out(out, E, nbytes, torch.uint8, codes.device)
+    out = _mxfp4_out(out, E, nbytes, torch.uint8, codes)
     _call_on(codes.device, "pdscope_mxfp4_pack", _p(codes), _p(scales), E, H, I, _p(out))
     return out
 
