@@ -226,6 +226,21 @@ def test_the_layer_over_its_own_output(rep, T):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("rep", ["mxfp4", "bf16"])
+def test_the_largest_layer(rep):
+    """Every limit but that on I at once: 16 tokens, 256 experts (eight blocks, each in 32 slots), k = 16 and
+    H = 4096, with more partial rows than 16 bits count."""
+    T, H, I, E, k = 16, 4096, 8320, 256, 16
+    lay = Layer(T, H, I, 8, 8, rep, seed=16)
+    g = torch.Generator(device=DEV).manual_seed(17)
+    lay.E, lay.k = E, k
+    lay.gate = (0.02 * torch.randn((E, H), generator=g, device=DEV)).to(torch.bfloat16)
+    lay.slots = lay.slots.repeat(E // 8)
+    lay.ws = layer.MoEWorkspace(T, H, I, E, k, DEV, few_tokens=True)
+    lay.block_of = lambda e: lay.experts[e % 8].double()
+    lay.check(lay.run())
+
+
 def test_refusals():
     lay = Layer(4, 256, 128, 8, 2, "bf16")
     x17 = torch.zeros((17, 256), dtype=torch.bfloat16, device=DEV)

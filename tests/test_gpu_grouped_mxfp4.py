@@ -162,6 +162,22 @@ def test_replay_of_a_prompt():
         assert torch.equal(got, want)
 
 
+def test_rows_past_2_to_the_32_values():
+    """2.2 million tokens, whose h has 4.5e9 values: tokens of the first rows, the last and some
+    between have what a call over them alone gives (a row's products do not depend on
+    the rows beside it)."""
+    T, H, I, E, k = 2_200_000, 128, 1024, 4, 2
+    x, ids, w, blocks, slots = make(T, H, I, E, k, seed=31)
+    ws = layer.MoEWorkspace(T, H, I, E, k, DEV)
+    assert ws.h_ws.numel() > 2 ** 32
+    out = layer.experts_resident(x, ids, w, slots, ws, block_m=64, representation="mxfp4")
+    pick = torch.cat([torch.arange(50), torch.arange(T // 2, T // 2 + 50), torch.arange(T - 50, T)]).to(DEV)
+    few = layer.MoEWorkspace(pick.numel(), H, I, E, k, DEV)
+    want = layer.experts_resident(x[pick], ids[pick], w[pick], slots, few, block_m=64, representation="mxfp4")
+    assert torch.equal(out[pick], want)
+    check(want, x[pick], ids[pick], w[pick], blocks, H, I)
+
+
 def test_refusals():
     T, H, I, E, k = 20, 256, 128, 4, 2
     x, ids, w, blocks, slots = make(T, H, I, E, k)

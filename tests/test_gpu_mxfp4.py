@@ -90,6 +90,22 @@ def test_infinities_and_nan_stay_in_their_block():
     assert torch.equal(nan.all(1), want) and torch.equal(nan.any(1), want)
 
 
+def test_more_than_2_to_the_32_weights():
+    """1000 experts (4.7e9 weights), eight of them again and again: every block and every value
+    equals the first eight's."""
+    H, I, n, times = 2048, 768, 8, 125
+    g = torch.Generator(device="cuda").manual_seed(7)
+    some = (0.05 * torch.randn((n, 3 * I * H), generator=g, device="cuda")).to(torch.bfloat16)
+    first = ops.mxfp4_quantize(some, H, I)
+    blocks = ops.mxfp4_quantize(some.repeat(times, 1), H, I)
+    assert blocks.shape[0] * 3 * I * H > 2 ** 32
+    assert (blocks.view(times, n, -1) == first).all()
+    values = ops.mxfp4_dequantize(blocks, H, I).view(torch.int16)
+    want = ops.mxfp4_dequantize(first, H, I).view(torch.int16)
+    for at in (0, 61 * n, (times - 1) * n):
+        assert torch.equal(values[at:at + n], want)
+
+
 def test_refusals():
     w = torch.zeros((2, 3 * 128 * 128), dtype=torch.bfloat16, device="cuda")
     with pytest.raises(ValueError, match="H % 128"):

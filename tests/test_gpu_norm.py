@@ -202,6 +202,26 @@ def test_replay_and_another_stream():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("k", [0, 1])
+def test_rows_past_2_to_the_31_values(k):
+    """1.1 million rows of 2048: the first, the last and some between have what a call over them
+    alone gives."""
+    T, H, n = 1_100_000, 2048, 1000
+    g = torch.Generator(device=DEV).manual_seed(5)
+    some = [torch.randn((n, H), generator=g, device=DEV).to(BF16) for _ in range(2)]
+    block, resid = (t.repeat(T // n, 1) for t in some)
+    block[-3:] = 2 * block[-3:]
+    pre = (1 + 0.2 * torch.randn(H, generator=g, device=DEV)).to(BF16)
+    if k:
+        w = torch.ones((T, 1), dtype=BF16, device=DEV)
+        got = ops.merge_norm_residual(block, torch.arange(T, dtype=torch.int32, device=DEV), w, resid, pre_weight=pre)
+    else:
+        got = ops.norm_residual(block, resid, pre_weight=pre)
+    for rows in (slice(0, 7), slice(T // 2, T // 2 + 7), slice(T - 7, T)):
+        want = ops.norm_residual(block[rows], resid[rows], pre_weight=pre)
+        assert all(torch.equal(a[rows], b) for a, b in zip(got, want))
+
+
 def test_refusals():
     c = make(4, 128)
     b, r = c["block"], c["resid"]
