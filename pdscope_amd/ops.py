@@ -92,8 +92,36 @@ def route_workspace(device, T: int = 1, H: int = 16, E: int = 32) -> torch.Tenso
 
 
 def slot_table(tensors, device) -> torch.Tensor:
-    """Device int64 table of expert base addresses (gate|up|down blocks)."""
-    return torch.tensor([t.data_ptr() for t in tensors], dtype=torch.int64, device=device)
+    """Device int64 table of expert base addresses (gate|up|down blocks; an
+    empty tensor is an expert without a copy).  The table remembers the size
+    and type of the blocks it was made of, and so do views of it (slices): the
+    entry points refuse it for a representation or a shape whose blocks are
+    others.  A copy of it, or a table made otherwise, is not checked, and new
+    addresses written into it must be those of such blocks."""
+    tensors = list(tensors)
+    table = torch.tensor([t.data_ptr() for t in tensors], dtype=torch.int64, device=device)
+    held = [t for t in tensors if t.numel()]
+    if held:
+        table.pd_blocks = (min(t.numel() * t.element_size() for t in held), frozenset(t.dtype for t in held))
+    return table
+
+
+def check_slots(slots, H, I, representation="bf16"):
+    """Refuse a table that slot_table made of blocks smaller than this
+    representation's experts of this shape, which the kernels would read past
+    the end of, or (4-bit) of blocks that are not bytes."""
+    known = getattr(slots, "pd_blocks", None)
+    if known is None:
+        known = getattr(getattr(slots, "_base", None), "pd_blocks", None)
+        if known is None:
+            return
+    held, dtypes = known
+    mx = is_mxfp4(representation)
+    need = mxfp4_block_bytes(H, I) if mx else 6 * H * I
+    if held < need:
+        raise ValueError(f"slots address blocks of {held} bytes, {representation} experts of H={H}, I={I} have {need}")
+    if mx and dtypes != {torch.uint8}:
+        raise ValueError(f"slots address blocks of {', '.join(sorted(map(str, dtypes)))}, 4-bit experts are torch.uint8")
 
 
 # --------------------------------------------------------------------- A1/A2
@@ -279,6 +307,7 @@ def swiglu_grouped(x, perm_token, offsets, sel, tile_start, max_tiles, block_m, 
     _need(slots, "slots", torch.int64, 1, dev)
     _need(h_ws, "h_ws", BF16, None, dev)
     _need(y, "y", BF16, None, dev)
+    check_slots(slots, H, I)
     if h_ws.numel() < perm_token.numel() * I or y.numel() < perm_token.numel() * H:
         raise ValueError("h_ws / y workspaces are smaller than rows x I / rows x H")
     _lib.call("pdscope_swiglu_grouped", _p(x), _p(perm_token), _p(offsets), _p(sel), sel.numel(), _p(tile_start),
@@ -291,6 +320,7 @@ def swiglu_grouped_gateup(x, perm_token, offsets, sel, tile_start, max_tiles, bl
     dev = x.device
     _need(x, "inputs", BF16, 2)
     _need(h_ws, "h_ws", BF16, None, dev)
+    check_slots(slots, H, I)
     if h_ws.numel() < perm_token.numel() * I:
         raise ValueError("h_ws is smaller than rows x I")
     _lib.call("pdscope_swiglu_grouped_gateup", _p(x), _p(perm_token), _p(offsets), _p(sel), sel.numel(),
@@ -312,9 +342,11 @@ def swiglu_grouped_layer(x, perm_token, offsets, sel, tile_start, max_tiles, blo
     _need(y, "y", BF16, None, dev)
     if h_ws.numel() < perm_token.numel() * I or y.numel() < perm_token.numel() * H:
         raise ValueError("h_ws / y workspaces are smaller than rows x I / rows x H")
+    check_slots(slots, H, I)
     slot, shared_I, h_shared, y_shared = shared if shared is not None else (None, 0, None, None)
     T = x.shape[0]
     if slot is not None:
+        check_slots(slot, H, shared_I)
         _need(slot, "shared_slot", torch.int64, 1, dev)
         _need(h_shared, "h_shared", BF16, None, dev)
         _need(y_shared, "y_shared", BF16, None, dev)
@@ -331,6 +363,7 @@ def swiglu_grouped_down(h_ws, offsets, sel, tile_start, max_tiles, block_m, slot
     """Only the down-projection launch of swiglu_grouped (K3, second half)."""
     dev = h_ws.device
     _need(y, "y", BF16, None, dev)
+    check_slots(slots, H, I)
     _lib.call("pdscope_swiglu_grouped_down", _p(h_ws), _p(offsets), _p(sel), sel.numel(), _p(tile_start),
               int(max_tiles), int(block_m), _p(slots), H, I, _p(y), _stream(dev))
 
@@ -354,6 +387,7 @@ def swiglu_decode(x, ids, w, slots, H, I, h_ws, out, *, merge="fused"):
     _need(slots, "slots", torch.int64, 1, dev)
     _need(h_ws, "h_ws", BF16, None, dev)
     _need(out, "out", BF16, None, dev)
+    check_slots(slots, H, I)
     k = ids.numel()
     if x.numel() != H or out.numel() != H or w.numel() != k or h_ws.numel() < k * I:
         raise ValueError("decode expects one token: x/out [H], ids/weights [k], h_ws >= k*I")
@@ -378,6 +412,8 @@ def decode_shared_layer(x, gate, slots, I, top_k, normalize, shared_slot, shared
     E, H = gate.shape
     for t, n in ((slots, "slots"), (shared_slot, "shared_slot")):
         _need(t, n, torch.int64, 1, dev)
+    check_slots(slots, H, I)
+    check_slots(shared_slot, H, shared_I)
     if bias is not None:
         _need(bias, "bias", torch.float32, 1, dev)
         if bias.numel() != E:
@@ -476,6 +512,7 @@ def decode_layer(x, gate, slots, I, top_k, normalize, *, bias=None, out, logits,
     _need(gate, "gate", BF16, 2, dev)
     _need(slots, "slots", torch.int64, 1, dev)
     E, H = gate.shape
+    check_slots(slots, H, I)
     if x.numel() != H or out.numel() != H or logits.numel() != E or ids.numel() != top_k or weights.numel() != top_k:
         raise ValueError("decode_layer expects one token: x/out [H], logits [E], ids/weights [k]")
     if h_ws.numel() < top_k * I or slots.numel() < E:
@@ -542,6 +579,7 @@ class DecodeBinding:
         _need(gate, "gate", BF16, 2, dev)
         _need(slots, "slots", torch.int64, 1, dev)
         E, H = gate.shape
+        check_slots(slots, H, int(I))
         k = int(top_k)
         if slots.numel() < E or not slots.is_contiguous():
             raise ValueError("DecodeBinding: slots must be a contiguous table of E entries")
@@ -739,6 +777,7 @@ def swiglu_grouped_mxfp4(x, perm_token, offsets, sel, tile_start, max_tiles, blo
     _need(slots, "slots", torch.int64, 1, dev)
     _need(h_ws, "h_ws", BF16, None, dev)
     _need(y, "y", BF16, None, dev)
+    check_slots(slots, H, I, "mxfp4")
     if x.shape[1] != H:
         raise ValueError(f"inputs must be [T, {H}], got {list(x.shape)}")
     if h_ws.numel() < perm_token.numel() * I or y.numel() < perm_token.numel() * H:
@@ -782,6 +821,7 @@ def moe_few(x, gate, slots, I, top_k, normalize, *, bias=None, add_in=None, repr
     if type(top_k) is not int or not moe_few_supported(T, H, I, E, top_k):
         raise ValueError(f"moe_few: unsupported shape T={T}, H={H}, I={I}, E={E}, k={top_k}")
     _need(slots, "slots", torch.int64, 1, dev)
+    check_slots(slots, H, I, representation)
     if slots.numel() < E:
         raise ValueError("slots must hold one entry per expert")
     if bias is not None:
