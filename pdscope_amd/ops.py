@@ -769,7 +769,8 @@ def grouped_mxfp4_block_m(rows_hint: int) -> int:
 
 
 def swiglu_grouped_mxfp4(x, perm_token, offsets, sel, tile_start, max_tiles, block_m, slots, H, I, h_ws, y):
-    """swiglu_grouped over the 4-bit blocks in `slots`; block_m 32 or 64."""
+    """swiglu_grouped over the 4-bit blocks in `slots` (an entry for each of the
+    offsets.numel() - 1 experts, of which `sel` names some); block_m 32 or 64."""
     _need(x, "inputs", BF16, 2)
     dev = x.device
     for t, n in ((perm_token, "perm_token"), (offsets, "offsets"), (sel, "sel"), (tile_start, "tile_start")):
@@ -782,8 +783,10 @@ def swiglu_grouped_mxfp4(x, perm_token, offsets, sel, tile_start, max_tiles, blo
         raise ValueError(f"inputs must be [T, {H}], got {list(x.shape)}")
     if h_ws.numel() < perm_token.numel() * I or y.numel() < perm_token.numel() * H:
         raise ValueError("h_ws / y workspaces are smaller than rows x I / rows x H")
-    if tile_start.numel() < sel.numel() + 1 or offsets.numel() < slots.numel() + 1:
-        raise ValueError("tile_start must hold one entry more than sel, offsets one more than slots")
+    if tile_start.numel() < sel.numel() + 1 or offsets.numel() < 2:
+        raise ValueError("tile_start must hold one entry more than sel, offsets one more than there are experts")
+    if slots.numel() < offsets.numel() - 1:
+        raise ValueError("slots must hold one entry per expert")
     if max(x.numel(), perm_token.numel() * I) >= 1 << 35:
         raise ValueError("swiglu_grouped_mxfp4 addresses fewer than 2^35 activations")
     _call_on(dev, "pdscope_swiglu_grouped_mxfp4", _p(x), _p(perm_token), _p(offsets), _p(sel), sel.numel(),
