@@ -163,6 +163,14 @@ def experts_resident(x, ids, weights, slots, ws: MoEWorkspace, out=None, *, bloc
         if shared_slot is not None:
             raise ValueError("shared experts join 4-bit routed experts through add_in")
         _, _, _, packed = ws.views(T)
+        # the launches below take these sizes as given
+        if ids.ndim != 2 or ids.shape[0] != T or not 1 <= ids.shape[1] <= k:
+            raise ValueError(f"ids must be [{T}, 1 to {k}], got {list(ids.shape)}")
+        if weights.shape != ids.shape:
+            raise ValueError(f"weights must be {list(ids.shape)}, got {list(weights.shape)}")
+        for t, name in ((out, "out"), (add_in, "add_in")):
+            if t is not None and (t.ndim != 2 or t.shape[0] < T or t.shape[1] != H):
+                raise ValueError(f"{name} must be [{T}, {H}], got {list(t.shape)}")
         bm = block_m or ops.grouped_mxfp4_block_m((T * k) // E)
         ops.pack(ids, E, out=packed, workspace=ws.pack_ws, schedule=(ws.sel_all, bm, ws.sel_order, ws.tile_start))
         ops.swiglu_grouped_mxfp4(x, packed.perm_token, packed.offsets, ws.sel_order, ws.tile_start,
