@@ -175,7 +175,7 @@ struct FewStage {
 
 // A wave's share of H: KQ groups of 128 inputs (gate/up) and 2 KQ groups of 64
 // outputs (down), dealt to the eight waves in turn; groups past the end read the
-// last one (an L2 hit) against x = 0, and their outputs are not stored.  The
+// last one (an L2 hit), whose values are not used.  The
 // activations stay in registers where they fit beside the sums and the ring, and
 // in LDS above that (XL; the shares of the inputs are then summed in two steps, to
 // fit both).  H = 4096, I = 1408, 40 experts touched by 16 tokens: 79 us a layer from
@@ -211,8 +211,8 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
     if (XL)
         for (int i = tid; i < T * KQ * 128; i += 512) {
             const int t = i / (KQ * 128), c = i % (KQ * 128);
-            *reinterpret_cast<uint4 *>(s_x + t * kRowX + 8 * c) =
-                8 * c < H ? ld_g(a.x + (uint32_t)(t * H + 8 * c)) : make_uint4(0, 0, 0, 0);
+            if (8 * c < H)
+                *reinterpret_cast<uint4 *>(s_x + t * kRowX + 8 * c) = ld_g(a.x + (uint32_t)(t * H + 8 * c));
         }
 #pragma unroll
     for (int q = 0; q < (XL ? 0 : KQ); ++q)
@@ -515,7 +515,9 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
             auto mfma = [](bf16x8_t w, bf16x8_t v, f32x4_t c) {
                 return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, v, c, 0, 0, 0);
             };
-            if (s < NS1) {
+            // an input group past the end has no products: against x = 0 an infinite
+            // weight of the group that is read in its place would be NaN
+            if (s < NS1 && ((MX ? s : s >> 1) < KQ - 1 || wave + 8 * (KQ - 1) < KG)) {
 #pragma unroll
                 for (int jj = 0; jj < (MX ? 4 : 2); ++jj) {
                     const int q = MX ? s : s >> 1, piece32 = MX ? jj : 2 * (s & 1) + (jj & 1);
@@ -533,7 +535,7 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
                             acc1[i] = mfma(__builtin_bit_cast(bf16x8_t, d.v[4 * jj + i]), v, acc1[i]);
                     }
                 }
-            } else {
+            } else if (s >= NS1) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     f32x4_t *o = acc2[2 * (s - NS1) + h];
