@@ -498,12 +498,17 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
                     gs += s_part[w * 1024 + tid];
                     us += s_part[w * 1024 + 512 + tid];
                 }
-                // h as the sum of two bf16 values (16 bits of it): the matrix cores
+                // h as the sum of two bf16 values (off by 2^-16 of it): the matrix cores
                 // take bf16, and a second product per weight costs nothing beside
-                // the stream, so h adds no rounding that out would show
+                // the stream, so h adds no rounding that out would show.  The first
+                // part is cut off, not rounded, and the second is never 0: both
+                // have the sign of h, so an infinite weight's two products are the
+                // same infinity (they were opposite ones, or infinity times 0)
                 const float h = silu_fast(gs) * us;
-                const uint32_t h0 = f2bf(h);
-                const float rest = (h0 & 0x7f80u) == 0x7f80u ? 0.0f : h - bf2f(h0);  // none of an infinity
+                const uint32_t h0 = __float_as_uint(h) >> 16;
+                float rest = h - bf2f(h0);
+                rest = rest == 0.0f ? bf2f(h0) * 0x1p-24f : rest;
+                rest = (h0 & 0x7f80u) == 0x7f80u ? h : rest;  // an infinity or NaN in both
                 const int at = ((tid >> 2) & 15) * 40 + (tid >> 8) * 16 + ((tid >> 6) & 3) * 4 + (tid & 3);
                 s_h[at] = (uint16_t)h0;
                 s_h[kFewMaxT * 40 + at] = (uint16_t)f2bf(rest);
