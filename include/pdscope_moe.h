@@ -432,12 +432,15 @@ int pdscope_swiglu_grouped_mxfp4(const void *x, const int32_t *perm_token, const
  *   ids     = the k experts of the largest logit + bias, equal ones by ascending id,
  *             NaN after everything else; weights the softmax of those (normalize) or
  *             their share of the softmax over all E, as pdscope_route_topk has them
- *   out[t]  = bf16(add_in[t] + sum_s w[t,s] * down(bf16(silu(gate x_t) * up x_t)))
- * with fp32 accumulation and no rounding between the down product and out
- * (pdscope_swiglu_decode and the grouped path also round gate, up and each
- * expert's row to bf16).  An expert without a copy (slots entry 0) adds nothing.
+ *   out[t]  = bf16(add_in[t] + sum_s w[t,s] * down(h)), h = silu(gate x_t) * up x_t
+ * with fp32 accumulation; h enters the down product as the sum of two bf16 values
+ * of its sign (off by 2^-16 of it), and nothing is rounded between that product and out
+ * (the 4-bit grouped path rounds h and each expert's row to bf16; the bf16 grouped
+ * path and pdscope_swiglu_decode gate and up too).  An expert without a copy
+ * (slots entry 0) adds nothing.
  * x [T,H], gate [E,H], bias [E] fp32 or NULL, add_in [T,H] bf16 or NULL, logits
  * [T,E] bf16, ids [T,k] int32, weights [T,k] bf16, out [T,H] bf16.
+ * x and add_in, one or both, may be the buffer of out; nothing else may overlap an output.
  * workspace: pdscope_moe_few_workspace_size bytes, 16-byte aligned, any contents
  * (0 bytes: outside the limits); calls that overlap in time need one each.
  * Limits: 1 <= T <= 16, E <= 256, 1 <= k <= min(E, 16), H % 128 == 0, H <= 4096,

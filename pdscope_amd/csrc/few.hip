@@ -628,10 +628,10 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
 // One workgroup per token and 64 columns: 32 quarter-waves take its rows in turn,
 // 16 bytes a lane, and are summed in order.  Bound by latency (1.6 MB of rows at
 // T = 1, 192 of them).
+// out may be add_in (each value is read by the thread that writes it, before it does).
 __global__ __launch_bounds__(512) void few_merge_kernel(const float *__restrict__ partial,
                                                         const int32_t *__restrict__ row_base,
-                                                        const uint16_t *__restrict__ add_in, int H,
-                                                        uint16_t *__restrict__ out) {
+                                                        const uint16_t *add_in, int H, uint16_t *out) {
     __shared__ float s_sum[32][65];
     const int t = blockIdx.y, q = threadIdx.x >> 4, l = threadIdx.x & 15;
     const int col = blockIdx.x * 64 + 4 * l;
