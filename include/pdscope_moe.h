@@ -392,7 +392,8 @@ void pdscope_decode_unbind(pdscope_decode_binding *binding);
  *               2^-127), each value is rounded to the nearest of 0, 0.5, 1, 1.5, 2,
  *               3, 4, 6 times that, ties to the even code, above 6 to 6.  32 values
  *               with an infinity or NaN among them become NaN (byte 255).
- *   dequantize  the values of blocks, as bf16 (exact).
+ *   dequantize  the values of blocks, as bf16: exact, but for those of 2^128 and more
+ *               (scale bytes 253 and 254, from a checkpoint only), which are infinite.
  *   pack        blocks of a checkpoint's tensors: codes [n, 3*I*H/2] (input 2i of
  *               a row in the low half of byte i) and scales [n, 3*I*H/32], gate|up|
  *               down row-major each; moves bytes only.

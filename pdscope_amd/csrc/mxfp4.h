@@ -42,8 +42,10 @@ __device__ __forceinline__ float mx_scale(uint32_t w) {
     return __uint_as_float(B == 0 ? w << 23 : B == 1 ? w << 15 : B == 2 ? w << 7 : w >> 1);
 }
 
-// The eight values of a word of codes, times the scale, as bf16.  Exact: two
-// significant bits, and bf16 has the exponents of e8m0 and more below.
+// The eight values of a word of codes, times the scale, as bf16.  Exact below
+// 2^128: two significant bits, and bf16 has the exponents of e8m0 and more below.
+// From there on (scale bytes 253 and 254, which quantising never gives, with
+// codes of 4 and 2 up) they are infinite.
 __device__ __forceinline__ bf16x8_t mx_decode(uint32_t codes, float scale) {
     const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0);
     const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1);

@@ -736,7 +736,8 @@ def mxfp4_quantize(experts, H, I, out=None) -> torch.Tensor:
 
 
 def mxfp4_dequantize(blocks, H, I, out=None) -> torch.Tensor:
-    """The values of 4-bit blocks as bf16 blocks [E, 3*I*H] (exact)."""
+    """The values of 4-bit blocks as bf16 blocks [E, 3*I*H]: exact, but for those
+    of 2^128 and more (a checkpoint's scale bytes 253 and 254), which are infinite."""
     _need(blocks, "blocks", torch.uint8, 2)
     nbytes = mxfp4_block_bytes(H, I)
     E, n = blocks.shape
