@@ -175,10 +175,9 @@ struct FewStage {
 
 // A wave's share of H: KQ groups of 128 inputs (gate/up) and 2 KQ groups of 64
 // outputs (down), dealt to the eight waves in turn; groups past the end read the
-// last one (an L2 hit), whose values are not used.  The
-// activations stay in registers where they fit beside the sums and the ring, and
-// in LDS above that (XL; the shares of the inputs are then summed in two steps, to
-// fit both).  H = 4096, I = 1408, 40 experts touched by 16 tokens: 79 us a layer from
+// last one (an L2 hit), whose values are not used.  The activations stay in
+// registers where they fit beside the sums and the ring, and in LDS above that (XL;
+// the shares of the inputs are then summed in two steps, to fit both).  H = 4096, I = 1408, 40 experts touched by 16 tokens: 79 us a layer from
 // LDS against 118 from spilled registers over 4-bit experts, 292 against 453 over
 // bf16 ones.
 template <bool MX, int KQ>
@@ -211,8 +210,8 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
     if (XL)
         for (int i = tid; i < T * KQ * 128; i += 512) {
             const int t = i / (KQ * 128), c = i % (KQ * 128);
-            if (8 * c < H)
-                *reinterpret_cast<uint4 *>(s_x + t * kRowX + 8 * c) = ld_g(a.x + (uint32_t)(t * H + 8 * c));
+            *reinterpret_cast<uint4 *>(s_x + t * kRowX + 8 * c) =
+                8 * c < H ? ld_g(a.x + (uint32_t)(t * H + 8 * c)) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
     for (int q = 0; q < (XL ? 0 : KQ); ++q)
@@ -468,6 +467,7 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc2[q][i] = f32x4_t{};
 
+    const uint32_t held = wave + 8 * (KQ - 1) < KG ? ~0u : 0u;  // all bits, or none for a last group past the end
     const uint16_t *x_row = s_x + (XL ? min(r, T - 1) * kRowX + wave * kGroupIn + 8 * g : 0);
     auto chunk = [&](const Chunk &c, const Chunk &next, bool more) __attribute__((always_inline)) {
         f32x4_t acc1[4] = {};
@@ -520,9 +520,17 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
             auto mfma = [](bf16x8_t w, bf16x8_t v, f32x4_t c) {
                 return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, v, c, 0, 0, 0);
             };
-            // an input group past the end has no products: against x = 0 an infinite
-            // weight of the group that is read in its place would be NaN
-            if (s < NS1 && ((MX ? s : s >> 1) < KQ - 1 || wave + 8 * (KQ - 1) < KG)) {
+            if (s < NS1) {
+                // an input group past the end counts as weights of 0 (4-bit: any code at
+                // the smallest scale) against x = 0: an infinite weight of the group that
+                // is read in its place would be NaN.  A branch round the products costs
+                // the widest bf16 layers 2 to 11% (H = 2560, 16 tokens, 201 us a layer
+                // to 223; this 202)
+                if ((MX ? s : s >> 1) == KQ - 1) {
+#pragma unroll
+                    for (int i = MX ? 4 : 0; i < (MX ? 5 : 8); ++i)
+                        d.v[i] = make_uint4(d.v[i].x & held, d.v[i].y & held, d.v[i].z & held, d.v[i].w & held);
+                }
 #pragma unroll
                 for (int jj = 0; jj < (MX ? 4 : 2); ++jj) {
                     const int q = MX ? s : s >> 1, piece32 = MX ? jj : 2 * (s & 1) + (jj & 1);
@@ -540,7 +548,7 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
                             acc1[i] = mfma(__builtin_bit_cast(bf16x8_t, d.v[4 * jj + i]), v, acc1[i]);
                     }
                 }
-            } else if (s >= NS1) {
+            } else {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     f32x4_t *o = acc2[2 * (s - NS1) + h];
