@@ -14,11 +14,14 @@
 // rows whose 16-byte chunk c lies in slot c ^ (row % 16), so that the 16 rows of a
 // fragment read lie in 16 bank groups.
 //
-// Thin experts are bound by HBM (Qwen shape T=33, gate/up 6.2 TB/s).  Long
-// prompts reach 1.19 PFLOP/s in gate/up and 1.02 in down (Qwen shape T=4096, 173
-// and 101 us; a 128-row tile 185 and 108): there the matrix cores are busy for
-// 59% and 47% of the time, and 23% and 32% of the waves' time is waits (barriers and
-// loads: a step's loads have one step of three workgroups to land).
+// Thin experts are bound by HBM (Qwen shape T=33, medians of a trace: gate/up 33.4
+// us, 5.6 TB/s, down 18.0 and 5.2; the fastest of 30 launches 32.1 and 17.5).  Long
+// prompts reach 1.12 PFLOP/s in gate/up and 0.96 in down (Qwen shape T=4096,
+// medians 185 and 108 us, the fastest 175 and 102; where a 128-row tile was timed beside
+// it, 173 and 101 against 185 and 108): there the matrix cores are busy for 59% and
+// 46% of the time, 22% and 34% of the waves' time is waits (barriers and loads: a
+// step's loads have one step of three workgroups to land) and 19% and 16% vector
+// instructions, the decoding of the weights among them.
 // Measured on the 128-row tile and not kept: direct-to-LDS loads through buffer
 // descriptors, which need no address arithmetic (1-3%, and 4 GiB of activations
 // at most); weights two steps ahead (216 us); eight waves to a tile, which read
@@ -27,9 +30,14 @@
 // us against 314); activation fragments read two or three ahead (the same); 32x32x16
 // products (361 against 317).
 //
-// h, and each expert's row of y before the merge, are rounded to bf16: h is the
-// matrix cores' input, and y in fp32 would be a quarter of the traffic of a long
-// prompt on top (out is off by three bf16 roundings in all, 0.3% of its norm).
+// h, and each expert's row of y before the merge, are rounded to bf16 (out is off by
+// three bf16 roundings in all, 0.0029 of its norm, against 0.0017 for its own alone).
+// h is the matrix cores' input: a second part of it, as few.hip has one, would double the
+// products of down, which bound a long prompt, and the workspace that holds h.  y is
+// what pdscope_merge and the norms' launch read of either representation; in fp32
+// it would be a quarter of the traffic of a long prompt on top.  Neither would cost
+// time where experts are thin (T=33: y is 1 MB beside 283 MB of weights); there
+// the types of h_ws and y are the reason, which are one for every length.
 #include <algorithm>
 #include <type_traits>
 
@@ -273,8 +281,8 @@ PD_API int pdscope_swiglu_grouped_mxfp4(const void *x, const int32_t *perm_token
     auto *h = (uint16_t *)h_ws, *out = (uint16_t *)y;
     // 32 rows: bound by the weight stream.  gate/up on four waves, four workgroups
     // per CU; down (a short K loop) on eight, two per CU: fewer, wider workgroups
-    // read each expert's h fewer times (Qwen shape T=33, gate/up 31.0 us = 6.1
-    // TB/s, eight waves 32.8; down 17.5, four waves 20.6).  64 rows: four waves;
+    // read each expert's h fewer times (Qwen shape T=33, timed beside each other:
+    // gate/up 31.0 us, eight waves 32.8; down 17.5, four waves 20.6).  64 rows: four waves;
     // three workgroups fit a CU (166 registers), whose steps interleave.
     if (block_m == 32) return mx_grouped_launch<32, 4, 4, 8, 2>(c, xs, perm_token, h, out);
     return mx_grouped_launch<64, 4, 2, 4, 2>(c, xs, perm_token, h, out);
