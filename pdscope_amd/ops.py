@@ -93,17 +93,26 @@ def route_workspace(device, T: int = 1, H: int = 16, E: int = 32) -> torch.Tenso
 
 def slot_table(tensors, device) -> torch.Tensor:
     """Device int64 table of expert base addresses (gate|up|down blocks; an
-    empty tensor is an expert without a copy).  The table remembers the size
-    and type of the blocks it was made of, and so do views of it (slices): the
-    entry points refuse it for a representation or a shape whose blocks are
-    others.  A copy of it, or a table made otherwise, is not checked, and new
-    addresses written into it must be those of such blocks."""
+    empty tensor is an expert without a copy; a bf16 tensor may be the start of
+    its block in a larger storage).  The table remembers the size and type of
+    the blocks it was made of, and so do views of it (slices): the entry points
+    refuse it for a representation or a shape whose blocks are others.  A copy
+    of it, or a table made otherwise, is not checked, and new addresses written
+    into it must be those of such blocks."""
     tensors = list(tensors)
     table = torch.tensor([t.data_ptr() for t in tensors], dtype=torch.int64, device=device)
     held = [t for t in tensors if t.numel()]
     if held:
-        table.pd_blocks = (min(t.numel() * t.element_size() for t in held), frozenset(t.dtype for t in held))
+        table.pd_blocks = (min(map(_block_extent, held)), frozenset(t.dtype for t in held))
     return table
+
+
+def _block_extent(t) -> int:
+    """Bytes that a block may have from t's address on: t's own, and what its
+    storage holds behind them where its type says that they are bf16 too."""
+    if t.dtype is BF16:
+        return t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
+    return t.numel() * t.element_size()
 
 
 def check_slots(slots, H, I, representation="bf16"):

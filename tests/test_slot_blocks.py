@@ -116,6 +116,10 @@ def test_tables_that_pass():
     ops.check_slots(ops.slot_table([some[0], some[:0], some[1]], "cpu"), H, I)
     ops.check_slots(ops.slot_table([some, some[1]], "cpu"), H, I)
     ops.check_slots(ops.slot_table([some[0].view(torch.uint8)], "cpu"), H, I)  # bf16 experts kept as bytes
+    gate = [some[e, :I * H].view(I, H) for e in range(2)]  # the first matrix of each block
+    ops.check_slots(ops.slot_table(gate, "cpu"), H, I)
+    with pytest.raises(ValueError, match="slots address blocks"):
+        ops.check_slots(ops.slot_table([some[1, 8:]], "cpu"), H, I)
     mixed = ops.slot_table([some[0], torch.zeros(FOUR, dtype=torch.uint8)], "cpu")
     for rep in ("bf16", "mxfp4"):
         with pytest.raises(ValueError, match="slots address blocks"):
