@@ -523,7 +523,7 @@ __global__ __launch_bounds__(512) void few_experts_kernel(FewArgs a) {
             if (s < NS1) {
                 // an input group past the end counts as weights of 0 (4-bit: any code at
                 // the smallest scale) against x = 0: an infinite weight of the group that
-                // is read in its place would be NaN.  A branch round the products costs
+                // is read in its place would be NaN.  A branch around the products costs
                 // the widest bf16 layers 2 to 11% (H = 2560, 16 tokens, 201 us a layer
                 // to 223; this 202)
                 if ((MX ? s : s >> 1) == KQ - 1) {
