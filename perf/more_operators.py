@@ -1,0 +1,421 @@
+"""Operators of a serving step over 8-bit activations and 4-bit weights.
+
+* ``norm``: the norm after a block, the residual sum and the norm before the
+  next block, whose output comes as bf16 (for the router) and as 8-bit rows
+  (e4m3 values with one e8m0 scale per 32 channels) for the experts;
+* ``experts``: the routed SwiGLU experts, ragged products grouped by expert, over
+  such 8-bit rows and 4-bit expert blocks (e2m1 values, e8m0 scales), whose
+  hidden rows are 8-bit rows too;
+* ``linear``: products of 1 to a few thousand rows with a 4-bit matrix that has a
+  scale, and where given a zero point, for each group of 32 to 128 inputs: the
+  attention's projections and the vocabulary head.
+
+Weights are N(0, 0.02), activations N(0, 1), as in the framework's synthetic
+layers; quantised weights are those weights quantised.  A state keeps them as a
+checkpoint does, in row-major order; a program of the framework also keeps the
+blocks laid out from them, its slot table and its workspaces.
+"""
+import math
+
+import torch
+
+own = False
+DEV = "cuda"
+BF16 = torch.bfloat16
+F8 = torch.float8_e4m3fn
+
+SHAPES = {
+    # the two layer shapes of pdscope_amd.synthetic (dsv2: its always-on shared
+    # experts' output is added to the routed experts' sum)
+    "qwen": dict(H=2048, I=768, E=128, k=8, normalize=True, add_in=False),
+    "dsv2": dict(H=2048, I=1408, E=64, k=6, normalize=False, add_in=True),
+    # smaller layers: fewer experts, a narrower hidden size
+    "small": dict(H=1024, I=512, E=64, k=4, normalize=True, add_in=False),
+    "narrow": dict(H=1536, I=384, E=96, k=6, normalize=True, add_in=False),
+}
+GRAPH_MAX_T = 16  # decode steps are captured and replayed
+
+
+def listed():
+    return [
+        # between two blocks, one token: latency
+        dict(name="norm_t1", op="norm", T=1, H=2048, k=0, resid="bf16", params="bf16", gate="none", post=False),
+        # an odd number of tokens of a mixed batch, a narrower layer, a gate and a post norm in 32 bits
+        dict(name="norm_t777", op="norm", T=777, H=1504, k=0, resid="fp32", params="fp32", gate="channel", post=True),
+        # after the experts of a long prompt, the merge of 8 rows a token included
+        dict(name="norm_merge_t4096", op="norm", T=4096, H=2048, k=8, resid="bf16", params="bf16", gate="none",
+             post=False),
+        # one token of a small layer
+        dict(name="experts_small_t1", op="experts", shape="small", T=1, skew=False),
+        # a decode batch: one to a few rows an expert, nearly every expert read
+        dict(name="experts_qwen_t33", op="experts", shape="qwen", T=33, skew=False),
+        # a mixed batch of decode tokens and prompt chunks, an odd length, uneven routing
+        dict(name="experts_qwen_t1303", op="experts", shape="qwen", T=1303, skew=True),
+        # a long prompt
+        dict(name="experts_dsv2_t4096", op="experts", shape="dsv2", T=4096, skew=False),
+        # the output projection of eight layers for the token of one user: latency
+        dict(name="linear_t1", op="linear", T=1, N=2048, K=4096, G=128, zeros=False, bias=False, layers=8),
+        # the vocabulary head for that token: bandwidth
+        dict(name="linear_head_t1", op="linear", T=1, N=151936, K=2048, G=64, zeros=True, bias=False, layers=1),
+        # a few requests, small groups, zero points and a bias; an odd number of outputs
+        dict(name="linear_t5", op="linear", T=5, N=4097, K=2816, G=32, zeros=True, bias=True, layers=4),
+        # a full small batch through the query projection
+        dict(name="linear_t16", op="linear", T=16, N=4096, K=2048, G=128, zeros=False, bias=True, layers=4),
+        # a prompt through it
+        dict(name="linear_t2048", op="linear", T=2048, N=4096, K=2048, G=128, zeros=True, bias=False, layers=1),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["norm", "experts", "linear"])
+    if op == "norm":
+        return dict(op=op, T=_log_int(rng, 1, 4095), H=32 * rng.randint(2, 128), k=rng.choice([0, 0, 1, 4, 6, 8]),
+                    resid=rng.choice(["bf16", "fp32"]), params=rng.choice(["bf16", "fp32"]),
+                    gate=rng.choice(["none", "channel", "token", "full"]), post=rng.random() < 0.5)
+    if op == "experts":
+        return dict(op=op, shape=rng.choice(sorted(SHAPES)), T=_log_int(rng, 1, 4095), skew=rng.random() < 0.5)
+    K = 32 * _log_int(rng, 4, 256)
+    T = _log_int(rng, 1, 2047)
+    return dict(op=op, T=T, N=_log_int(rng, 17, 8191), K=K, G=rng.choice([g for g in (32, 64, 128) if K % g == 0]),
+                zeros=rng.random() < 0.5, bias=rng.random() < 0.5, layers=rng.randint(1, 2) if T <= GRAPH_MAX_T else 1)
+
+
+# ------------------------------------------------------------------ inputs
+
+
+def _normal(gen, shape, std=1.0, dtype=BF16):
+    return (torch.randn(shape, generator=gen, device=DEV, dtype=torch.float32) * std).to(dtype)
+
+
+def _rows8(v):
+    """Values and scale exponents of v [.., n] in blocks of 32: the smallest power of
+    two that brings the block's largest magnitude to at most 448, from 2^-127 on;
+    each value rounded to the nearest e4m3 value, ties to even."""
+    b = v.unflatten(-1, (-1, 32))
+    m, e = torch.frexp(b.abs().amax(-1))
+    s = torch.where(m > 0.875, e - 8, e - 9).clamp(min=-127).unsqueeze(-1)
+    a = torch.ldexp(b, -s)
+    ulp = torch.ldexp(torch.ones_like(a), (torch.frexp(a).exponent - 1).clamp(min=-6) - 3)
+    return (torch.round(a / ulp) * ulp).flatten(-2), s.squeeze(-1)
+
+
+def _rows8_values(v):
+    """fp32 values of v's 8-bit rows."""
+    a, s = _rows8(v)
+    return torch.ldexp(a.float().unflatten(-1, (-1, 32)), s.unsqueeze(-1)).flatten(-2)
+
+
+def _checkpoint(gen, E, numel, block=1 << 25):
+    """Codes and scales of E experts of `numel` weights: N(0, 0.02) in e2m1 with the
+    scale 2^(floor(log2 of the largest magnitude of 32) - 2), magnitudes above 6 to 6."""
+    codes = torch.empty((E, numel // 2), dtype=torch.uint8, device=DEV)
+    scales = torch.empty((E, numel // 32), dtype=torch.uint8, device=DEV)
+    step = max(1, block // numel)
+    for e in range(0, E, step):
+        n = min(step, E - e)
+        b = _normal(gen, (n, numel // 32, 32), 0.02).float()
+        s = torch.frexp(b.abs().amax(-1)).exponent - 3
+        a = torch.ldexp(b, -s.unsqueeze(-1))
+        m = a.abs()
+        c = torch.where(m < 2, torch.round(2 * m), torch.where(m < 4, torch.round(m) + 2, torch.round(m / 2) + 4))
+        c = (c.clamp(max=7) + 8 * torch.signbit(a)).to(torch.uint8).flatten(1)
+        codes[e:e + n], scales[e:e + n] = c[:, 0::2] | (c[:, 1::2] << 4), (s + 127).to(torch.uint8)
+    return codes, scales
+
+
+class _Norm:
+    def __init__(self, case, gen):
+        T, H, k = case["T"], case["H"], case["k"]
+        P = torch.float32 if case["params"] == "fp32" else BF16
+        R = torch.float32 if case["resid"] == "fp32" else BF16
+        if k:
+            self.y = _normal(gen, (T * k, H))
+            self.row_of = torch.randperm(T * k, generator=gen, device=DEV).to(torch.int32)
+            self.w = torch.softmax(torch.randn((T, k), generator=gen, device=DEV), dim=1).to(BF16)
+        else:
+            self.block = _normal(gen, (T, H))
+        self.k = k
+        self.resid = _normal(gen, (T, H), 2.0, R)
+        self.pre = 1 + _normal(gen, (H,), 0.1, P)
+        self.post = 1 + _normal(gen, (H,), 0.1, P) if case["post"] else None
+        shape = {"none": None, "channel": (H,), "token": (T, 1), "full": (T, H)}[case["gate"]]
+        self.gate = None if shape is None else _normal(gen, shape, 0.5, P)
+        self.scale, self.eps = (0.75 if case["post"] else 1.0), 1e-6
+
+
+class _Experts:
+    def __init__(self, case, gen):
+        s = SHAPES[case["shape"]]
+        H, I, E, k, T = s["H"], s["I"], s["E"], s["k"], case["T"]
+        self.H, self.I, self.E, self.k = H, I, E, k
+        # the rows that the norm before the layer left
+        a, e = _rows8(torch.randn((T, H), generator=gen, device=DEV))
+        self.x, self.xs = a.to(F8), (e + 127).to(torch.uint8)
+        # the routing that the layer's router made of its logits
+        logits = torch.randn((T, E), generator=gen, device=DEV)
+        if case["skew"]:
+            logits = logits + 0.5 * torch.randn(E, generator=gen, device=DEV)
+        p = torch.softmax(logits, dim=1)
+        w, ids = torch.topk(p, k, dim=1)
+        self.ids = ids.to(torch.int32)
+        self.weights = (w / w.sum(dim=1, keepdim=True) if s["normalize"] else w).to(BF16)
+        self.add_in = _normal(gen, (T, H), 0.5) if s["add_in"] else None
+        self.codes, self.scales = _checkpoint(gen, E, 3 * I * H)
+        if own:
+            from pdscope_amd import layer, ops
+            self.experts = ops.mxfp4_pack(self.codes, self.scales, H, I)
+            self.slots = ops.slot_table([self.experts[e] for e in range(E)], DEV)
+            self.ws = layer.MoEWorkspace(T, H, I, E, k, DEV)
+
+
+class _Linear:
+    def __init__(self, case, gen):
+        T, N, K, G = case["T"], case["N"], case["K"], case["G"]
+        self.G, self.layers = G, []
+        for _ in range(case["layers"]):
+            w = _normal(gen, (N, K // G, G), 0.02).float()
+            if case["zeros"]:
+                lo, hi = w.amin(2).clamp(max=0), w.amax(2).clamp(min=0)
+                s = ((hi - lo) / 15).to(BF16)
+                z = torch.round(-lo / s.float()).clamp(0, 15).to(torch.uint8)
+            else:
+                s, z = (w.abs().amax(2) / 7).to(BF16), None
+            q = torch.round(w / s.float().unsqueeze(2)) + (8 if z is None else z.float().unsqueeze(2))
+            q = q.clamp(0, 15).to(torch.uint8).view(N, K)
+            self.layers.append(dict(codes=q[:, 0::2] | (q[:, 1::2] << 4), scales=s, zeros=z, x=_normal(gen, (T, K)),
+                                    bias=_normal(gen, (N,), 0.5) if case["bias"] else None))
+        self.graph = None
+        if own:
+            from pdscope_amd import ops
+            for lay in self.layers:
+                lay["w"] = ops.int4_pack(lay["codes"], lay["scales"], lay["zeros"])
+            if T <= GRAPH_MAX_T:
+                # a serving loop captures its decode step once and replays it
+                cur, side = torch.cuda.current_stream(), torch.cuda.Stream()
+                side.wait_stream(cur)
+                with torch.cuda.stream(side):
+                    self.step()
+                cur.wait_stream(side)
+                torch.cuda.synchronize()
+                self.graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(self.graph):
+                    self.outputs = self.step()
+
+    def step(self):
+        from pdscope_amd import ops
+        return [ops.linear_int4(lay["x"], lay["w"], bias=lay["bias"]) for lay in self.layers]
+
+
+STATES = {"norm": _Norm, "experts": _Experts, "linear": _Linear}
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device=DEV).manual_seed(1_000_003 * (int(seed) % 1_000_000) + 29)
+    return STATES[case["op"]](case, gen)
+
+
+# ------------------------------------------------------------- plain forms
+
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)
+
+
+def _pairs(device):
+    """[256, 2]: the two values of a byte of codes."""
+    v = torch.tensor(_E2M1, device=device)
+    return torch.stack([v.repeat(16), v.repeat_interleave(16)], dim=1)
+
+
+def _dequantize4(codes, scales):
+    """fp32 [.., K] of codes [.., K/2] and scales [.., K/32]."""
+    v = _pairs(codes.device)[codes.int()].flatten(-2).unflatten(-1, (-1, 32))
+    return torch.ldexp(v, (scales.int() - 127).unsqueeze(-1)).flatten(-2)
+
+
+def _norm_plain(s):
+    # in 64 bits: the 8-bit rows have values next to a border between two codes
+    r = s.resid.double()
+    if s.k:
+        a = (s.y[s.row_of.long()].double().view(*s.w.shape, -1) * s.w.double().unsqueeze(2)).sum(1)
+    else:
+        a = s.block.double()
+    if s.post is not None:
+        a = a * torch.rsqrt((a * a).mean(1, keepdim=True) + s.eps) * s.post.double()
+    if s.gate is not None:
+        a = a * s.gate.double()
+    r = r + s.scale * a
+    n = r * torch.rsqrt((r * r).mean(1, keepdim=True) + s.eps) * s.pre.double()
+    return r.to(s.resid.dtype), n.to(BF16), _rows8_values(n).to(BF16)
+
+
+def _experts_plain(s):
+    """The rows of each expert, padded to the fullest one, in one batched product."""
+    T = s.x.shape[0]
+    flat = s.ids.flatten().long()
+    counts = torch.bincount(flat, minlength=s.E)
+    order = torch.argsort(flat, stable=True)
+    first = torch.cumsum(counts, 0) - counts
+    place = torch.arange(T * s.k, device=DEV) - first[flat[order]]
+    v = torch.ldexp(s.x.float().unflatten(1, (-1, 32)), (s.xs.int() - 127).unsqueeze(2)).flatten(1)
+    x = torch.zeros((s.E, int(counts.max()), s.H), device=DEV)
+    x[flat[order], place] = v[order // s.k]
+    g, u, d = _dequantize4(s.codes, s.scales).split(s.I * s.H, dim=1)
+    g = torch.bmm(x, g.view(-1, s.I, s.H).transpose(1, 2))
+    u = torch.bmm(x, u.view(-1, s.I, s.H).transpose(1, 2))
+    h = _rows8_values(g / (1 + torch.exp(-g)) * u)
+    y = torch.bmm(h, d.view(-1, s.H, s.I).transpose(1, 2))
+    rows = torch.empty((T * s.k, s.H), device=DEV)
+    rows[order] = y[flat[order], place]
+    out = (rows.view(T, s.k, s.H) * s.weights.float().unsqueeze(2)).sum(1)
+    if s.add_in is not None:
+        out = out + s.add_in.float()
+    return out.to(BF16)
+
+
+def _linear_plain(lay, G):
+    q = torch.stack([lay["codes"] & 15, lay["codes"] >> 4], dim=-1).flatten(1).float().unflatten(1, (-1, G))
+    z = 8.0 if lay["zeros"] is None else lay["zeros"].float().unsqueeze(2)
+    w = ((q - z) * lay["scales"].float().unsqueeze(2)).flatten(1)
+    y = lay["x"].float() @ w.T
+    return (y if lay["bias"] is None else y + lay["bias"].float()).to(BF16)
+
+
+# --------------------------------------------------- the framework's calls
+
+
+def _run_own(s):
+    from pdscope_amd import layer, ops
+    if isinstance(s, _Linear):
+        if s.graph is None:
+            return s.step()
+        s.graph.replay()
+        return s.outputs
+    if isinstance(s, _Experts):
+        return layer.experts_resident(ops.MxRows(s.x, s.xs), s.ids, s.weights, s.slots, s.ws, add_in=s.add_in,
+                                      representation="mxfp4")
+    args = dict(post_weight=s.post, gate=s.gate, scale=s.scale, pre_weight=s.pre, eps=s.eps, want_mxfp8=True)
+    if s.k:
+        r, n, rows = ops.merge_norm_residual(s.y, s.row_of, s.w, s.resid, **args)
+    else:
+        r, n, rows = ops.norm_residual(s.block, s.resid, **args)
+    return r, n, ops.mxfp8_dequantize(rows)
+
+
+def run(state):
+    if own:
+        return _run_own(state)
+    if isinstance(state, _Linear):
+        return [_linear_plain(lay, state.G) for lay in state.layers]
+    return _experts_plain(state) if isinstance(state, _Experts) else _norm_plain(state)
+
+
+# -------------------------------------------------------------------- work
+
+
+def work(case):
+    """Inputs read once, outputs written once; the multiply-adds of the products.
+    Experts that the tokens reach: the expected number for uniform routing."""
+    T = case["T"]
+    if case["op"] == "norm":
+        H, k = case["H"], case["k"]
+        R, P = (4 if case["resid"] == "fp32" else 2), (4 if case["params"] == "fp32" else 2)
+        gate = {"none": 0, "channel": H, "token": T, "full": T * H}[case["gate"]]
+        # the sum, the bf16 norm and the 8-bit rows' values
+        byts = T * H * (2 * max(k, 1) + 2 * R + 2 + 2) + 6 * T * k + P * (H * (1 + case["post"]) + gate)
+        return {"bytes": byts, "flops": T * H * (2 * k + 12)}
+    if case["op"] == "experts":
+        s = SHAPES[case["shape"]]
+        H, I, E, k = s["H"], s["I"], s["E"], s["k"]
+        touched = k if T == 1 else E * (1 - (1 - k / E) ** T)
+        byts = touched * 3 * H * I * 17 / 32 + T * H * (33 / 32 + (4 if s["add_in"] else 2)) + T * k * 6
+        return {"bytes": byts, "flops": 6.0 * T * k * H * I}
+    N, K, G = case["N"], case["K"], case["G"]
+    byts = N * K / 2 + N * (K // G) * (3 if case["zeros"] else 2) + 2 * T * (N + K) + 2 * N * case["bias"]
+    return {"bytes": byts * case["layers"], "flops": 2.0 * T * N * K * case["layers"]}
+
+
+# ------------------------------------------------------------------- exact
+
+
+def _e4m3_grid():
+    """The finite magnitudes of e4m3 by code: exponent field 0 counts eighths of 2^-6,
+    field f has 1 to 1.875 times 2^(f - 7); the last code is a NaN."""
+    c = torch.arange(127, dtype=torch.float64, device=DEV)
+    f, m = torch.floor(c / 8), c % 8
+    return torch.where(f == 0, m / 8 * 2.0 ** -6, (1 + m / 8) * torch.exp2(f - 7))
+
+
+def _rows8_exact(v):
+    """8-bit rows' values of fp64 v [.., n], from the codes' grid: the nearest of two
+    neighbours, halfway the even code."""
+    grid = _e4m3_grid()
+    mids = (grid[1:] + grid[:-1]) / 2
+    b = v.reshape(-1, 32)
+    top = b.abs().amax(1, keepdim=True)
+    unit = torch.exp2(torch.ceil(torch.log2((top / 448).clamp(min=2.0 ** -127))))
+    unit = torch.where(top > 448 * unit, unit * 2, torch.where(top <= 224 * unit, unit / 2, unit)).clamp(min=2.0 ** -127)
+    a = (b / unit).abs()
+    code = torch.searchsorted(mids, a)  # the midpoints below a
+    tie = (code < 126) & (a == mids[code.clamp(max=125)]) & (code % 2 == 1)
+    return (grid[code + tie.long()] * unit * torch.sign(b)).view(v.shape)
+
+
+def _values4(codes, scales):
+    """fp64 values of e2m1 codes and scales: sign, two exponent bits (bias 1), one
+    mantissa bit, times 2^(scale - 127)."""
+    c = torch.stack([codes & 15, codes >> 4], dim=-1).flatten(-2).long()
+    e, m = (c >> 1) & 3, (c & 1).double()
+    mag = torch.where(e == 0, m * 0.5, (1 + 0.5 * m) * torch.exp2((e - 1).double()))
+    v = torch.where((c & 8) != 0, -mag, mag).unflatten(-1, (-1, 32))
+    return (v * torch.exp2(scales.double() - 127).unsqueeze(-1)).flatten(-2)
+
+
+def exact(case, seed):
+    """The operators in 64 bits.  The experts' hidden rows are 8-bit rows by definition."""
+    global own
+    kept, own = own, False
+    try:
+        s = prepare(case, seed)
+    finally:
+        own = kept
+    if case["op"] == "norm":
+        r = s.resid.double()
+        if s.k:
+            a = torch.zeros_like(r)
+            for j in range(s.k):
+                a += s.w[:, j:j + 1].double() * s.y[s.row_of.view(-1, s.k)[:, j].long()].double()
+        else:
+            a = s.block.double()
+        if s.post is not None:
+            a = a / torch.sqrt(a.square().mean(1, keepdim=True) + s.eps) * s.post.double()
+        r = r + s.scale * (a if s.gate is None else a * s.gate.double())
+        n = r / torch.sqrt(r.square().mean(1, keepdim=True) + s.eps) * s.pre.double()
+        return r, n, _rows8_exact(n)
+    if case["op"] == "experts":
+        H, I = s.H, s.I
+        x = (s.x.double().unflatten(1, (-1, 32)) * torch.exp2(s.xs.double() - 127).unsqueeze(2)).flatten(1)
+        ids, w = s.ids.long(), s.weights.double()
+        out = torch.zeros_like(x) if s.add_in is None else s.add_in.double()
+        for e in torch.unique(ids).tolist():
+            t, slot = torch.nonzero(ids == e, as_tuple=True)
+            block = _values4(s.codes[e], s.scales[e])
+            g = x[t] @ block[:I * H].view(I, H).T
+            u = x[t] @ block[I * H:2 * I * H].view(I, H).T
+            h = _rows8_exact(g * torch.sigmoid(g) * u)
+            out.index_add_(0, t, (h @ block[2 * I * H:].view(H, I).T) * w[t, slot].unsqueeze(1))
+        return out
+    outs = []
+    for lay in s.layers:
+        N, K = lay["codes"].shape[0], lay["x"].shape[1]
+        y = torch.zeros((lay["x"].shape[0], N), dtype=torch.float64, device=DEV)
+        x = lay["x"].double()
+        for n in range(0, N, 8192):  # rows of the matrix at a time
+            q = torch.empty((min(8192, N - n), K), dtype=torch.float64, device=DEV)
+            q[:, 0::2], q[:, 1::2] = lay["codes"][n:n + 8192] % 16, lay["codes"][n:n + 8192] // 16
+            zero = 8 if lay["zeros"] is None else lay["zeros"][n:n + 8192].double().repeat_interleave(s.G, 1)
+            y[:, n:n + 8192] = x @ ((q - zero) * lay["scales"][n:n + 8192].double().repeat_interleave(s.G, 1)).T
+        outs.append(y if lay["bias"] is None else y + lay["bias"].double())
+    return outs
