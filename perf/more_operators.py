@@ -91,6 +91,11 @@ def _normal(gen, shape, std=1.0, dtype=BF16):
     return (torch.randn(shape, generator=gen, device=DEV, dtype=torch.float32) * std).to(dtype)
 
 
+def _pow2(e):
+    """2^e in 64 bits for whole numbers e, exactly."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
 def _rows8(v):
     """Values and scale exponents of v [.., n] in blocks of 32: the smallest power of
     two that brings the block's largest magnitude to at most 448, from 2^-127 on;
@@ -98,15 +103,15 @@ def _rows8(v):
     b = v.unflatten(-1, (-1, 32))
     m, e = torch.frexp(b.abs().amax(-1))
     s = torch.where(m > 0.875, e - 8, e - 9).clamp(min=-127).unsqueeze(-1)
-    a = torch.ldexp(b, -s)
-    ulp = torch.ldexp(torch.ones_like(a), (torch.frexp(a).exponent - 1).clamp(min=-6) - 3)
+    a = b * _pow2(-s).to(b.dtype)
+    ulp = _pow2((torch.frexp(a).exponent - 1).clamp(min=-6) - 3).to(b.dtype)
     return (torch.round(a / ulp) * ulp).flatten(-2), s.squeeze(-1)
 
 
 def _rows8_values(v):
     """fp32 values of v's 8-bit rows."""
     a, s = _rows8(v)
-    return torch.ldexp(a.float().unflatten(-1, (-1, 32)), s.unsqueeze(-1)).flatten(-2)
+    return (a.float().unflatten(-1, (-1, 32)) * _pow2(s).float().unsqueeze(-1)).flatten(-2)
 
 
 def _checkpoint(gen, E, numel, block=1 << 25):
@@ -119,7 +124,7 @@ def _checkpoint(gen, E, numel, block=1 << 25):
         n = min(step, E - e)
         b = _normal(gen, (n, numel // 32, 32), 0.02).float()
         s = torch.frexp(b.abs().amax(-1)).exponent - 3
-        a = torch.ldexp(b, -s.unsqueeze(-1))
+        a = b * _pow2(-s).float().unsqueeze(-1)
         m = a.abs()
         c = torch.where(m < 2, torch.round(2 * m), torch.where(m < 4, torch.round(m) + 2, torch.round(m / 2) + 4))
         c = (c.clamp(max=7) + 8 * torch.signbit(a)).to(torch.uint8).flatten(1)
@@ -232,7 +237,7 @@ def _pairs(device):
 def _dequantize4(codes, scales):
     """fp32 [.., K] of codes [.., K/2] and scales [.., K/32]."""
     v = _pairs(codes.device)[codes.int()].flatten(-2).unflatten(-1, (-1, 32))
-    return torch.ldexp(v, (scales.int() - 127).unsqueeze(-1)).flatten(-2)
+    return (v * _pow2(scales.int() - 127).float().unsqueeze(-1)).flatten(-2)
 
 
 def _norm_plain(s):
@@ -259,7 +264,7 @@ def _experts_plain(s):
     order = torch.argsort(flat, stable=True)
     first = torch.cumsum(counts, 0) - counts
     place = torch.arange(T * s.k, device=DEV) - first[flat[order]]
-    v = torch.ldexp(s.x.float().unflatten(1, (-1, 32)), (s.xs.int() - 127).unsqueeze(2)).flatten(1)
+    v = (s.x.float().unflatten(1, (-1, 32)) * _pow2(s.xs.int() - 127).float().unsqueeze(2)).flatten(1)
     x = torch.zeros((s.E, int(counts.max()), s.H), device=DEV)
     x[flat[order], place] = v[order // s.k]
     g, u, d = _dequantize4(s.codes, s.scales).split(s.I * s.H, dim=1)
@@ -345,7 +350,7 @@ def _e4m3_grid():
     field f has 1 to 1.875 times 2^(f - 7); the last code is a NaN."""
     c = torch.arange(127, dtype=torch.float64, device=DEV)
     f, m = torch.floor(c / 8), c % 8
-    return torch.where(f == 0, m / 8 * 2.0 ** -6, (1 + m / 8) * torch.exp2(f - 7))
+    return torch.where(f == 0, m / 8 * 2.0 ** -6, (1 + m / 8) * _pow2(f - 7))
 
 
 def _rows8_exact(v):
@@ -355,7 +360,7 @@ def _rows8_exact(v):
     mids = (grid[1:] + grid[:-1]) / 2
     b = v.reshape(-1, 32)
     top = b.abs().amax(1, keepdim=True)
-    unit = torch.exp2(torch.ceil(torch.log2((top / 448).clamp(min=2.0 ** -127))))
+    unit = _pow2(torch.ceil(torch.log2((top / 448).clamp(min=2.0 ** -127))))
     unit = torch.where(top > 448 * unit, unit * 2, torch.where(top <= 224 * unit, unit / 2, unit)).clamp(min=2.0 ** -127)
     a = (b / unit).abs()
     code = torch.searchsorted(mids, a)  # the midpoints below a
@@ -368,9 +373,9 @@ def _values4(codes, scales):
     mantissa bit, times 2^(scale - 127)."""
     c = torch.stack([codes & 15, codes >> 4], dim=-1).flatten(-2).long()
     e, m = (c >> 1) & 3, (c & 1).double()
-    mag = torch.where(e == 0, m * 0.5, (1 + 0.5 * m) * torch.exp2((e - 1).double()))
+    mag = torch.where(e == 0, m * 0.5, (1 + 0.5 * m) * _pow2(e - 1))
     v = torch.where((c & 8) != 0, -mag, mag).unflatten(-1, (-1, 32))
-    return (v * torch.exp2(scales.double() - 127).unsqueeze(-1)).flatten(-2)
+    return (v * _pow2(scales.int() - 127).unsqueeze(-1)).flatten(-2)
 
 
 def exact(case, seed):
@@ -396,7 +401,7 @@ def exact(case, seed):
         return r, n, _rows8_exact(n)
     if case["op"] == "experts":
         H, I = s.H, s.I
-        x = (s.x.double().unflatten(1, (-1, 32)) * torch.exp2(s.xs.double() - 127).unsqueeze(2)).flatten(1)
+        x = (s.x.double().unflatten(1, (-1, 32)) * _pow2(s.xs.int() - 127).unsqueeze(2)).flatten(1)
         ids, w = s.ids.long(), s.weights.double()
         out = torch.zeros_like(x) if s.add_in is None else s.add_in.double()
         for e in torch.unique(ids).tolist():
