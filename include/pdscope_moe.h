@@ -484,6 +484,82 @@ int pdscope_merge_norm_residual(const void *y, int64_t y_rows, const int32_t *ro
                                 void *stream);
 
 /*
+ * 8-bit rows (microscaled floating point): activations as e4m3 codes [rows, n] with
+ * one e8m0 scale 2^(byte - 127) per 32 consecutive values, [rows, n / 32]; 33/32 byte
+ * a value.  No counterpart in the reference, whose activations are bf16 only.
+ *   quantize    x [rows, n] bf16.  A block of 32 whose largest magnitude is m has the
+ *               smallest scale 2^e, e >= -127, with m <= 448 * 2^e; each value is
+ *               rounded to the nearest code, ties to the even one.  32 values with an
+ *               infinity or NaN among them become NaN (byte 255).
+ *   dequantize  the values as bf16: exact from 2^-126 on.
+ * Limits: n % 32 == 0, rows * n below 2^35 - 4096; x and codes 16-byte aligned.
+ */
+int pdscope_mxfp8_quantize(const void *x, int64_t rows, int n, void *codes, void *scales, void *stream);
+int pdscope_mxfp8_dequantize(const void *codes, const void *scales, int64_t rows, int n, void *x, void *stream);
+
+/*
+ * pdscope_norm_residual and pdscope_merge_norm_residual, with n as 8-bit rows too
+ * (out_codes [T,H], out_scales [T,H/32], both given; out_norm may be NULL then), by
+ * the rule above from the unrounded n.  Sums and values are held in 64 bits, and each
+ * result is rounded once from that, so that no code depends on the order of a sum.
+ * The outputs' overlaps are those of pdscope_norm_residual; codes and scales may overlap nothing.
+ * Limits: theirs, and H % 32 == 0.
+ */
+int pdscope_norm_residual_mxfp8(const void *block, const void *resid, int resid_f32, const void *post_w,
+                                const void *gate, int gate_rows, int gate_cols, float scale, const void *pre_w,
+                                int params_f32, float eps, int T, int H, void *out_resid, void *out_norm,
+                                void *out_codes, void *out_scales, void *stream);
+int pdscope_merge_norm_residual_mxfp8(const void *y, int64_t y_rows, const int32_t *row_of, const void *w, int k,
+                                      const void *add_in, const void *resid, int resid_f32, const void *post_w,
+                                      const void *gate, int gate_rows, int gate_cols, float scale, const void *pre_w,
+                                      int params_f32, float eps, int T, int H, void *out_resid, void *out_norm,
+                                      void *out_codes, void *out_scales, void *stream);
+
+/*
+ * pdscope_swiglu_grouped_mxfp4 over 8-bit rows x [T,H] (codes and scales):
+ *   h[r] = rows8(silu(x . gate_e^T) * (x . up_e^T)),  y[r] = bf16(h[r] . down_e^T)
+ * with exact products of the codes' values and fp32 sums; h [rows,I] and h_scales
+ * [rows,I/32] are 8-bit rows by the rule above, from the unrounded product.  A
+ * row of h with an infinity or NaN makes its row of y NaN.  block_m: 32 or 64, the row
+ * tile of the schedule (pdscope_grouped_mxfp8_block_m picks it from the mean rows
+ * per selected expert).  Rows of an expert without a copy keep what y holds.
+ * Limits: H % 128 == 0 and I % 128 == 0, at most 65536 each; x, h and y 16-byte, scales
+ * 4-byte aligned; fewer than 2^36 values in x and in h.
+ */
+int pdscope_grouped_mxfp8_block_m(int rows_hint);
+int pdscope_swiglu_grouped_mxfp8(const void *x, const void *x_scales, const int32_t *perm_token,
+                                 const int32_t *offsets, const int32_t *sel, int nsel, const int32_t *tile_start,
+                                 int max_tiles, int block_m, const void *const *slots, int H, int I, void *h,
+                                 void *h_scales, void *y, void *stream);
+
+/*
+ * 4-bit matrices with group scales, W[n,k] = s[n,k/G] * (q[n,k] - z[n,k/G]): q and z
+ * whole numbers 0..15 (z is 8 throughout without zero points), G = 32, 64 or 128.
+ *   bytes       size of a matrix' buffer (0: outside the limits).
+ *   pack        from a checkpoint's tensors: codes [N,K/2] (input 2i of a row in the
+ *               low half of byte i), scales [N,K/G] of 16 bits (bf16 or fp16), zeros
+ *               [N,K/G] bytes of which the low four bits count, or NULL; moves bits only.
+ *   quantize    from bf16 weight [N,K]: s = bf16(max|w| / 7) and z = 8, or (zeros) s =
+ *               bf16((max(w,0) - min(w,0)) / 15) and z = round(-min(w,0) / s); q =
+ *               round(w / s) + z cut to 0..15, in fp32, ties to even.  Finite weights.
+ *   dequantize  the values as bf16 [N,K], each rounded once.
+ * pdscope_linear_int4: y [T,N] = bf16(x [T,K] . W^T + bias), bias [N] bf16 or NULL,
+ * with exact products of x and q, fp32 sums and fp32 scales; a row of x with an
+ * infinity or NaN gives NaN.  y may overlap nothing.
+ * Limits: 1 <= N <= 2^24, K % G == 0, K <= 2^20, fewer than 2^37 - 2^13 weights in whole
+ * 16 x 128 units; T >= 1, (N/16) * (T/16), each rounded up, below 2^23; x, w, codes
+ * and weight 16-byte aligned.
+ */
+size_t pdscope_int4_bytes(int N, int K, int G, int zeros);
+int pdscope_int4_pack(const void *codes, const void *scales, const void *zeros, int N, int K, int G, void *out,
+                      void *stream);
+int pdscope_int4_quantize(const void *weight, int N, int K, int G, int zeros, void *out, void *stream);
+int pdscope_int4_dequantize(const void *w, int N, int K, int G, int zeros, int fp16_scales, void *weight,
+                            void *stream);
+int pdscope_linear_int4(const void *x, const void *w, const void *bias, int T, int N, int K, int G, int zeros,
+                        int fp16_scales, void *y, void *stream);
+
+/*
  * A7 demand staging: replaces the three per-projection non_blocking copies
  * (expertbench/executor.py:341-363).  One hipMemcpyAsync of `bytes` from
  * page-locked host memory into a cache or staging slot on `stream`, then

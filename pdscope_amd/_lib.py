@@ -74,6 +74,20 @@ SIGNATURES = {
                                _vp], _i32),
     "pdscope_merge_norm_residual": ([_vp, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _f32, _vp, _i32,
                                      _f32, _i32, _i32, _vp, _vp, _vp], _i32),
+    "pdscope_mxfp8_quantize": ([_vp, _i64, _i32, _vp, _vp, _vp], _i32),
+    "pdscope_mxfp8_dequantize": ([_vp, _vp, _i64, _i32, _vp, _vp], _i32),
+    "pdscope_norm_residual_mxfp8": ([_vp, _vp, _i32, _vp, _vp, _i32, _i32, _f32, _vp, _i32, _f32, _i32, _i32, _vp, _vp,
+                                     _vp, _vp, _vp], _i32),
+    "pdscope_merge_norm_residual_mxfp8": ([_vp, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _f32, _vp,
+                                           _i32, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _vp], _i32),
+    "pdscope_grouped_mxfp8_block_m": ([_i32], _i32),
+    "pdscope_swiglu_grouped_mxfp8": ([_vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp,
+                                      _vp], _i32),
+    "pdscope_int4_bytes": ([_i32, _i32, _i32, _i32], _sz),
+    "pdscope_int4_pack": ([_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp], _i32),
+    "pdscope_int4_quantize": ([_vp, _i32, _i32, _i32, _i32, _vp, _vp], _i32),
+    "pdscope_int4_dequantize": ([_vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp], _i32),
+    "pdscope_linear_int4": ([_vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp], _i32),
     "pdscope_stage_expert": ([_vp, _vp, _sz, _vp, _vp], _i32),
     "pdscope_stage_merge": ([_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp], _i32),
     "pdscope_dispatch_pack": ([_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp], _i32),

@@ -129,6 +129,36 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
+// The same butterfly on 64-bit values, halves moved alike.
+__device__ __forceinline__ double wave_sum(double v) {
+    auto halves = [](double d) { return (uint64_t)__double_as_longlong(d); };
+    auto whole = [](uint32_t lo, uint32_t hi) { return __longlong_as_double((long long)((uint64_t)hi << 32 | lo)); };
+    {
+        const uint64_t u = halves(v);
+        const auto lo = __builtin_amdgcn_permlane32_swap((uint32_t)u, (uint32_t)u, false, false);
+        const auto hi = __builtin_amdgcn_permlane32_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+        v = whole(lo[0], hi[0]) + whole(lo[1], hi[1]);
+    }
+    {
+        const uint64_t u = halves(v);
+        const auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
+        const auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+        v = whole(lo[0], hi[0]) + whole(lo[1], hi[1]);
+    }
+#define PD_STEP(CTRL)                                                                            \
+    {                                                                                            \
+        const uint64_t u = halves(v);                                                            \
+        v += whole((uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xf, 0xf, true),   \
+                   (uint32_t)__builtin_amdgcn_mov_dpp((int)(u >> 32), CTRL, 0xf, 0xf, true));    \
+    }
+    PD_STEP(0x128)  // row_ror:8
+    PD_STEP(0x124)  // row_ror:4
+    PD_STEP(0x122)  // row_ror:2
+    PD_STEP(0x121)  // row_ror:1
+#undef PD_STEP
+    return v;
+}
+
 // Sums through DPP lane moves (no LDS round trips, unlike the shuffles
 // above).  Fixed order: neighbours (xor 1), then pairs (xor 2) within quads,
 // then lane i with 7-i of each half-row and with 15-i of each row, after

@@ -1,0 +1,319 @@
+// The grouped SwiGLU expert FFN over 8-bit rows (mxfp8.h) and 4-bit expert blocks
+// (mxfp4.h): products grouped by expert, every expert with as many rows as were
+// routed to it.
+//
+//   gate/up : h[r,:] = rows8(silu(x_r . gate) * (x_r . up))
+//   down    : y[r,n] = bf16(h_r . down_n)
+//
+// Both operands go to the scaled matrix instruction as they are, codes and
+// scales: v_mfma_scale_f32_16x16x128_f8f6f4, whose products are exact and whose
+// sums are fp32.  Of its first operand (e2m1) lane l = r + 16 g holds row r and the
+// 32 inputs of scale block g; of the second (e4m3) row r and the inputs 16 g
+// .. + 15 and 64 + 16 g .. + 15, beside the scale of block g.
+#include <algorithm>
+#include <type_traits>
+
+#include "mxfp4.h"
+#include "mxfp8.h"
+#include "ring.h"
+
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+
+namespace pd {
+
+struct Mx8Grouped {
+    const uint8_t *a, *a_scales;  // gate/up: x [T, H]; down: h [rows, I]
+    const int32_t *perm_token, *offsets, *sel;
+    int nsel;
+    const int32_t *tile_start;
+    const uint8_t *const *slots;
+    int H, I;
+    uint8_t *out, *out_scales;  // gate/up: h codes and scales; down: y bf16 [rows, H], null
+};
+
+// bytes of a staged output row: 32 columns of h codes or 64 of bf16 y per wave, off the bank line
+template <int NW, bool GATEUP>
+constexpr int kMx8OutRow = NW * (GATEUP ? 32 : 128) + 16;
+template <int BM>
+constexpr int kMx8Stage = BM * 128 + 256;  // codes and scales of a step's 128 inputs
+template <int BM, int NW, bool GATEUP>
+constexpr int kMx8Lds = std::max(2 * kMx8Stage<BM>, BM * kMx8OutRow<NW, GATEUP> + (GATEUP ? BM * NW : 0));
+
+// Direct-to-LDS loads that the compiler does not know of: lane l's BYTES at src land at
+// dst + BYTES l (dst is wave-uniform, an LDS offset).  It would let no LDS read
+// pass one in flight, of whatever address (its own wait before the first read
+// of a step was for that step's loads); here the waits of the K loop order
+// them.  The wait state lets m0 settle.
+template <int BYTES>
+__device__ __forceinline__ void load_lds_hidden(const uint8_t *src, uint32_t dst) {
+    static_assert(BYTES == 16 || BYTES == 4, "direct-to-LDS sizes");
+    if constexpr (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_offset(const void *p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)(uint32_t)(uintptr_t)p);
+}
+
+// BM rows x four groups (128 h columns or 256 y columns), K in steps of 128, two
+// stages of activations; at least OCC workgroups per CU.
+template <int BM, int NW, bool GATEUP, int OCC>
+__global__ __launch_bounds__(64 * NW, OCC * NW / 4) void mx8_grouped_kernel(Mx8Grouped p) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kMx8Lds<BM, NW, GATEUP>];
+    constexpr int TM = BM / 16;
+    const int H = p.H, I = p.I;
+    const int K = GATEUP ? H : I, KT = K / kGroupIn;
+    const int groups = GATEUP ? I / 32 : H / kGroupRows, NT = (groups + NW - 1) / NW;
+
+    // ---- tile: eight contiguous pieces of the list, one per XCD, columns fastest
+    const int total = p.tile_start[p.nsel] * NT;
+    const int per_xcd = (total + 7) >> 3, pos = blockIdx.x >> 3;
+    if (pos >= per_xcd) return;
+    const int t = (blockIdx.x & 7) * per_xcd + pos;
+    if (t >= total) return;
+    const int mt = t / NT, nt = t - mt * NT;
+    // the expert: the last lo with tile_start[lo] <= mt
+    int lo = 0;
+#pragma unroll 4
+    for (int b0 = 1; b0 < p.nsel; b0 += 64) {
+        const int j = b0 + (threadIdx.x & 63);
+        lo += __popcll(__ballot(j < p.nsel && p.tile_start[j] <= mt));
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int e = p.sel[lo];
+    const int row_end = p.offsets[e + 1], m0 = p.offsets[e] + (mt - p.tile_start[lo]) * BM;
+    const uint8_t *base = p.slots[e];
+    if (base == nullptr) return;  // no copy: the rows keep what they hold
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int rg = nt * NW + wave;            // this wave's row group
+    const int rg_in = min(rg, groups - 1);    // past the end: read the last one, store nothing
+    const uint8_t *const wbase =
+        base + ((GATEUP ? 0 : mx_gateup_groups(H, I)) + (size_t)rg_in * KT) * kGroupBytes;
+
+    // ---- activation loads: load q of wave w fills rows 8 (NW q + w) .. + 7 of 128
+    // bytes, whose 16-byte chunk c lies in slot c ^ (row / 2 % 8); lane l takes row + l /
+    // 8 and the chunk that belongs in its slot
+    constexpr int RQ = 8 * NW, AL = (BM + RQ - 1) / RQ;  // rows per load of all waves, loads of a wave
+    static_assert(BM % RQ == 0 || BM < RQ, "activation loads");
+    uint32_t arow[AL];
+    const int lrow = 8 * wave + (lane >> 3);  // in its load's rows
+    const uint32_t achunk = (uint32_t)((lane & 7) ^ ((lrow >> 1) & 7));
+#pragma unroll
+    for (int q = 0; q < AL; ++q) {
+        const int row = min(m0 + RQ * q + lrow, row_end - 1);
+        arow[q] = (uint32_t)(GATEUP ? p.perm_token[row] : row) * (uint32_t)(K / 16) + achunk;
+    }
+    // scales: lane l of the first wave takes row l's four of a step
+    uint32_t srow = 0;
+    if (wave == 0) {
+        const int row = min(m0 + min(lane, BM - 1), row_end - 1);
+        srow = (uint32_t)(GATEUP ? p.perm_token[row] : row) * (uint32_t)KT;
+    }
+
+    f32x4_t acc[4][TM];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int m = 0; m < TM; ++m) acc[i][m] = f32x4_t{};
+
+    auto kloop = [&](auto live, auto once) __attribute__((always_inline)) {
+        constexpr int L = decltype(live)::value;  // token tiles with rows of the expert
+        auto ld = [](const uint8_t *q) -> u32x4_t {
+            return decltype(once)::value ? __builtin_nontemporal_load(gptr(q)) : *gptr(q);
+        };
+        auto issue_a = [&](int kt) __attribute__((always_inline)) {
+            const uint32_t st = lds_offset(smem) + (kt & 1) * kMx8Stage<BM>;
+#pragma unroll
+            for (int q = 0; q < AL; ++q) {
+                if (RQ * q + 8 * wave >= 16 * L) continue;  // rows that no product reads
+                uint32_t o = arow[q];
+                opaque(o);
+                load_lds_hidden<16>(p.a + kt * 128 + (size_t)o * 16, st + (RQ * q + 8 * wave) * 128);
+            }
+            if (wave == 0) {
+                uint32_t o = srow;
+                opaque(o);
+                load_lds_hidden<4>(p.a_scales + ((size_t)o + kt) * 4, st + BM * 128);
+            }
+        };
+        // word i of d[q]: row 16 i + r, inputs 32 g + 8 q .. + 7; word i of the four is
+        // what the product of row tile i takes.  s: byte i is the scale of that block
+        auto issue_w = [&](int kt, u32x4_t (&d)[4], uint32_t &s) __attribute__((always_inline)) {
+            const uint8_t *b = wbase + (size_t)kt * kGroupBytes;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) d[q] = ld(b + g * 1024 + (r + 16 * q) * 16);
+            s = *reinterpret_cast<const uint32_t *>(b + kGroupScales + (r * 4 + g) * 4);
+        };
+        // Step kt: everything asked for in step kt - 1 has landed; then ask for kt + 1 and
+        // run the products of kt from d.
+        auto step = [&](auto more, int kt, u32x4_t (&d)[4], uint32_t &s, u32x4_t (&next)[4], uint32_t &snext)
+            __attribute__((always_inline)) {
+            wait_vm<0>();
+            ring_barrier();
+            // what a step asks for it asks for first, and the moves that put a row tile's words
+            // side by side are its own, behind the wait for them
+#pragma unroll
+            for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(d[q]));
+            if constexpr (decltype(more)::value) {
+                issue_a(kt + 1);
+                issue_w(kt + 1, next, snext);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const uint8_t *st = smem + (kt & 1) * kMx8Stage<BM>;
+            i32x8_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = i32x8_t{(int)d[0][i], (int)d[1][i], (int)d[2][i], (int)d[3][i], 0, 0, 0, 0};
+#pragma unroll
+            for (int m = 0; m < L; ++m) {
+                const uint8_t *row = st + (16 * m + r) * 128;
+                const uint4 x0 = *reinterpret_cast<const uint4 *>(row + ((g ^ (r >> 1)) << 4));
+                const uint4 x1 = *reinterpret_cast<const uint4 *>(row + (((4 + g) ^ (r >> 1)) << 4));
+                const int xs = st[BM * 128 + (16 * m + r) * 4 + g];
+                const i32x8_t x = {(int)x0.x, (int)x0.y, (int)x0.z, (int)x0.w, (int)x1.x, (int)x1.y, (int)x1.z, (int)x1.w};
+                acc[0][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[0], x, acc[0][m], 4, 0, 0, (int)s, 0, xs);
+                acc[1][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[1], x, acc[1][m], 4, 0, 1, (int)s, 0, xs);
+                acc[2][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[2], x, acc[2][m], 4, 0, 2, (int)s, 0, xs);
+                acc[3][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[3], x, acc[3][m], 4, 0, 3, (int)s, 0, xs);
+            }
+        };
+        u32x4_t w0[4], w1[4];
+        uint32_t s0, s1;
+        issue_w(0, w0, s0);
+        issue_a(0);
+        // no branch round the loads: their registers would be merged, and waited for, behind it
+        int kt = 0;
+        for (; kt + 2 < KT; kt += 2) {
+            step(std::true_type{}, kt, w0, s0, w1, s1);
+            step(std::true_type{}, kt + 1, w1, s1, w0, s0);
+        }
+        if (KT - kt == 2) {
+            step(std::true_type{}, kt, w0, s0, w1, s1);
+            step(std::false_type{}, kt + 1, w1, s1, w0, s0);
+        } else {
+            step(std::false_type{}, kt, w0, s0, w1, s1);
+        }
+    };
+    // one straight-line loop for each number of 16-row tiles that hold rows, and for
+    // weights that no other tile reads, which are not kept in the caches
+    const int live = (min(BM, row_end - m0) + 15) / 16;
+    auto run = [&](auto once) __attribute__((always_inline)) {
+        if (live == 1) kloop(std::integral_constant<int, 1>{}, once);
+        else if (live == 2) kloop(std::integral_constant<int, 2>{}, once);
+        else if constexpr (TM == 4) {
+            if (live == 3) kloop(std::integral_constant<int, 3>{}, once);
+            else kloop(std::integral_constant<int, 4>{}, once);
+        }
+    };
+    if (row_end - p.offsets[e] <= BM) run(std::true_type{});
+    else run(std::false_type{});
+
+    // ---- epilogue: a lane holds token row r of each tile and weight rows 4 g ..
+    // + 3 of each 16-row tile; through LDS, out in whole-row 16-byte stores.  The 32
+    // columns of h that a wave has of a row are one scale block, in four lanes.
+    constexpr int OB = kMx8OutRow<NW, GATEUP>;
+    uint8_t *const out_s = smem + BM * OB;
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+        if (m >= live) continue;
+        uint8_t *row = smem + (16 * m + r) * OB;
+        if constexpr (GATEUP) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[4 * i + q] = silu_fast(acc[i][m][q]) * acc[i + 2][m][q];
+            const uint32_t byte = mx8_scale_byte(max_over_quarters(top_magnitude8(v)));
+            const uint2 c = mx8_encode8(v, byte);
+            *reinterpret_cast<uint32_t *>(row + wave * 32 + 4 * g) = c.x;
+            *reinterpret_cast<uint32_t *>(row + wave * 32 + 16 + 4 * g) = c.y;
+            if (g == 0) out_s[(16 * m + r) * NW + wave] = (uint8_t)byte;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4_t v = acc[i][m];
+                *reinterpret_cast<uint2 *>(row + wave * 128 + i * 32 + 8 * g) =
+                    make_uint2(f2bf2_hw(v[0], v[1]), f2bf2_hw(v[2], v[3]));
+            }
+        }
+    }
+    __syncthreads();
+    const int rows = min(BM, row_end - m0);
+    constexpr int CO = NW * (GATEUP ? 32 : 128), CH = CO / 16;  // bytes and 16-byte pieces of a row
+    const int ldo = GATEUP ? I : 2 * H, bytes = min(CO, ldo - nt * CO);  // bytes % 128 == 0
+    for (int c = tid; c < rows * CH; c += 64 * NW) {
+        const int row = c / CH, ch = c % CH;
+        if (ch * 16 < bytes)
+            st_through(p.out + (size_t)(m0 + row) * ldo + nt * CO + ch * 16,
+                       *reinterpret_cast<const uint4 *>(smem + row * OB + ch * 16));
+    }
+    if constexpr (GATEUP) {
+        // scales: four bytes (128 columns) at a time
+        for (int c = tid; c < rows * (NW / 4); c += 64 * NW) {
+            const int row = c / (NW / 4), ch = c % (NW / 4);
+            if (ch * 128 < bytes)
+                *reinterpret_cast<uint32_t *>(p.out_scales + (size_t)(m0 + row) * (I / 32) + nt * NW + ch * 4) =
+                    *reinterpret_cast<const uint32_t *>(out_s + row * NW + ch * 4);
+        }
+    }
+}
+
+struct Mx8Call {
+    const int32_t *offsets, *sel;
+    int nsel;
+    const int32_t *tile_start;
+    int max_tiles;
+    const uint8_t *const *slots;
+    int H, I;
+    hipStream_t s;
+};
+
+// NWG / NWD waves and OCCG / OCCD workgroups per CU of the gate/up and down halves
+template <int BM, int NWG, int OCCG, int NWD, int OCCD>
+static int mx8_grouped_launch(const Mx8Call &c, const uint8_t *x, const uint8_t *xs, const int32_t *perm, uint8_t *h,
+                              uint8_t *hs, uint8_t *y) {
+    auto grid = [&](int nt) { return (unsigned)(((size_t)c.max_tiles * nt + 7) / 8 * 8); };
+    mx8_grouped_kernel<BM, NWG, true, OCCG><<<grid((c.I / 32 + NWG - 1) / NWG), 64 * NWG, 0, c.s>>>(
+        Mx8Grouped{x, xs, perm, c.offsets, c.sel, c.nsel, c.tile_start, c.slots, c.H, c.I, h, hs});
+    const int rc = check_launch("mx8_grouped_kernel<gateup>");
+    if (rc) return rc;
+    mx8_grouped_kernel<BM, NWD, false, OCCD><<<grid((c.H / kGroupRows + NWD - 1) / NWD), 64 * NWD, 0, c.s>>>(
+        Mx8Grouped{h, hs, nullptr, c.offsets, c.sel, c.nsel, c.tile_start, c.slots, c.H, c.I, y, nullptr});
+    return check_launch("mx8_grouped_kernel<down>");
+}
+
+}  // namespace pd
+
+using namespace pd;
+
+PD_API int pdscope_grouped_mxfp8_block_m(int rows_hint) { return rows_hint <= 16 ? 32 : 64; }
+
+PD_API int pdscope_swiglu_grouped_mxfp8(const void *x, const void *x_scales, const int32_t *perm_token,
+                                        const int32_t *offsets, const int32_t *sel, int nsel, const int32_t *tile_start,
+                                        int max_tiles, int block_m, const void *const *slots, int H, int I, void *h,
+                                        void *h_scales, void *y, void *stream) {
+    if (!x || !x_scales || !perm_token || !offsets || !sel || !tile_start || !slots || !h || !h_scales || !y)
+        return fail(kEInval, "grouped_mxfp8: null pointer");
+    if (nsel < 1 || max_tiles < 1 || max_tiles > (1 << 22))
+        return fail(kEInval, "grouped_mxfp8: need nsel >= 1 and 1 <= max_tiles <= 4194304");
+    if (block_m != 32 && block_m != 64) return fail(kEInval, "grouped_mxfp8: block_m must be 32 or 64");
+    if (!mx_shape_ok(H, I) || H > 65536 || I > 65536)
+        return fail(kEInval, "grouped_mxfp8: need H % 128 == 0 and I % 128 == 0 (at most 65536)");
+    for (const void *p : {x, (const void *)h, (const void *)y})
+        if (reinterpret_cast<uintptr_t>(p) % 16) return fail(kEInval, "grouped_mxfp8: x, h and y need 16-byte alignment");
+    for (const void *p : {x_scales, (const void *)h_scales})
+        if (reinterpret_cast<uintptr_t>(p) % 4) return fail(kEInval, "grouped_mxfp8: scales need 4-byte alignment");
+    // a launch has fewer than 2^32 threads: at least 128 columns of h or 256 of y a workgroup
+    // of 256, or 512 of y one of 512
+    if ((int64_t)max_tiles * ((std::max(I, H / 2) + 127) / 128) * 256 > ((int64_t)1 << 32) - 8192)
+        return fail(kEInval, "grouped_mxfp8: too many tiles for one launch");
+    const Mx8Call c{offsets, sel, nsel, tile_start, max_tiles, (const uint8_t *const *)slots, H, I,
+                    reinterpret_cast<hipStream_t>(stream)};
+    auto *xc = (const uint8_t *)x, *xs = (const uint8_t *)x_scales;
+    auto *hc = (uint8_t *)h, *hs = (uint8_t *)h_scales, *out = (uint8_t *)y;
+    if (block_m == 32) return mx8_grouped_launch<32, 4, 4, 8, 2>(c, xc, xs, perm_token, hc, hs, out);
+    return mx8_grouped_launch<64, 4, 2, 4, 2>(c, xc, xs, perm_token, hc, hs, out);
+}

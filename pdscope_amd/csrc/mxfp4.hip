@@ -10,6 +10,7 @@
 // value on the bf16 side, 17/32 on the other (64 experts of the Qwen shape:
 // quantised in 145 us, 5.3 TB/s, and back in 142; 165 by whole groups).
 #include "mxfp4.h"
+#include "mxfp8.h"
 
 namespace pd {
 
@@ -39,14 +40,6 @@ __device__ __forceinline__ GroupAt group_at(int g, int H, int I) {
         for (int i = 0; i < 4; ++i) a.row[i] = (size_t)2 * I * H + (size_t)(rg * 64 + i * 16) * I;
     }
     return a;
-}
-
-// max of the values of lanes l, l ^ 16, l ^ 32 and l ^ 48, in each of them
-__device__ __forceinline__ uint32_t max_over_quarters(uint32_t v) {
-    const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    v = max(a[0], a[1]);
-    const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return max(b[0], b[1]);
 }
 
 // Eight bf16 values to a word of codes: times 2^(127 - byte) (exact), then the

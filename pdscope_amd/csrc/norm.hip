@@ -13,7 +13,16 @@
 // One workgroup per row, its values in registers from the first load to the last
 // store, so every byte moves once: bound by HBM for many rows, by the latency
 // of a load, two reductions and a store for one.
-#include "common.h"
+//
+// With 8-bit rows (MX) n also goes out as e4m3 codes with a scale per 32
+// channels (mxfp8.h), for the experts' products; out_norm is then optional.  A
+// thread's eight channels and its three neighbours' make a scale block.  Everything is
+// held in 64 bits then, and the codes are rounded from that: they do not depend
+// on the order of the sums, where 32 bits move one code in some hundred
+// thousand to its neighbour.  The vector units run 64-bit products at the 32-bit rate.
+#include <type_traits>
+
+#include "mxfp8.h"
 
 namespace pd {
 
@@ -30,10 +39,11 @@ struct NormArgs {
     int H;
     void *out_resid;
     uint16_t *out_norm;
+    uint8_t *out_codes, *out_scales;  // 8-bit rows [T, H] and [T, H / 32], or null
 };
 
 // Eight values of a row.  VEC: consecutive ones from 8 c on (16-byte aligned);
-// else values c, c + n, c + 2n, ...
+// else values c, c + n, c + 2n, ... (8-bit rows: consecutive ones, one at a time)
 template <bool VEC>
 struct Eight {
     int at, step;
@@ -94,50 +104,66 @@ __device__ __forceinline__ void store8(void *base, const Eight<VEC> &e, int H, c
     }
 }
 
+__device__ __forceinline__ float row_sum(float v) { return wave_sum_dpp(v); }
+__device__ __forceinline__ double row_sum(double v) { return wave_sum(v); }
+
 // Sum over the workgroup, the same in every thread: waves in order.
-__device__ __forceinline__ float block_sum(float v, float *s_sum) {
-    v = wave_sum_dpp(v);
+template <typename F>
+__device__ __forceinline__ F block_sum(F v, F *s_sum) {
+    v = row_sum(v);
     const int nw = blockDim.x >> 6;
     if (nw == 1) return v;
     __syncthreads();  // s_sum may still be read from the sum before
     if (lane_id() == 0) s_sum[threadIdx.x >> 6] = v;
     __syncthreads();
-    float t = 0.0f;
+    F t = 0;
     for (int w = 0; w < nw; ++w) t += s_sum[w];
     return t;
 }
 
-// NV: eights of a row per thread.
-template <bool VEC, bool R32, bool P32, int NV>
+// 1 / sqrt(mean + eps), correctly rounded root and quotient
+__device__ __forceinline__ float inv_rms(float sum, int H, float eps) { return 1.0f / sqrtf(sum / (float)H + eps); }
+__device__ __forceinline__ double inv_rms(double sum, int H, float eps) { return 1.0 / sqrt(sum / (double)H + (double)eps); }
+
+// What is stored of a value: itself, or the 32-bit value that keeps for any
+// shorter type on which side of its borders a 64-bit one lies.
+__device__ __forceinline__ float narrow(float v) { return v; }
+__device__ __forceinline__ float narrow(double v) { return round_to_odd(v); }
+
+// NV: eights of a row per thread; MX: 8-bit rows as well.
+template <bool VEC, bool R32, bool P32, int NV, bool MX>
 __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
-    __shared__ float s_sum[16];
+    using F = std::conditional_t<MX, double, float>;
+    __shared__ F s_sum[16];
     const int t = blockIdx.x, H = a.H, n = blockDim.x;
     Eight<VEC> at[NV];
     bool on[NV];  // has values of the row (every thread keeps its place in the sums)
-    float v[NV][8], res[NV][8];
+    F v[NV][8];
+    float res[NV][8];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int q = threadIdx.x + j * n;
-        at[j] = VEC ? Eight<VEC>{8 * q, 1} : Eight<VEC>{(int)threadIdx.x + j * 8 * n, n};
+        at[j] = VEC || MX ? Eight<VEC>{8 * q, 1} : Eight<VEC>{(int)threadIdx.x + j * 8 * n, n};
         on[j] = at[j].at < H;
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[j][i] = res[j][i] = 0.0f;
         if (!on[j]) continue;
         load8<VEC, R32>((const char *)a.resid + (size_t)t * H * (R32 ? 4 : 2), at[j], H, res[j]);
-        if (a.k == 0) {
-            load8<VEC, false>(a.block + (size_t)t * H, at[j], H, v[j]);
-        } else if (a.add_in) {
-            load8<VEC, false>(a.add_in + (size_t)t * H, at[j], H, v[j]);
+        if (a.k == 0 || a.add_in) {
+            float b[8];
+            load8<VEC, false>((a.k == 0 ? a.block : a.add_in) + (size_t)t * H, at[j], H, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j][i] = b[i];
         }
     }
     if (a.k) {
-        // slot order, fp32; a row outside y (an expert computed elsewhere) adds nothing
+        // slot order; a row outside y (an expert computed elsewhere) adds nothing
         const int32_t *rows = a.row_of + (size_t)t * a.k;
         const uint16_t *ws = a.w + (size_t)t * a.k;
 #pragma unroll 8
         for (int s = 0; s < a.k; ++s) {
             const int32_t row = rows[s];
-            const float w = bf2f(ws[s]);
+            const F w = bf2f(ws[s]);
             if (row < 0 || row >= a.y_rows) continue;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
@@ -145,23 +171,23 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
                 float y[8];
                 load8<VEC, false, true>(a.block + (size_t)row * H, at[j], H, y);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[j][i] = fmaf(w, y[i], v[j][i]);
+                for (int i = 0; i < 8; ++i) v[j][i] = fma(w, (F)y[i], v[j][i]);
             }
         }
     }
-    float f = a.scale;
+    F f = a.scale;
     if (a.gate && !a.gate_cols)
         f *= P32 ? ((const float *)a.gate)[a.gate_rows ? t : 0] : bf2f(((const uint16_t *)a.gate)[a.gate_rows ? t : 0]);
     if (a.post_w) {
-        float q = 0.0f;
+        F q = 0;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (on[j] && at[j].idx(i) < H) q = fmaf(v[j][i], v[j][i], q);
-        f *= 1.0f / sqrtf(block_sum(q, s_sum) / (float)H + a.eps);
+                if (on[j] && at[j].idx(i) < H) q = fma(v[j][i], v[j][i], q);
+        f *= inv_rms(block_sum(q, s_sum), H, a.eps);
     }
-    float q = 0.0f;
+    F q = 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         if (!on[j]) continue;
@@ -178,13 +204,18 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            v[j][i] = fmaf(f, v[j][i], res[j][i]);
-            if (at[j].idx(i) < H) q = fmaf(v[j][i], v[j][i], q);
+            v[j][i] = fma(f, v[j][i], (F)res[j][i]);
+            if (at[j].idx(i) < H) q = fma(v[j][i], v[j][i], q);
         }
-        if (a.out_resid) store8<VEC, R32>((char *)a.out_resid + (size_t)t * H * (R32 ? 4 : 2), at[j], H, v[j]);
+        if (a.out_resid) {
+            float r[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = R32 ? (float)v[j][i] : narrow(v[j][i]);
+            store8<VEC, R32>((char *)a.out_resid + (size_t)t * H * (R32 ? 4 : 2), at[j], H, r);
+        }
     }
-    if (!a.out_norm) return;
-    const float rs = 1.0f / sqrtf(block_sum(q, s_sum) / (float)H + a.eps);
+    if (!MX && !a.out_norm) return;
+    const F rs = inv_rms(block_sum(q, s_sum), H, a.eps);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         if (!on[j]) continue;
@@ -197,28 +228,51 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[j][i] *= rs;
         }
-        store8<VEC, false>(a.out_norm + (size_t)t * H, at[j], H, v[j]);
+        float o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = narrow(v[j][i]);
+        if (!MX || a.out_norm) store8<VEC, false>(a.out_norm + (size_t)t * H, at[j], H, o);
+        if constexpr (MX) {
+            const uint32_t byte = mx8_scale_byte(max_over_quad(top_magnitude8(o)));
+            const uint2 c = mx8_encode8(o, byte);
+            uint8_t *codes = a.out_codes + (size_t)t * H + at[j].at;
+            if (VEC) {
+                *reinterpret_cast<uint2 *>(codes) = c;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) codes[i] = (uint8_t)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+            }
+            if ((threadIdx.x & 3) == 0) a.out_scales[((size_t)t * H + at[j].at) / 32] = (uint8_t)byte;
+        }
     }
 }
 
 constexpr int kNormMaxH = 16384;
 
-template <bool VEC, bool R32, bool P32>
+template <bool VEC, bool R32, bool P32, bool MX>
 static void norm_launch(const NormArgs &a, int T, hipStream_t s) {
     const int n = (a.H + 511) / 512 * 64;  // eight values a thread
-    if (n <= 1024) norm_kernel<VEC, R32, P32, 1><<<T, n, 0, s>>>(a);
-    else norm_kernel<VEC, R32, P32, 2><<<T, (n / 2 + 63) / 64 * 64, 0, s>>>(a);
+    if (n <= 1024) norm_kernel<VEC, R32, P32, 1, MX><<<T, n, 0, s>>>(a);
+    else norm_kernel<VEC, R32, P32, 2, MX><<<T, (n / 2 + 63) / 64 * 64, 0, s>>>(a);
+}
+
+template <bool VEC, bool R32, bool P32>
+static void norm_launch(const NormArgs &a, int T, hipStream_t s) {
+    if (a.out_codes) norm_launch<VEC, R32, P32, true>(a, T, s);
+    else norm_launch<VEC, R32, P32, false>(a, T, s);
 }
 
 static int norm_call(const char *what, const NormArgs &a, int resid_f32, int params_f32, int T, void *stream) {
     // a row of up to 1024 threads: fewer than 2^32 in a launch
     if (T < 1 || T >= (1 << 22) || a.H < 1 || a.H > kNormMaxH)
         return fail(kEInval, std::string(what) + ": need T >= 1 and below 2^22, and 1 <= H <= 16384");
-    if (!a.block || !a.resid || (!a.out_resid && !a.out_norm)) return fail(kEInval, std::string(what) + ": null pointer");
+    if (!a.block || !a.resid || (!a.out_resid && !a.out_norm && !a.out_codes))
+        return fail(kEInval, std::string(what) + ": null pointer");
+    if (a.out_codes && a.H % 32) return fail(kEInval, std::string(what) + ": 8-bit rows need H % 32 == 0");
     if (!(a.eps >= 0.0f)) return fail(kEInval, std::string(what) + ": eps must not be negative");
     bool vec = a.H % 8 == 0;
     for (const void *p : {(const void *)a.block, (const void *)a.add_in, a.resid, a.post_w, a.gate_cols ? a.gate : nullptr,
-                          a.pre_w, (const void *)a.out_resid, (const void *)a.out_norm})
+                          a.pre_w, (const void *)a.out_resid, (const void *)a.out_norm, (const void *)a.out_codes})
         vec = vec && reinterpret_cast<uintptr_t>(p) % 16 == 0;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const int variant = (vec ? 4 : 0) | (resid_f32 ? 2 : 0) | (params_f32 ? 1 : 0);
@@ -244,7 +298,7 @@ PD_API int pdscope_norm_residual(const void *block, const void *resid, int resid
                                  int params_f32, float eps, int T, int H, void *out_resid, void *out_norm,
                                  void *stream) {
     const NormArgs a{(const uint16_t *)block, nullptr, nullptr, nullptr, 0, 0, resid, post_w, gate, pre_w,
-                     gate_rows, gate_cols, scale, eps, H, out_resid, (uint16_t *)out_norm};
+                     gate_rows, gate_cols, scale, eps, H, out_resid, (uint16_t *)out_norm, nullptr, nullptr};
     return norm_call("norm_residual", a, resid_f32, params_f32, T, stream);
 }
 
@@ -256,6 +310,31 @@ PD_API int pdscope_merge_norm_residual(const void *y, int64_t y_rows, const int3
     if (!row_of || !w) return fail(kEInval, "merge_norm_residual: null pointer");
     if (k < 1 || y_rows < 1) return fail(kEInval, "merge_norm_residual: need k >= 1 and y_rows >= 1");
     const NormArgs a{(const uint16_t *)y, row_of, (const uint16_t *)w, (const uint16_t *)add_in, y_rows, k, resid, post_w,
-                     gate, pre_w, gate_rows, gate_cols, scale, eps, H, out_resid, (uint16_t *)out_norm};
+                     gate, pre_w, gate_rows, gate_cols, scale, eps, H, out_resid, (uint16_t *)out_norm, nullptr, nullptr};
     return norm_call("merge_norm_residual", a, resid_f32, params_f32, T, stream);
+}
+
+PD_API int pdscope_norm_residual_mxfp8(const void *block, const void *resid, int resid_f32, const void *post_w,
+                                       const void *gate, int gate_rows, int gate_cols, float scale, const void *pre_w,
+                                       int params_f32, float eps, int T, int H, void *out_resid, void *out_norm,
+                                       void *out_codes, void *out_scales, void *stream) {
+    if (!out_codes || !out_scales) return fail(kEInval, "norm_residual_mxfp8: null pointer");
+    const NormArgs a{(const uint16_t *)block, nullptr, nullptr, nullptr, 0, 0, resid, post_w, gate, pre_w,
+                     gate_rows, gate_cols, scale, eps, H, out_resid, (uint16_t *)out_norm, (uint8_t *)out_codes,
+                     (uint8_t *)out_scales};
+    return norm_call("norm_residual_mxfp8", a, resid_f32, params_f32, T, stream);
+}
+
+PD_API int pdscope_merge_norm_residual_mxfp8(const void *y, int64_t y_rows, const int32_t *row_of, const void *w, int k,
+                                             const void *add_in, const void *resid, int resid_f32, const void *post_w,
+                                             const void *gate, int gate_rows, int gate_cols, float scale,
+                                             const void *pre_w, int params_f32, float eps, int T, int H,
+                                             void *out_resid, void *out_norm, void *out_codes, void *out_scales,
+                                             void *stream) {
+    if (!row_of || !w || !out_codes || !out_scales) return fail(kEInval, "merge_norm_residual_mxfp8: null pointer");
+    if (k < 1 || y_rows < 1) return fail(kEInval, "merge_norm_residual_mxfp8: need k >= 1 and y_rows >= 1");
+    const NormArgs a{(const uint16_t *)y, row_of, (const uint16_t *)w, (const uint16_t *)add_in, y_rows, k, resid, post_w,
+                     gate, pre_w, gate_rows, gate_cols, scale, eps, H, out_resid, (uint16_t *)out_norm,
+                     (uint8_t *)out_codes, (uint8_t *)out_scales};
+    return norm_call("merge_norm_residual_mxfp8", a, resid_f32, params_f32, T, stream);
 }

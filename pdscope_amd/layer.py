@@ -14,13 +14,14 @@ import torch
 from . import ops
 
 BF16 = torch.bfloat16
+ACTIVATIONS = ("bf16", "mxfp8")
 
 
 class MoEWorkspace:
     """Device buffers for up to ``max_tokens`` tokens of one layer shape."""
 
     def __init__(self, max_tokens: int, H: int, I: int, E: int, k: int, device, *, route_only: bool = False,
-                 shared_I: int | None = None, few_tokens: bool = False):
+                 shared_I: int | None = None, few_tokens: bool = False, mxfp8: bool = False):
         device = torch.device(device)
         n = max_tokens * k
         i32 = dict(dtype=torch.int32, device=device)
@@ -52,6 +53,9 @@ class MoEWorkspace:
             if need == 0:
                 raise ValueError("this layer shape is outside moe_few (ops.moe_few_supported)")
             self.few_ws = torch.empty(need, dtype=torch.uint8, device=device)
+        # 8-bit rows of x for moe_forward(activations="mxfp8") without rows of the caller's
+        self.x_rows = ops.mxfp8_empty(max_tokens, H, device) if mxfp8 else None
+        self._h_rows = None
         # always-on shared experts (one fused MLP of intermediate shared_I over every token)
         self.shared_I = shared_I
         if shared_I:
@@ -76,6 +80,16 @@ class MoEWorkspace:
             buf = torch.empty((max(n, self.max_tokens * self.k), self.H), dtype=BF16, device=self.device)
             self._xg = buf
         return buf[:n]
+
+    def h_rows(self) -> ops.MxRows:
+        """The hidden rows' buffer as 8-bit rows [rows, I] (in h_ws' first bytes)."""
+        if self._h_rows is None:
+            n = self.h_ws.numel()
+            rows = n // self.I
+            raw = self.h_ws.view(torch.uint8)
+            self._h_rows = ops.MxRows(raw[:n].view(ops.F8).view(rows, self.I),
+                                      raw[n:n + n // 32].view(rows, self.I // 32))
+        return self._h_rows
 
     def identity_rows(self, n: int) -> torch.Tensor:
         """int32 [n] = 0..n-1: the row map of activations already in grouped order."""
@@ -155,10 +169,15 @@ def experts_resident(x, ids, weights, slots, ws: MoEWorkspace, out=None, *, bloc
     merge: 'fused' (fp32 sum, one rounding) or 'reference' (bf16 adds in
     ascending expert id, the reference runtime's default merge).
     representation: what `slots` addresses, "bf16" or "mxfp4" blocks (4-bit, any
-    T: K2, their grouped launches, K5; shared experts' output comes through add_in)."""
-    T = x.shape[0]
+    T: K2, their grouped launches, K5; shared experts' output comes through add_in).
+    x: bf16 rows, or 8-bit ones (ops.MxRows) for 4-bit experts, whose products then
+    run on 8-bit rows throughout."""
+    mx8 = isinstance(x, ops.MxRows)
+    T = x.codes.shape[0] if mx8 else x.shape[0]
     H, I, E, k = ws.H, ws.I, ws.E, ws.k
     out = ws.out[:T] if out is None else out
+    if mx8 and not ops.is_mxfp4(representation):
+        raise ValueError('8-bit rows need 4-bit experts (representation="mxfp4")')
     if ops.is_mxfp4(representation):
         if shared_slot is not None:
             raise ValueError("shared experts join 4-bit routed experts through add_in")
@@ -171,10 +190,11 @@ def experts_resident(x, ids, weights, slots, ws: MoEWorkspace, out=None, *, bloc
         for t, name in ((out, "out"), (add_in, "add_in")):
             if t is not None and (t.ndim != 2 or t.shape[0] < T or t.shape[1] != H):
                 raise ValueError(f"{name} must be [{T}, {H}], got {list(t.shape)}")
-        bm = block_m or ops.grouped_mxfp4_block_m((T * k) // E)
+        bm = block_m or (ops.grouped_mxfp8_block_m if mx8 else ops.grouped_mxfp4_block_m)((T * k) // E)
         ops.pack(ids, E, out=packed, workspace=ws.pack_ws, schedule=(ws.sel_all, bm, ws.sel_order, ws.tile_start))
-        ops.swiglu_grouped_mxfp4(x, packed.perm_token, packed.offsets, ws.sel_order, ws.tile_start,
-                                 (T * k + bm - 1) // bm + E, bm, slots, H, I, ws.h_ws, ws.y)
+        grouped = ops.swiglu_grouped_mxfp8 if mx8 else ops.swiglu_grouped_mxfp4
+        grouped(x, packed.perm_token, packed.offsets, ws.sel_order, ws.tile_start, (T * k + bm - 1) // bm + E, bm,
+                slots, H, I, ws.h_rows() if mx8 else ws.h_ws, ws.y)
         if before_merge is not None:
             before_merge()
         ops.merge(ws.y, packed.row_of, weights, out, add_in=add_in, mode=merge)
@@ -252,7 +272,8 @@ def moe_few(x, gate, slots, ws: MoEWorkspace, *, normalize=True, bias=None, add_
 
 
 def moe_forward(x, gate, slots, ws: MoEWorkspace, *, normalize=True, bias=None, block_m=None, fused_decode=True,
-                shared_slot=None, merge="fused", next_gate=None, pred_out=None, representation="bf16"):
+                shared_slot=None, merge="fused", next_gate=None, pred_out=None, representation="bf16",
+                activations="bf16", x_rows=None):
     """Full layer: returns (out [T,H] bf16, logits, ids int32 [T,k], weights bf16 [T,k]).
 
     merge: 'fused' (each token's k weighted rows summed in fp32, one
@@ -271,8 +292,23 @@ def moe_forward(x, gate, slots, ws: MoEWorkspace, *, normalize=True, bias=None, 
     experts take up to 16 tokens through moe_few where the workspace was built
     with few_tokens=True and merge is 'fused', and more through route (K1) and
     their grouped launches; shared experts stay bf16 (one MLP, read once for all tokens).
+    activations: "bf16", or "mxfp8" to run the grouped products of 4-bit experts on 8-bit
+    rows: x_rows (ops.MxRows of x, as the norm before the layer writes them) where
+    given, else x quantised here (the workspace must have been built with
+    mxfp8=True).  Router, shared experts and moe_few take x in bf16 all the same.
     """
     T = x.shape[0]
+    if activations not in ACTIVATIONS:
+        raise ValueError(f"activations must be one of {ACTIVATIONS}, got {activations!r}")
+    if activations == "mxfp8":
+        if not ops.is_mxfp4(representation):
+            raise ValueError('8-bit rows need 4-bit experts (representation="mxfp4")')
+        if x_rows is None and ws.x_rows is None:
+            raise ValueError("8-bit activations need x_rows or a workspace built with mxfp8=True")
+        if x_rows is not None and (not isinstance(x_rows, ops.MxRows) or x_rows.codes.shape != x.shape):
+            raise ValueError(f"x_rows must be MxRows of {list(x.shape)}")
+    elif x_rows is not None:
+        raise ValueError('x_rows are read with activations="mxfp8"')
     if ops.is_mxfp4(representation):
         if next_gate is not None or pred_out is not None:
             raise ValueError("the fused next-layer prediction needs bf16 experts")
@@ -285,7 +321,12 @@ def moe_forward(x, gate, slots, ws: MoEWorkspace, *, normalize=True, bias=None, 
             return moe_few(x, gate, slots, ws, normalize=normalize, bias=bias, add_in=y_shared,
                            representation=representation)
         logits, ids, weights = route(x, gate, ws, normalize=normalize, bias=bias)
-        out = experts_resident(x, ids, weights, slots, ws, block_m=block_m, add_in=y_shared, merge=merge,
+        rows = x
+        if activations == "mxfp8":
+            rows = x_rows
+            if rows is None:
+                rows = ops.mxfp8_quantize(x, out=ops.MxRows(ws.x_rows.codes[:T], ws.x_rows.scales[:T]))
+        out = experts_resident(rows, ids, weights, slots, ws, block_m=block_m, add_in=y_shared, merge=merge,
                                representation=representation)
         return out, logits, ids, weights
     if shared_slot is not None:

@@ -804,6 +804,205 @@ def swiglu_grouped_mxfp4(x, perm_token, offsets, sel, tile_start, max_tiles, blo
     return y
 
 
+# ------------------------------------------------------------- 8-bit rows
+
+F8 = torch.float8_e4m3fn
+
+
+@dataclass
+class MxRows:
+    """8-bit rows: e4m3 codes with one e8m0 scale 2^(byte - 127) per 32 consecutive values."""
+    codes: torch.Tensor   # float8_e4m3fn [T, n]
+    scales: torch.Tensor  # uint8 [T, n / 32]
+
+
+def _need_rows(rows, name, T, n, device):
+    if not isinstance(rows, MxRows):
+        raise ValueError(f"{name} must be MxRows")
+    _need(rows.codes, f"{name}.codes", F8, 2, device)
+    _need(rows.scales, f"{name}.scales", torch.uint8, 2, rows.codes.device)
+    shape = tuple(rows.codes.shape)
+    if shape != (shape[0] if T is None else T, shape[1] if n is None else n):
+        raise ValueError(f"{name}.codes must be [{T}, {n}], got {list(shape)}")
+    if shape[1] % 32 or tuple(rows.scales.shape) != (shape[0], shape[1] // 32):
+        raise ValueError(f"{name}.scales must be [T, n / 32] of codes [T, n] with n % 32 == 0, got "
+                         f"{list(rows.scales.shape)} for {list(shape)}")
+
+
+def mxfp8_empty(T, n, device) -> MxRows:
+    """8-bit rows to be written: codes [T, n], scales [T, n / 32]."""
+    if n % 32:
+        raise ValueError(f"8-bit rows need a length of whole blocks of 32, got {n}")
+    return MxRows(torch.empty((T, n), dtype=F8, device=device),
+                  torch.empty((T, n // 32), dtype=torch.uint8, device=device))
+
+
+def mxfp8_quantize(x, out: MxRows | None = None) -> MxRows:
+    """8-bit rows of bf16 rows x [T, n], n % 32 == 0 (see pdscope_mxfp8_quantize for the rounding)."""
+    _need(x, "x", BF16, 2)
+    T, n = x.shape
+    if out is None:
+        out = mxfp8_empty(T, n, x.device)
+    else:
+        _need_rows(out, "out", T, n, x.device)
+    if T:
+        _call_on(x.device, "pdscope_mxfp8_quantize", _p(x), T, n, _p(out.codes), _p(out.scales))
+    return out
+
+
+def mxfp8_dequantize(rows: MxRows, out=None) -> torch.Tensor:
+    """The values of 8-bit rows as bf16 [T, n]: exact from 2^-126 on."""
+    _need_rows(rows, "rows", None, None, None)
+    T, n = rows.codes.shape
+    if out is None:
+        out = torch.empty((T, n), dtype=BF16, device=rows.codes.device)
+    elif not _fits(out, BF16, (T, n), rows.codes.device):
+        _refuse(out, "out", BF16, (T, n), rows.codes.device)
+    if T:
+        _call_on(out.device, "pdscope_mxfp8_dequantize", _p(rows.codes), _p(rows.scales), T, n, _p(out))
+    return out
+
+
+def grouped_mxfp8_block_m(rows_hint: int) -> int:
+    """Row tile of swiglu_grouped_mxfp8 for rows_hint mean rows per expert."""
+    return int(_lib.load().pdscope_grouped_mxfp8_block_m(int(rows_hint)))
+
+
+def swiglu_grouped_mxfp8(x: MxRows, perm_token, offsets, sel, tile_start, max_tiles, block_m, slots, H, I,
+                         h_ws: MxRows, y):
+    """swiglu_grouped_mxfp4 over 8-bit rows x; the experts' hidden rows go through h_ws
+    [rows, I] as 8-bit rows too (see pdscope_swiglu_grouped_mxfp8); block_m 32 or 64."""
+    _need_rows(x, "inputs", None, H, None)
+    dev = x.codes.device
+    for t, n in ((perm_token, "perm_token"), (offsets, "offsets"), (sel, "sel"), (tile_start, "tile_start")):
+        _need(t, n, torch.int32, 1, dev)
+    _need(slots, "slots", torch.int64, 1, dev)
+    _need_rows(h_ws, "h_ws", None, I, dev)
+    _need(y, "y", BF16, None, dev)
+    check_slots(slots, H, I, "mxfp4")
+    if h_ws.codes.shape[0] < perm_token.numel() or y.numel() < perm_token.numel() * H:
+        raise ValueError("h_ws / y workspaces are smaller than rows x I / rows x H")
+    if tile_start.numel() < sel.numel() + 1 or offsets.numel() < 2:
+        raise ValueError("tile_start must hold one entry more than sel, offsets one more than there are experts")
+    if slots.numel() < offsets.numel() - 1:
+        raise ValueError("slots must hold one entry per expert")
+    if max(x.codes.numel(), perm_token.numel() * I) >= 1 << 36:
+        raise ValueError("swiglu_grouped_mxfp8 addresses fewer than 2^36 activations")
+    _call_on(dev, "pdscope_swiglu_grouped_mxfp8", _p(x.codes), _p(x.scales), _p(perm_token), _p(offsets), _p(sel),
+             sel.numel(), _p(tile_start), int(max_tiles), int(block_m), _p(slots), H, I, _p(h_ws.codes),
+             _p(h_ws.scales), _p(y))
+    return y
+
+
+# ------------------------------------------- 4-bit matrices with group scales
+
+@dataclass
+class Int4Weight:
+    """A 4-bit matrix [N, K] with a scale for each `group` inputs of a row, laid out by
+    int4_pack or int4_quantize."""
+    units: torch.Tensor  # uint8 [int4_bytes(N, K, group, zeros)]
+    N: int
+    K: int
+    group: int
+    zeros: bool          # zero points, or 8 throughout
+    scale_dtype: torch.dtype = BF16
+
+
+def int4_bytes(N: int, K: int, group: int, zeros: bool = False) -> int:
+    """Bytes of a laid-out 4-bit matrix."""
+    n = int(_lib.load().pdscope_int4_bytes(int(N), int(K), int(group), int(bool(zeros))))
+    if n == 0:
+        raise ValueError(f"4-bit matrices need N >= 1, groups of 32, 64 or 128 inputs and K % group == 0, got N={N}, "
+                         f"K={K}, group={group}")
+    return n
+
+
+def _int4_out(out, N, K, group, zeros, scale_dtype, device):
+    need = int4_bytes(N, K, group, zeros)
+    if out is None:
+        out = torch.empty(need, dtype=torch.uint8, device=device)
+    _need(out, "out", torch.uint8, 1, device)
+    if out.numel() != need:
+        raise ValueError(f"out must hold {need} bytes, got {out.numel()}")
+    return Int4Weight(out, N, K, group, zeros, scale_dtype)
+
+
+def int4_pack(codes, scales, zeros=None, out=None) -> Int4Weight:
+    """A checkpoint's tensors laid out: codes uint8 [N, K/2] (two whole numbers 0..15
+    a byte, the first in the low half), scales bf16 or fp16 [N, K/group], zero points
+    uint8 [N, K/group] (0..15) or None (8).  W = scale * (code - zero)."""
+    _need(codes, "codes", torch.uint8, 2)
+    dev = codes.device
+    _need(scales, "scales", None, 2, dev)
+    if scales.dtype not in (BF16, torch.float16):
+        raise ValueError(f"scales must be bf16 or fp16, got {scales.dtype}")
+    N, K = codes.shape[0], 2 * codes.shape[1]
+    groups = scales.shape[1]
+    if scales.shape[0] != N or groups < 1 or K % groups:
+        raise ValueError(f"scales must be [{N}, {K} / group], got {list(scales.shape)}")
+    if zeros is not None:
+        _need(zeros, "zeros", torch.uint8, 2, dev)
+        if zeros.shape != scales.shape:
+            raise ValueError(f"zeros must be {list(scales.shape)}, got {list(zeros.shape)}")
+    w = _int4_out(out, N, K, K // groups, zeros is not None, scales.dtype, dev)
+    _call_on(dev, "pdscope_int4_pack", _p(codes), _p(scales), _p(zeros), N, K, w.group, _p(w.units))
+    return w
+
+
+def int4_quantize(weight, group=128, zeros=False, out=None) -> Int4Weight:
+    """4-bit form of a bf16 matrix [N, K] (see pdscope_int4_quantize for the rounding);
+    zeros: a zero point for each group, else 8."""
+    _need(weight, "weight", BF16, 2)
+    N, K = weight.shape
+    w = _int4_out(out, N, K, int(group), bool(zeros), BF16, weight.device)
+    _call_on(weight.device, "pdscope_int4_quantize", _p(weight), N, K, w.group, int(w.zeros), _p(w.units))
+    return w
+
+
+def _need_int4(w, device=None):
+    if not isinstance(w, Int4Weight):
+        raise ValueError("weight must be an Int4Weight")
+    _need(w.units, "weight.units", torch.uint8, 1, device)
+    if w.units.numel() != int4_bytes(w.N, w.K, w.group, w.zeros):
+        raise ValueError("weight.units is not of the size of its shape")
+    if w.scale_dtype not in (BF16, torch.float16):
+        raise ValueError(f"scales must be bf16 or fp16, got {w.scale_dtype}")
+
+
+def int4_dequantize(w: Int4Weight, out=None) -> torch.Tensor:
+    """The values of a 4-bit matrix as bf16 [N, K], each rounded once."""
+    _need_int4(w)
+    dev = w.units.device
+    if out is None:
+        out = torch.empty((w.N, w.K), dtype=BF16, device=dev)
+    elif not _fits(out, BF16, (w.N, w.K), dev):
+        _refuse(out, "out", BF16, (w.N, w.K), dev)
+    _call_on(dev, "pdscope_int4_dequantize", _p(w.units), w.N, w.K, w.group, int(w.zeros),
+             int(w.scale_dtype is torch.float16), _p(out))
+    return out
+
+
+def linear_int4(x, w: Int4Weight, bias=None, out=None) -> torch.Tensor:
+    """x [T, K] bf16 times a 4-bit matrix: bf16 [T, N] = x W^T + bias ([N] bf16 or
+    None), rounded once; any T (see pdscope_linear_int4)."""
+    _need(x, "x", BF16, 2)
+    dev = x.device
+    _need_int4(w, dev)
+    T, K = x.shape
+    if K != w.K:
+        raise ValueError(f"x must be [T, {w.K}], got {list(x.shape)}")
+    if bias is not None and not _fits(bias, BF16, (w.N,), dev):
+        _refuse(bias, "bias", BF16, (w.N,), dev)
+    if out is None:
+        out = torch.empty((T, w.N), dtype=BF16, device=dev)
+    elif not _fits(out, BF16, (T, w.N), dev):
+        _refuse(out, "out", BF16, (T, w.N), dev)
+    if T:
+        _call_on(dev, "pdscope_linear_int4", _p(x), _p(w.units), _p(bias), T, w.N, K, w.group, int(w.zeros),
+                 int(w.scale_dtype is torch.float16), _p(out))
+    return out
+
+
 # --------------------------------------------------------- a few tokens' layer
 
 FEW_MAX_TOKENS = 16
@@ -872,7 +1071,7 @@ def _refuse(t, name, dtype, shape, dev):
     raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
 
 
-def _norm_args(T, H, dev, resid, post_weight, gate, pre_weight, out_resid, out_norm, want_resid):
+def _norm_args(T, H, dev, resid, post_weight, gate, pre_weight, out_resid, out_norm, want_resid, want_norm):
     """Checks of norm_residual / merge_norm_residual and their allocated outputs."""
     shape = (T, H)
     R = resid.dtype if isinstance(resid, torch.Tensor) else None
@@ -910,32 +1109,51 @@ def _norm_args(T, H, dev, resid, post_weight, gate, pre_weight, out_resid, out_n
     elif want_resid:
         out_resid = torch.empty_like(resid)
     if out_norm is None:
-        out_norm = torch.empty_like(resid, dtype=BF16)
+        if want_norm:
+            out_norm = torch.empty_like(resid, dtype=BF16)
     elif not _fits(out_norm, BF16, shape, dev):
         _refuse(out_norm, "out_norm", BF16, shape, dev)
     return int(R is torch.float32), rows, cols, int(P is torch.float32), out_resid, out_norm
 
 
+def _mx_out(out_mxfp8, T, H, dev):
+    """The 8-bit rows that a norm writes."""
+    if out_mxfp8 is None:
+        return mxfp8_empty(T, H, dev)
+    _need_rows(out_mxfp8, "out_mxfp8", T, H, dev)
+    return out_mxfp8
+
+
 def norm_residual(block, resid, *, post_weight=None, gate=None, scale=1.0, pre_weight=None, eps=1e-6, out_resid=None,
-                  out_norm=None, want_resid=True):
+                  out_norm=None, want_resid=True, want_norm=True, want_mxfp8=False, out_mxfp8=None):
     """The norm after a block (post_weight [H]; None: none), its gate and
     residual scale, the residual sum and the norm before the next block
     (pre_weight [H]; None: ones) in one launch: returns (resid + scale * gate *
     norm(block), its RMS norm as bf16).  block [T, H] bf16; resid [T, H] bf16
     or fp32 (the sum has its type; out_resid may be resid); weights and gate
     ([H], [T, 1] or [T, H]) bf16 or fp32, all alike.  want_resid=False without
-    out_resid computes the norm alone and returns None for the sum."""
+    out_resid computes the norm alone and returns None for the sum.
+    want_mxfp8 (or out_mxfp8, an MxRows of that shape) also writes the norm as 8-bit
+    rows, rounded from the unrounded norm, and returns them third; H % 32 == 0.
+    Then want_norm=False without out_norm leaves the bf16 norm out (None)."""
     _need(block, "block", BF16, 2)
     T, H = block.shape
+    mx = want_mxfp8 or out_mxfp8 is not None
     f32, rows, cols, p32, out_resid, out_norm = _norm_args(T, H, block.device, resid, post_weight, gate, pre_weight,
-                                                           out_resid, out_norm, want_resid)
-    _call_on(block.device, "pdscope_norm_residual", _p(block), _p(resid), f32, _p(post_weight), _p(gate), rows, cols,
-             float(scale), _p(pre_weight), p32, float(eps), T, H, _p(out_resid), _p(out_norm))
-    return out_resid, out_norm
+                                                           out_resid, out_norm, want_resid, want_norm or not mx)
+    args = (_p(block), _p(resid), f32, _p(post_weight), _p(gate), rows, cols, float(scale), _p(pre_weight), p32,
+            float(eps), T, H, _p(out_resid), _p(out_norm))
+    if not mx:
+        _call_on(block.device, "pdscope_norm_residual", *args)
+        return out_resid, out_norm
+    out = _mx_out(out_mxfp8, T, H, block.device)
+    _call_on(block.device, "pdscope_norm_residual_mxfp8", *args, _p(out.codes), _p(out.scales))
+    return out_resid, out_norm, out
 
 
 def merge_norm_residual(y, row_of, w, resid, *, add_in=None, post_weight=None, gate=None, scale=1.0, pre_weight=None,
-                        eps=1e-6, out_resid=None, out_norm=None, want_resid=True):
+                        eps=1e-6, out_resid=None, out_norm=None, want_resid=True, want_norm=True, want_mxfp8=False,
+                        out_mxfp8=None):
     """norm_residual of the experts' weighted merge, which is summed in the same
     launch (as merge(y, row_of, w, add_in=add_in) in mode 'fused', and not rounded):
     y [rows, H] grouped expert rows, row_of [T*k] int32 (an entry outside
@@ -955,12 +1173,17 @@ def merge_norm_residual(y, row_of, w, resid, *, add_in=None, post_weight=None, g
         _need(add_in, "add_in", BF16, 2, dev)
         if tuple(add_in.shape) != (T, H):
             raise ValueError(f"add_in must be [{T}, {H}], got {list(add_in.shape)}")
+    mx = want_mxfp8 or out_mxfp8 is not None
     f32, rows, cols, p32, out_resid, out_norm = _norm_args(T, H, dev, resid, post_weight, gate, pre_weight, out_resid,
-                                                           out_norm, want_resid)
-    _call_on(dev, "pdscope_merge_norm_residual", _p(y), y.numel() // H, _p(row_of), _p(w), k, _p(add_in), _p(resid),
-             f32, _p(post_weight), _p(gate), rows, cols, float(scale), _p(pre_weight), p32, float(eps), T, H,
-             _p(out_resid), _p(out_norm))
-    return out_resid, out_norm
+                                                           out_norm, want_resid, want_norm or not mx)
+    args = (_p(y), y.numel() // H, _p(row_of), _p(w), k, _p(add_in), _p(resid), f32, _p(post_weight), _p(gate), rows,
+            cols, float(scale), _p(pre_weight), p32, float(eps), T, H, _p(out_resid), _p(out_norm))
+    if not mx:
+        _call_on(dev, "pdscope_merge_norm_residual", *args)
+        return out_resid, out_norm
+    out = _mx_out(out_mxfp8, T, H, dev)
+    _call_on(dev, "pdscope_merge_norm_residual_mxfp8", *args, _p(out.codes), _p(out.scales))
+    return out_resid, out_norm, out
 
 
 def stage_expert(dst, src, *, event=None, stream=None):

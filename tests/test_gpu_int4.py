@@ -1,0 +1,210 @@
+"""4-bit matrices with group scales: layout, quantising and the products of 1 to a few thousand rows.
+
+The product's bound, with u = 2^-24: q x is exact, a group's two sums are off by (G + 2) u of their
+summed magnitudes, and what is made of them by 3 roundings a group, one a group's addition and one
+for each of up to 16 parts of the K axis: (G + K / G + 24) u (s (q + z) . |x|), then half a step of bf16."""
+import pytest
+import torch
+
+from moe64 import assert_within
+from pdscope_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F16 = torch.bfloat16, torch.float16
+U, B = 2.0 ** -24, 2.0 ** -8
+
+
+def make(N, K, G, *, zeros=False, dtype=BF16, seed=1):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, device=DEV, dtype=torch.uint8)
+    scales = (0.002 + 0.01 * torch.rand((N, K // G), generator=g, device=DEV)).to(dtype)
+    z = torch.randint(0, 16, (N, K // G), generator=g, device=DEV, dtype=torch.uint8) if zeros else None
+    return codes, scales, z
+
+
+def values64(codes, scales, z, G):
+    q = torch.stack([codes & 15, codes >> 4], -1).flatten(1).double()
+    z = torch.full_like(scales, 8.0, dtype=torch.float64) if z is None else z.double()
+    s = scales.double().repeat_interleave(G, 1)
+    z = z.repeat_interleave(G, 1)
+    return (q - z) * s, (q + z) * s.abs()
+
+
+def check(y, x, codes, scales, z, G, bias=None):
+    w, mass = values64(codes, scales, z, G)
+    K = x.shape[1]
+    want = x.double() @ w.T
+    bound = (G + K // G + 24) * U * (x.double().abs() @ mass.T)
+    if bias is not None:
+        want, bound = want + bias.double(), bound + 2 * U * bias.double().abs()
+    assert_within(y, want, (1 + B) * bound + B * want.abs() + 2.0 ** -133)
+
+
+@pytest.mark.parametrize("N,K,G", [(1, 32, 32), (16, 128, 128), (17, 160, 32), (5, 192, 64), (100, 2048, 128), (33, 4096, 64),
+                                   (250, 96, 32)])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_layout_round_trip(N, K, G, zeros, dtype):
+    codes, scales, z = make(N, K, G, zeros=zeros, dtype=dtype, seed=N + K)
+    w = ops.int4_pack(codes, scales, z)
+    assert (w.N, w.K, w.group, w.zeros, w.scale_dtype) == (N, K, G, zeros, dtype)
+    assert w.units.numel() == ops.int4_bytes(N, K, G, zeros)
+    q = torch.stack([codes & 15, codes >> 4], -1).flatten(1).float()
+    zf = 8.0 if z is None else z.float().repeat_interleave(G, 1)
+    assert torch.equal(ops.int4_dequantize(w), ((q - zf) * scales.float().repeat_interleave(G, 1)).to(BF16))
+
+
+@pytest.mark.parametrize("N,K,G", [(1, 32, 32), (31, 2048, 128), (64, 4096, 64), (77, 224, 32), (4096, 2048, 128)])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_quantise(N, K, G, zeros):
+    """The stated rule in torch's fp32, whose products, quotients and roundings are the same ones."""
+    g = torch.Generator(device=DEV).manual_seed(N)
+    weight = (0.02 * torch.randn((N, K), generator=g, device=DEV) + 0.01).to(BF16)
+    weight[0, :32] = 0
+    if N > 1:
+        weight[1] = 0.25
+    v = weight.float().unflatten(1, (-1, G))
+    if zeros:
+        lo, hi = (-v).amax(2).clamp(min=0), v.amax(2).clamp(min=0)
+        s = ((hi + lo) / 15).to(BF16).float()
+        z = torch.where(s > 0, torch.round(lo / s).clamp(max=15), torch.zeros_like(s))
+    else:
+        s = (v.abs().amax(2) / 7).to(BF16).float()
+        z = torch.full_like(s, 8.0)
+    q = torch.where(s.unsqueeze(2) > 0, torch.round(v / s.unsqueeze(2)) + z.unsqueeze(2), z.unsqueeze(2)).clamp(0, 15)
+    w = ops.int4_quantize(weight, G, zeros)
+    q = q.flatten(1).to(torch.uint8)
+    want = ops.int4_pack(q[:, 0::2] | (q[:, 1::2] << 4), s.to(BF16), z.to(torch.uint8) if zeros else None)
+    assert torch.equal(w.units, want.units)
+    # and near the matrix: half a step, two roundings of the scale's eight bits over 15 steps
+    step = s.repeat_interleave(G, 1)
+    assert ((ops.int4_dequantize(w).float() - weight.float()).abs() <= 0.5 * step + 0.14 * step + 2.0 ** -8 * weight.float().abs()).all()
+
+
+SIZES = [(1, 1, 32, 32), (1, 16, 128, 128), (2, 15, 64, 64), (1, 4096, 2048, 128), (3, 513, 4096, 64), (5, 4097, 2816, 32),
+         (15, 33, 96, 32), (16, 2048, 4096, 128), (17, 100, 352, 32), (31, 257, 768, 128), (33, 640, 1408, 128),
+         (48, 255, 2048, 64), (64, 1000, 1024, 32), (65, 129, 256, 64), (128, 512, 2048, 128), (200, 77, 160, 32),
+         (513, 384, 640, 128), (1031, 1100, 2048, 64), (2048, 256, 4096, 128)]
+
+
+@pytest.mark.parametrize("T,N,K,G", SIZES)
+@pytest.mark.parametrize("zeros,bias", [(False, False), (True, True)])
+def test_products(T, N, K, G, zeros, bias):
+    codes, scales, z = make(N, K, G, zeros=zeros, seed=T)
+    g = torch.Generator(device=DEV).manual_seed(N)
+    x = torch.randn((T, K), generator=g, device=DEV).to(BF16)
+    b = torch.randn(N, generator=g, device=DEV).to(BF16) if bias else None
+    w = ops.int4_pack(codes, scales, z)
+    y = ops.linear_int4(x, w, b)
+    check(y, x, codes, scales, z, G, b)
+    assert torch.equal(y, ops.linear_int4(x, w, b))
+
+
+@pytest.mark.parametrize("T", [1, 7, 40, 300])
+def test_fp16_scales_and_large_inputs(T):
+    """fp16 scales (subnormal ones among them), inputs with a mean far from 0 and of 2^100."""
+    N, K, G = 200, 1024, 64
+    codes, scales, z = make(N, K, G, zeros=True, dtype=F16, seed=9)
+    scales[::3] *= 2.0 ** -10
+    x = (torch.randn((T, K), device=DEV) + 30).to(BF16)
+    w = ops.int4_pack(codes, scales, z)
+    check(ops.linear_int4(x, w), x, codes, scales, z, G)
+    x = (x * 2.0 ** 100).to(BF16)
+    check(ops.linear_int4(x, w), x, codes, scales, z, G)
+
+
+def test_every_count_of_rows():
+    N, K, G = 80, 256, 32
+    codes, scales, z = make(N, K, G, seed=3)
+    w = ops.int4_pack(codes, scales)
+    x = torch.randn((150, K), device=DEV).to(BF16)
+    for T in list(range(1, 70)) + [79, 80, 81, 95, 96, 97, 127, 128, 129, 150]:
+        check(ops.linear_int4(x[:T], w), x[:T], codes, scales, z, G)
+
+
+@pytest.mark.parametrize("T", [3, 40, 200])
+def test_rows_outside_are_left_and_nan_rows_stay_their_own(T):
+    N, K, G = 100, 160, 32
+    codes, scales, z = make(N, K, G, zeros=True, seed=4)
+    w = ops.int4_pack(codes, scales, z)
+    x = torch.randn((T, K), device=DEV).to(BF16)
+    room = torch.full((T + 4, N), 7.0, dtype=BF16, device=DEV)
+    want = ops.linear_int4(x, w, out=room[2:T + 2]).clone()
+    assert (room[:2] == 7).all() and (room[T + 2:] == 7).all()
+    x[1, 5], x[T - 1, K - 1] = float("nan"), float("inf")
+    y = ops.linear_int4(x, w)
+    assert torch.isnan(y[1]).all() and torch.isnan(y[T - 1]).all()
+    keep = torch.ones(T, dtype=torch.bool, device=DEV)
+    keep[1] = keep[T - 1] = False
+    assert torch.equal(y[keep], want[keep])
+
+
+def test_a_matrix_past_2_to_the_31_bytes():
+    N, K, G = 2_200_000, 2048, 128
+    codes = torch.randint(0, 256, (64, K // 2), device=DEV, dtype=torch.uint8).repeat(N // 64 + 1, 1)[:N]
+    scales = torch.linspace(0.001, 0.01, N, device=DEV).to(BF16).unsqueeze(1).expand(N, K // G).contiguous()
+    w = ops.int4_pack(codes, scales)
+    assert w.units.numel() > 2 ** 31
+    for T in (2, 70):
+        x = torch.randn((T, K), device=DEV).to(BF16)
+        y = ops.linear_int4(x, w)
+        for a in (0, N // 2 // 16 * 16, N - 100):
+            check(y[:, a:a + 100].contiguous(), x, codes[a:a + 100], scales[a:a + 100], None, G)
+
+
+@pytest.mark.parametrize("T", [2, 40, 150])
+def test_replay_and_another_stream(T):
+    N, K, G = 300, 2048, 128
+    codes, scales, z = make(N, K, G, zeros=True, seed=5)
+    w = ops.int4_pack(codes, scales, z)
+    x = torch.randn((T, K), device=DEV).to(BF16)
+    want = ops.linear_int4(x, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.linear_int4(x, w)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.linear_int4(x, w)
+    for _ in range(3):
+        got.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_no_rows():
+    codes, scales, _ = make(48, 64, 32)
+    w = ops.int4_pack(codes, scales)
+    assert ops.linear_int4(torch.empty((0, 64), dtype=BF16, device=DEV), w).shape == (0, 48)
+
+
+def test_refusals():
+    codes, scales, z = make(48, 256, 64, zeros=True)
+    with pytest.raises(ValueError, match="groups of 32"):
+        ops.int4_pack(codes, scales[:, :1].contiguous())
+    with pytest.raises(ValueError, match="scales must be"):
+        ops.int4_pack(codes, scales[:20].contiguous())
+    with pytest.raises(ValueError, match="bf16 or fp16"):
+        ops.int4_pack(codes, scales.float())
+    with pytest.raises(ValueError, match="zeros must be"):
+        ops.int4_pack(codes, scales, z[:, :2].contiguous())
+    w = ops.int4_pack(codes, scales, z)
+    x = torch.zeros((3, 256), dtype=BF16, device=DEV)
+    with pytest.raises(ValueError, match="x must be"):
+        ops.linear_int4(x[:, :128].contiguous(), w)
+    with pytest.raises(ValueError, match="bias must be"):
+        ops.linear_int4(x, w, torch.zeros(47, dtype=BF16, device=DEV))
+    with pytest.raises(ValueError, match="out must be"):
+        ops.linear_int4(x, w, out=torch.zeros((3, 49), dtype=BF16, device=DEV))
+    with pytest.raises(ValueError, match="size of its shape"):
+        ops.linear_int4(x, ops.Int4Weight(w.units, 64, 256, 64, True))
+    with pytest.raises(ValueError, match="16-byte"):
+        room = torch.zeros(3 * 256 + 1, dtype=BF16, device=DEV)
+        ops.linear_int4(room[1:].view(3, 256), w)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.linear_int4(torch.zeros((3, 512), dtype=BF16, device=DEV)[:, ::2], w)
