@@ -39,23 +39,6 @@ constexpr int kMx8Stage = BM * 128 + 256;  // codes and scales of a step's 128 i
 template <int BM, int NW, bool GATEUP>
 constexpr int kMx8Lds = std::max(2 * kMx8Stage<BM>, BM * kMx8OutRow<NW, GATEUP> + (GATEUP ? BM * NW : 0));
 
-// Direct-to-LDS loads that the compiler does not know of: lane l's BYTES at src land at
-// dst + BYTES l (dst is wave-uniform, an LDS offset).  It would let no LDS read
-// pass one in flight, of whatever address (its own wait before the first read
-// of a step was for that step's loads); here the waits of the K loop order
-// them.  The wait state lets m0 settle.
-template <int BYTES>
-__device__ __forceinline__ void load_lds_hidden(const uint8_t *src, uint32_t dst) {
-    static_assert(BYTES == 16 || BYTES == 4, "direct-to-LDS sizes");
-    if constexpr (BYTES == 16)
-        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
-    else
-        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
-}
-__device__ __forceinline__ uint32_t lds_offset(const void *p) {
-    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)(uint32_t)(uintptr_t)p);
-}
-
 // BM rows x four groups (128 h columns or 256 y columns), K in steps of 128, two
 // stages of activations; at least OCC workgroups per CU.
 template <int BM, int NW, bool GATEUP, int OCC>

@@ -36,6 +36,23 @@ __device__ __forceinline__ void load_lds16(const uint16_t *src, uint8_t *dst) {
     __builtin_amdgcn_global_load_lds((g_void_t *)(uintptr_t)src, (lds_void_t *)(uint32_t)(uintptr_t)dst, 16, 0, AUX);
 }
 
+// Direct-to-LDS loads that the compiler does not know of: lane l's BYTES at src land at
+// dst + BYTES l (dst is wave-uniform, an LDS offset).  It would let no LDS read
+// pass one in flight, of whatever address (its own wait before the first read
+// of a step was for that step's loads); here the waits of the K loop order
+// them.  The wait state lets m0 settle.
+template <int BYTES>
+__device__ __forceinline__ void load_lds_hidden(const uint8_t *src, uint32_t dst) {
+    static_assert(BYTES == 16 || BYTES == 4, "direct-to-LDS sizes");
+    if constexpr (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_offset(const void *p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)(uint32_t)(uintptr_t)p);
+}
+
 // Hides a per-lane load offset from loop-invariant code motion, so each
 // 64-bit address (uniform base + offset) is formed next to its load instead
 // of being hoisted out of the K loop as a live register pair per load.

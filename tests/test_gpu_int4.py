@@ -85,7 +85,12 @@ def test_quantise(N, K, G, zeros):
 SIZES = [(1, 1, 32, 32), (1, 16, 128, 128), (2, 15, 64, 64), (1, 4096, 2048, 128), (3, 513, 4096, 64), (5, 4097, 2816, 32),
          (15, 33, 96, 32), (16, 2048, 4096, 128), (17, 100, 352, 32), (31, 257, 768, 128), (33, 640, 1408, 128),
          (48, 255, 2048, 64), (64, 1000, 1024, 32), (65, 129, 256, 64), (128, 512, 2048, 128), (200, 77, 160, 32),
-         (513, 384, 640, 128), (1031, 1100, 2048, 64), (2048, 256, 4096, 128)]
+         (513, 384, 640, 128), (1031, 1100, 2048, 64), (2048, 256, 4096, 128),
+         # the launch for many rows: one step of the K axis, two, odd ones, ragged edges of every kind
+         (800, 1000, 96, 32), (800, 1000, 128, 128), (3100, 257, 352, 32), (3071, 255, 192, 64), (1500, 520, 1408, 128),
+         (1025, 771, 4096, 64), (2049, 513, 1056, 32),
+         # many row tiles for one workgroup
+         (1, 20000, 2048, 128), (3, 16401, 1152, 32), (16, 33000, 1984, 64), (2, 9000, 8192, 128), (4, 5000, 4096, 128)]
 
 
 @pytest.mark.parametrize("T,N,K,G", SIZES)
@@ -101,7 +106,7 @@ def test_products(T, N, K, G, zeros, bias):
     assert torch.equal(y, ops.linear_int4(x, w, b))
 
 
-@pytest.mark.parametrize("T", [1, 7, 40, 300])
+@pytest.mark.parametrize("T", [1, 7, 40, 300, 3100])
 def test_fp16_scales_and_large_inputs(T):
     """fp16 scales (subnormal ones among them), inputs with a mean far from 0 and of 2^100."""
     N, K, G = 200, 1024, 64
@@ -123,7 +128,7 @@ def test_every_count_of_rows():
         check(ops.linear_int4(x[:T], w), x[:T], codes, scales, z, G)
 
 
-@pytest.mark.parametrize("T", [3, 40, 200])
+@pytest.mark.parametrize("T", [3, 40, 200, 3100])
 def test_rows_outside_are_left_and_nan_rows_stay_their_own(T):
     N, K, G = 100, 160, 32
     codes, scales, z = make(N, K, G, zeros=True, seed=4)
@@ -153,7 +158,7 @@ def test_a_matrix_past_2_to_the_31_bytes():
             check(y[:, a:a + 100].contiguous(), x, codes[a:a + 100], scales[a:a + 100], None, G)
 
 
-@pytest.mark.parametrize("T", [2, 40, 150])
+@pytest.mark.parametrize("T", [2, 40, 1700])
 def test_replay_and_another_stream(T):
     N, K, G = 300, 2048, 128
     codes, scales, z = make(N, K, G, zeros=True, seed=5)
@@ -175,6 +180,21 @@ def test_replay_and_another_stream(T):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+def test_workspace_given():
+    T, N, K, G = 1000, 900, 512, 64
+    codes, scales, z = make(N, K, G, zeros=True, seed=6)
+    w = ops.int4_pack(codes, scales, z)
+    x = torch.randn((T, K), device=DEV).to(BF16)
+    need = ops.linear_int4_workspace_size(T, N, K, G)
+    assert need == T * (K // G) * 4
+    room = torch.full((need + 64,), 255, dtype=torch.uint8, device=DEV)  # NaN patterns: any contents
+    y = ops.linear_int4(x, w, workspace=room[:need])
+    check(y, x, codes, scales, z, G)
+    assert (room[need:] == 255).all() and torch.equal(y, ops.linear_int4(x, w))
+    with pytest.raises(ValueError, match="workspace must hold"):
+        ops.linear_int4(x, w, workspace=room[:need - 4])
 
 
 def test_no_rows():
