@@ -81,20 +81,25 @@ __global__ __launch_bounds__(64 * NW, OCC * NW / 4) void mx8_grouped_kernel(Mx8G
     // 8 and the chunk that belongs in its slot
     constexpr int RQ = 8 * NW, AL = (BM + RQ - 1) / RQ;  // rows per load of all waves, loads of a wave
     static_assert(BM % RQ == 0 || BM < RQ, "activation loads");
-    uint32_t arow[AL];
+    const uint8_t *arow[AL];
     const int lrow = 8 * wave + (lane >> 3);  // in its load's rows
     const uint32_t achunk = (uint32_t)((lane & 7) ^ ((lrow >> 1) & 7));
 #pragma unroll
     for (int q = 0; q < AL; ++q) {
         const int row = min(m0 + RQ * q + lrow, row_end - 1);
-        arow[q] = (uint32_t)(GATEUP ? p.perm_token[row] : row) * (uint32_t)(K / 16) + achunk;
+        arow[q] = p.a + (size_t)(GATEUP ? p.perm_token[row] : row) * K + achunk * 16;
     }
     // scales: lane l of the first wave takes row l's four of a step
-    uint32_t srow = 0;
-    if (wave == 0) {
-        const int row = min(m0 + min(lane, BM - 1), row_end - 1);
-        srow = (uint32_t)(GATEUP ? p.perm_token[row] : row) * (uint32_t)KT;
+    const uint8_t *srow = nullptr;
+    if (wave * 64 < BM) {
+        const int row = min(m0 + min(64 * wave + lane, BM - 1), row_end - 1);
+        srow = p.a_scales + (size_t)(GATEUP ? p.perm_token[row] : row) * (K / 32);
     }
+    // where the lane's pieces lie: of a row tile's codes and scales in a group of
+    // weights, and of 16 rows in a stage
+    const uint32_t wlane = (uint32_t)(g * 1024 + r * 16), slane = (uint32_t)(kGroupScales + (r * 4 + g) * 4);
+    const uint32_t lx0 = (uint32_t)(r * 128 + ((g ^ (r >> 1)) << 4)), lx1 = lx0 ^ 64, lxs = (uint32_t)(r * 4 + g);
+    const uint32_t lds0 = lds_offset(smem);
 
     f32x4_t acc[4][TM];
 #pragma unroll
@@ -107,77 +112,68 @@ __global__ __launch_bounds__(64 * NW, OCC * NW / 4) void mx8_grouped_kernel(Mx8G
         auto ld = [](const uint8_t *q) -> u32x4_t {
             return decltype(once)::value ? __builtin_nontemporal_load(gptr(q)) : *gptr(q);
         };
-        auto issue_a = [&](int kt) __attribute__((always_inline)) {
-            const uint32_t st = lds_offset(smem) + (kt & 1) * kMx8Stage<BM>;
+        auto issue_a = [&](int kt, uint32_t st) __attribute__((always_inline)) {
 #pragma unroll
             for (int q = 0; q < AL; ++q) {
                 if (RQ * q + 8 * wave >= 16 * L) continue;  // rows that no product reads
-                uint32_t o = arow[q];
-                opaque(o);
-                load_lds_hidden<16>(p.a + kt * 128 + (size_t)o * 16, st + (RQ * q + 8 * wave) * 128);
+                load_lds_hidden<16>(arow[q] + kt * 128, lds0 + st + (RQ * q + 8 * wave) * 128);
             }
-            if (wave == 0) {
-                uint32_t o = srow;
-                opaque(o);
-                load_lds_hidden<4>(p.a_scales + ((size_t)o + kt) * 4, st + BM * 128);
-            }
+            if (wave == 0) load_lds_hidden<4>(srow + kt * 4, lds0 + st + BM * 128);
         };
         // word i of d[q]: row 16 i + r, inputs 32 g + 8 q .. + 7; word i of the four is
         // what the product of row tile i takes.  s: byte i is the scale of that block
         auto issue_w = [&](int kt, u32x4_t (&d)[4], uint32_t &s) __attribute__((always_inline)) {
             const uint8_t *b = wbase + (size_t)kt * kGroupBytes;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) d[q] = ld(b + g * 1024 + (r + 16 * q) * 16);
-            s = *reinterpret_cast<const uint32_t *>(b + kGroupScales + (r * 4 + g) * 4);
+            for (int q = 0; q < 4; ++q) d[q] = ld(b + q * 256 + wlane);
+            s = *(const __attribute__((address_space(1))) uint32_t *)(uintptr_t)(b + slane);
         };
-        // Step kt: everything asked for in step kt - 1 has landed; then ask for kt + 1 and
-        // run the products of kt from d.
-        auto step = [&](auto more, int kt, u32x4_t (&d)[4], uint32_t &s, u32x4_t (&next)[4], uint32_t &snext)
-            __attribute__((always_inline)) {
+        // One set of registers for the words that are on their way: a step first puts
+        // each row tile's four words side by side, then asks for the next step's.
+        u32x4_t d[4];
+        uint32_t ds;
+        auto step = [&](auto more, int kt) __attribute__((always_inline)) {
+            const uint32_t st = (kt & 1) * kMx8Stage<BM>;
             wait_vm<0>();
             ring_barrier();
-            // what a step asks for it asks for first, and the moves that put a row tile's words
-            // side by side are its own, behind the wait for them
+            u32x4_t w[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(d[q]));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = u32x4_t{d[0][i], d[1][i], d[2][i], d[3][i]};
+                asm volatile("" : "+v"(w[i]));
+            }
+            int s = (int)ds;
+            asm volatile("" : "+v"(s));
             if constexpr (decltype(more)::value) {
-                issue_a(kt + 1);
-                issue_w(kt + 1, next, snext);
+                issue_a(kt + 1, kMx8Stage<BM> - st);
+                issue_w(kt + 1, d, ds);
             }
             __builtin_amdgcn_sched_barrier(0);
-            const uint8_t *st = smem + (kt & 1) * kMx8Stage<BM>;
-            i32x8_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = i32x8_t{(int)d[0][i], (int)d[1][i], (int)d[2][i], (int)d[3][i], 0, 0, 0, 0};
+            // one address each, the token tiles behind it as offsets of the instruction
+            uint32_t at0 = lx0 + st, at1 = lx1 + st, ats = lxs + st;
+            opaque(at0);
+            opaque(at1);
+            opaque(ats);
+            auto wide = [](u32x4_t v) { return i32x8_t{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; };
 #pragma unroll
             for (int m = 0; m < L; ++m) {
-                const uint8_t *row = st + (16 * m + r) * 128;
-                const uint4 x0 = *reinterpret_cast<const uint4 *>(row + ((g ^ (r >> 1)) << 4));
-                const uint4 x1 = *reinterpret_cast<const uint4 *>(row + (((4 + g) ^ (r >> 1)) << 4));
-                const int xs = st[BM * 128 + (16 * m + r) * 4 + g];
+                const uint4 x0 = *reinterpret_cast<const uint4 *>(smem + at0 + m * 2048);
+                const uint4 x1 = *reinterpret_cast<const uint4 *>(smem + at1 + m * 2048);
+                const int xs = smem[ats + (BM * 128 + m * 64)];
                 const i32x8_t x = {(int)x0.x, (int)x0.y, (int)x0.z, (int)x0.w, (int)x1.x, (int)x1.y, (int)x1.z, (int)x1.w};
-                acc[0][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[0], x, acc[0][m], 4, 0, 0, (int)s, 0, xs);
-                acc[1][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[1], x, acc[1][m], 4, 0, 1, (int)s, 0, xs);
-                acc[2][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[2], x, acc[2][m], 4, 0, 2, (int)s, 0, xs);
-                acc[3][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[3], x, acc[3][m], 4, 0, 3, (int)s, 0, xs);
+                acc[0][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(w[0]), x, acc[0][m], 4, 0, 0, s, 0, xs);
+                acc[1][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(w[1]), x, acc[1][m], 4, 0, 1, s, 0, xs);
+                acc[2][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(w[2]), x, acc[2][m], 4, 0, 2, s, 0, xs);
+                acc[3][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(w[3]), x, acc[3][m], 4, 0, 3, s, 0, xs);
             }
         };
-        u32x4_t w0[4], w1[4];
-        uint32_t s0, s1;
-        issue_w(0, w0, s0);
-        issue_a(0);
+        issue_w(0, d, ds);
+        issue_a(0, 0);
         // no branch round the loads: their registers would be merged, and waited for, behind it
-        int kt = 0;
-        for (; kt + 2 < KT; kt += 2) {
-            step(std::true_type{}, kt, w0, s0, w1, s1);
-            step(std::true_type{}, kt + 1, w1, s1, w0, s0);
-        }
-        if (KT - kt == 2) {
-            step(std::true_type{}, kt, w0, s0, w1, s1);
-            step(std::false_type{}, kt + 1, w1, s1, w0, s0);
-        } else {
-            step(std::false_type{}, kt, w0, s0, w1, s1);
-        }
+        for (int kt = 0; kt < KT - 1; ++kt) step(std::true_type{}, kt);
+        step(std::false_type{}, KT - 1);
     };
     // one straight-line loop for each number of 16-row tiles that hold rows, and for
     // weights that no other tile reads, which are not kept in the caches
