@@ -264,11 +264,14 @@ def main(argv=None):
     ap.add_argument("--merge", choices=["reference", "fused"], default="reference")
     ap.add_argument("--input-pregather", action="store_true")
     ap.add_argument("--graph-output-pool", action="store_true")
+    ap.add_argument("--int4-group", type=int, choices=[32, 64, 128], default=None,
+                    help="attention projections and vocabulary head on 4-bit weights with groups of this many inputs")
     ap.add_argument("--seed", type=int, default=20261011)
     ap.add_argument("--output", type=Path, required=True, help="result.json path (its directory holds the run)")
     args = ap.parse_args(argv)
     opts = dict(resident_graphs=args.graphs, merge=args.merge, input_pregather=args.input_pregather,
                 graph_output_pool=args.graph_output_pool)
+    model_options = {} if args.int4_group is None else dict(int4_group=args.int4_group)
     specs = build_cases(args.lengths, repetitions=args.repetitions, output_tokens=args.output_tokens,
                         warmups=args.warmups, demand_slots=args.demand_slots, **opts)
     identity = None
@@ -283,7 +286,7 @@ def main(argv=None):
         name = f"random-init Qwen3-30B-A3B-shaped, {args.random_layers} layers, seed {args.seed}"
     result = run(model, specs, output=args.output, argv=sys.argv if argv is None else argv, config=vars(args),
                  model_name=name, model_identity=identity, hot_per_layer=args.hot_per_layer,
-                 speculative_slots=args.speculative_slots, demand_slots=args.demand_slots, seed=args.seed, **opts)
+                 speculative_slots=args.speculative_slots, demand_slots=args.demand_slots, seed=args.seed, **opts, **model_options)
     print(records.json.dumps(dict(status=result["status"], output=str(args.output.resolve()))), flush=True)
 
 

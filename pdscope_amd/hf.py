@@ -14,11 +14,18 @@ runtime with a static hot set; ``forward_layer`` feeds each layer call with
 the caller's step (``session.step``: 0 for the prompt, then 1, 2, ... per
 decoded token) and the next layer's router for the gate-fallback prefetch,
 and keeps the runtime's per-layer trace rows.
+
+``install_int4_linears(model)`` replaces the linear modules that stay outside the
+expert blocks (the attention's projections, the vocabulary head) by ``Int4Linear``:
+4-bit codes with a scale per group of inputs, a little over a quarter of the bytes
+that a decoded token reads of them in bf16 (the reference keeps them as they are).
+``ModelSession(model, int4_group=128, ...)`` does so at start.
 """
 from __future__ import annotations
 
 import torch
 
+from . import ops
 from .cache import ExpertKey
 from .checkpoint import collect_model_experts, pin_cpu_master_storage
 from .pdscope_runtime import PDScopeCudaRuntime
@@ -56,16 +63,68 @@ def install_expert_blocks(model, forward_layer, *, return_router_logits=None):
     return originals
 
 
+class Int4Linear(torch.nn.Module):
+    """A linear module over a 4-bit matrix (ops.Int4Weight): bf16 inputs [..., K] on the
+    matrix' device to bf16 outputs [..., N].  Inference only: ops.linear_int4 has no
+    gradient."""
+
+    def __init__(self, weight: ops.Int4Weight, bias=None):
+        super().__init__()
+        self.register_buffer("units", weight.units)
+        self.register_buffer("bias", bias)
+        self.in_features, self.out_features = weight.K, weight.N
+        self._shape = (weight.N, weight.K, weight.group, weight.zeros, weight.scale_dtype)
+
+    @classmethod
+    def of(cls, linear: torch.nn.Linear, group=128, zeros=False):
+        """The 4-bit form of a bf16 linear module on the GPU (ops.int4_quantize)."""
+        bias = None if linear.bias is None else linear.bias.detach()
+        return cls(ops.int4_quantize(linear.weight.detach().contiguous(), group, zeros), bias)
+
+    @property
+    def weight4(self) -> ops.Int4Weight:
+        return ops.Int4Weight(self.units, *self._shape)
+
+    def forward(self, x):
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("Int4Linear has no gradient: run it under torch.no_grad() or inference_mode()")
+        out = ops.linear_int4(x.reshape(-1, x.shape[-1]).contiguous(), self.weight4, bias=self.bias)
+        return out.view(*x.shape[:-1], self.out_features)
+
+    def extra_repr(self):
+        return f"in_features={self.in_features}, out_features={self.out_features}, group={self._shape[2]}"
+
+
+def install_int4_linears(model, group=128, zeros=False, keep=()):
+    """Replace every torch.nn.Linear of a model that is on the GPU, but for routers and
+    experts (modules below a `mlp` with a `gate`) and the names in `keep`, by its
+    4-bit form; returns the replaced modules' names.  Their bf16 weights are freed
+    where nothing else holds them (a tied embedding does)."""
+    inside = [n + "." for n, m in model.named_modules() if hasattr(m, "gate") and n.rsplit(".", 1)[-1] == "mlp"]
+    found = [(n, m) for n, m in model.named_modules()
+             if type(m) is torch.nn.Linear and n not in keep and not any(n.startswith(p) for p in inside)]
+    for name, m in found:  # before anything is replaced
+        if m.weight.dtype != torch.bfloat16 or m.weight.device.type != "cuda":
+            raise ValueError(f"{name} must be bf16 on the GPU, got {m.weight.dtype} on {m.weight.device}")
+        if m.in_features % group:
+            raise ValueError(f"{name} has {m.in_features} inputs, not whole groups of {group}: keep it or take smaller groups")
+    for name, m in found:
+        parent, _, leaf = name.rpartition(".")
+        setattr(model.get_submodule(parent) if parent else model, leaf, Int4Linear.of(m, group, zeros))
+    return [n for n, _ in found]
+
+
 class ModelSession:
     """Qwen3-MoE model whose expert layers run on the gfx950 path.
 
     hot_per_layer: experts per layer placed in the static hot set (the first
     ones of ``hot_order[layer]`` when given, else ids 0, 1, ...);
     speculative_slots, demand_slots and the other keywords go to
-    PDScopeCudaRuntime."""
+    PDScopeCudaRuntime.  int4_group (32, 64 or 128): the linear modules outside the
+    expert blocks run on 4-bit weights (install_int4_linears)."""
 
     def __init__(self, model, *, hot_per_layer, speculative_slots, demand_slots=2, hot_order=None,
-                 device=0, block_cap_bytes=256 * 1024**2, **runtime_kwargs):
+                 device=0, block_cap_bytes=256 * 1024**2, int4_group=None, **runtime_kwargs):
         if model.config.model_type != "qwen3_moe":
             raise ValueError("only Qwen3 MoE supported")
         self.model = model
@@ -79,6 +138,7 @@ class ModelSession:
         for layer, decoder in enumerate(model.model.layers):
             self.gates[layer] = decoder.mlp.gate
         model.to(self.device)
+        self.int4_linears = [] if int4_group is None else install_int4_linears(model, int4_group)
         E = model.config.num_experts
         hot = []
         for layer in self.gates:

@@ -99,11 +99,15 @@ class MoEWorkspace:
             self._ident = buf
         return buf[:n]
 
-    def views(self, T: int):
+    def packed(self, T: int) -> ops.Packed:
+        """What pack writes for T tokens."""
         if not 0 < T <= self.max_tokens:
             raise ValueError(f"token count {T} outside workspace capacity {self.max_tokens}")
         n = T * self.k
-        packed = ops.Packed(self.counts, self.offsets, self.perm_token[:n], self.perm_pos[:n], self.row_of[:n])
+        return ops.Packed(self.counts, self.offsets, self.perm_token[:n], self.perm_pos[:n], self.row_of[:n])
+
+    def views(self, T: int):
+        packed = self.packed(T)
         return self.logits[:T], self.ids[:T], self.weights[:T], packed
 
 
@@ -181,7 +185,7 @@ def experts_resident(x, ids, weights, slots, ws: MoEWorkspace, out=None, *, bloc
     if ops.is_mxfp4(representation):
         if shared_slot is not None:
             raise ValueError("shared experts join 4-bit routed experts through add_in")
-        _, _, _, packed = ws.views(T)
+        packed = ws.packed(T)
         # the launches below take these sizes as given
         if ids.ndim != 2 or ids.shape[0] != T or not 1 <= ids.shape[1] <= k:
             raise ValueError(f"ids must be [{T}, 1 to {k}], got {list(ids.shape)}")

@@ -816,9 +816,22 @@ class MxRows:
     scales: torch.Tensor  # uint8 [T, n / 32]
 
 
+def _line(t, dtype, dev) -> bool:
+    """Whether _need(t, ..., dtype, 1, dev) passes."""
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.ndim == 1 and t.device == dev and t.is_contiguous()
+
+
 def _need_rows(rows, name, T, n, device):
+    """Refuse what is not 8-bit rows [T, n] (None: any) on `device`."""
     if not isinstance(rows, MxRows):
         raise ValueError(f"{name} must be MxRows")
+    c, s = rows.codes, rows.scales
+    if (isinstance(c, torch.Tensor) and isinstance(s, torch.Tensor) and c.dtype is F8 and s.dtype is torch.uint8
+            and c.ndim == 2 and c.shape[1] % 32 == 0 and s.shape == (c.shape[0], c.shape[1] // 32)
+            and (T is None or c.shape[0] == T) and (n is None or c.shape[1] == n) and c.device.type == "cuda"
+            and s.device == c.device and (device is None or c.device == device) and c.is_contiguous()
+            and s.is_contiguous()):
+        return
     _need(rows.codes, f"{name}.codes", F8, 2, device)
     _need(rows.scales, f"{name}.scales", torch.uint8, 2, rows.codes.device)
     shape = tuple(rows.codes.shape)
@@ -875,22 +888,25 @@ def swiglu_grouped_mxfp8(x: MxRows, perm_token, offsets, sel, tile_start, max_ti
     _need_rows(x, "inputs", None, H, None)
     dev = x.codes.device
     for t, n in ((perm_token, "perm_token"), (offsets, "offsets"), (sel, "sel"), (tile_start, "tile_start")):
-        _need(t, n, torch.int32, 1, dev)
-    _need(slots, "slots", torch.int64, 1, dev)
+        if not _line(t, torch.int32, dev):
+            _need(t, n, torch.int32, 1, dev)
+    if not _line(slots, torch.int64, dev):
+        _need(slots, "slots", torch.int64, 1, dev)
     _need_rows(h_ws, "h_ws", None, I, dev)
     _need(y, "y", BF16, None, dev)
     check_slots(slots, H, I, "mxfp4")
-    if h_ws.codes.shape[0] < perm_token.numel() or y.numel() < perm_token.numel() * H:
+    rows, nsel = perm_token.shape[0], sel.shape[0]
+    if h_ws.codes.shape[0] < rows or y.numel() < rows * H:
         raise ValueError("h_ws / y workspaces are smaller than rows x I / rows x H")
-    if tile_start.numel() < sel.numel() + 1 or offsets.numel() < 2:
+    if tile_start.shape[0] < nsel + 1 or offsets.shape[0] < 2:
         raise ValueError("tile_start must hold one entry more than sel, offsets one more than there are experts")
-    if slots.numel() < offsets.numel() - 1:
+    if slots.shape[0] < offsets.shape[0] - 1:
         raise ValueError("slots must hold one entry per expert")
-    if max(x.codes.numel(), perm_token.numel() * I) >= 1 << 36:
+    if max(x.codes.shape[0] * H, rows * I) >= 1 << 36:
         raise ValueError("swiglu_grouped_mxfp8 addresses fewer than 2^36 activations")
-    _call_on(dev, "pdscope_swiglu_grouped_mxfp8", _p(x.codes), _p(x.scales), _p(perm_token), _p(offsets), _p(sel),
-             sel.numel(), _p(tile_start), int(max_tiles), int(block_m), _p(slots), H, I, _p(h_ws.codes),
-             _p(h_ws.scales), _p(y))
+    _call_on(dev, "pdscope_swiglu_grouped_mxfp8", x.codes.data_ptr(), x.scales.data_ptr(), perm_token.data_ptr(),
+             offsets.data_ptr(), sel.data_ptr(), nsel, tile_start.data_ptr(), int(max_tiles), int(block_m),
+             slots.data_ptr(), H, I, h_ws.codes.data_ptr(), h_ws.scales.data_ptr(), y.data_ptr())
     return y
 
 

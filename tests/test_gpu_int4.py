@@ -228,3 +228,85 @@ def test_refusals():
         ops.linear_int4(room[1:].view(3, 256), w)
     with pytest.raises(ValueError, match="contiguous"):
         ops.linear_int4(torch.zeros((3, 512), dtype=BF16, device=DEV)[:, ::2], w)
+
+
+# ------------------------------------------------------- a model's linear modules
+
+def small_model(seed=1):
+    from transformers import Qwen3MoeConfig, Qwen3MoeForCausalLM
+    cfg = Qwen3MoeConfig(vocab_size=331, hidden_size=256, intermediate_size=512, moe_intermediate_size=128,
+                         num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=64,
+                         num_experts=32, num_experts_per_tok=4, norm_topk_prob=True, decoder_sparse_step=1,
+                         mlp_only_layers=[], initializer_range=0.05)
+    torch.manual_seed(seed)
+    model = Qwen3MoeForCausalLM(cfg).to(BF16).eval()
+    with torch.no_grad():
+        for d in model.model.layers:
+            d.mlp.gate.weight.normal_(0.0, 0.5)
+    return cfg, model
+
+
+PROJECTIONS = [f"model.layers.{layer}.self_attn.{p}_proj" for layer in (0, 1) for p in "qkvo"]
+
+
+def test_modules_of_a_model():
+    """Every linear module outside the expert blocks is replaced and gives its own 4-bit matrix'
+    products; routers, experts and what is kept are as they were."""
+    from pdscope_amd.hf import Int4Linear, install_int4_linears
+    _, model = small_model()
+    model.to(DEV)
+    before = {n: m for n, m in model.named_modules() if isinstance(m, torch.nn.Linear)}
+    names = install_int4_linears(model, 64, zeros=True, keep=("lm_head",))
+    assert sorted(names) == sorted(PROJECTIONS)
+    after = dict(model.named_modules())
+    for n, m in before.items():
+        assert (type(after[n]) is Int4Linear) == (n in names) and (n in names or after[n] is m)
+    for n in names:
+        q, m = after[n], before[n]
+        for shape in ((1, 1), (3, 7), (2, 80)):
+            x = torch.randn((*shape, m.in_features), device=DEV).to(BF16)
+            w = ops.int4_dequantize(ops.int4_quantize(m.weight.detach(), 64, True)).double()
+            y = q(x)
+            want = x.double() @ w.T
+            # the dequantised matrix is rounded to bf16: half a step of each weight more than the sums' bound
+            bound = (64 + 256 // 64 + 24) * U * 32 * (x.double().abs() @ w.abs().T) + B * (x.double().abs() @ w.abs().T)
+            assert y.shape == (*shape, m.out_features) and y.dtype is BF16
+            assert_within(y, want, (1 + B) * bound + B * want.abs() + 2.0 ** -133)
+    x = torch.randn((2, 256), device=DEV).to(BF16).requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        after[names[0]](x)
+    with pytest.raises(ValueError, match="whole groups"):
+        install_int4_linears(torch.nn.Sequential(torch.nn.Linear(96, 8)).to(BF16).to(DEV), 64)
+    with pytest.raises(ValueError, match="bf16 on the GPU"):
+        install_int4_linears(torch.nn.Sequential(torch.nn.Linear(128, 8)), 64)
+
+
+def test_model_session_on_four_bit_linears():
+    """A prompt and two tokens through a session with 4-bit projections and head against the same
+    model with these modules' dequantised matrices in bf16: they differ by the roundings of bf16
+    matrices and of attention, as the two models of test_gpu_hybrid.py do."""
+    from pdscope_amd.hf import Int4Linear, ModelSession
+    cfg, ours = small_model()
+    _, native = small_model()
+    native.to(DEV)
+    with torch.no_grad():
+        for n, m in native.named_modules():
+            if n in PROJECTIONS or n == "lm_head":
+                m.weight.copy_(ops.int4_dequantize(ops.int4_quantize(m.weight.detach(), 128)))
+    session = ModelSession(ours, hot_per_layer=6, speculative_slots=2, demand_slots=2, device=0, int4_group=128)
+    try:
+        assert sorted(session.int4_linears) == sorted(PROJECTIONS + ["lm_head"])
+        assert type(ours.lm_head) is Int4Linear
+        ids = torch.randint(0, cfg.vocab_size, (1, 24), generator=torch.Generator().manual_seed(2)).to(DEV)
+        with torch.no_grad():
+            past_a = past_b = None
+            for step in range(3):
+                session.step = step
+                a = native(ids, past_key_values=past_a, use_cache=True)
+                b = ours(ids, past_key_values=past_b, use_cache=True)
+                past_a, past_b = a.past_key_values, b.past_key_values
+                r, g = a.logits[0, -1].float(), b.logits[0, -1].float()
+                assert (r - g).norm() <= 3e-2 * r.norm()
+                ids = r.argmax().view(1, 1)
+    finally:
+        session.close()
