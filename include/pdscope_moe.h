@@ -547,11 +547,9 @@ int pdscope_swiglu_grouped_mxfp8(const void *x, const void *x_scales, const int3
  * with exact products of x and q, fp32 sums and fp32 scales; a row of x with an
  * infinity or NaN gives NaN, and a row of W with an infinite or NaN scale NaN or
  * infinities.  y may overlap nothing.
- * workspace: pdscope_linear_int4_workspace_size bytes (0 for few rows: NULL then), 4-byte
- * aligned, any contents; calls that overlap in time need one each.
  * Limits: 1 <= N <= 2^24, K % G == 0, K <= 2^20, fewer than 2^37 - 2^13 weights in whole
- * 16 x 128 units; T >= 1, (N/16) * (T/16), each rounded up, below 2^22; T * K below
- * 2^35 - 4096; x, w, codes and weight 16-byte aligned.
+ * 16 x 128 units; T >= 1, (N/16) * (T/16), each rounded up, below 2^22; x, w,
+ * codes and weight 16-byte aligned.
  */
 size_t pdscope_int4_bytes(int N, int K, int G, int zeros);
 int pdscope_int4_pack(const void *codes, const void *scales, const void *zeros, int N, int K, int G, void *out,
@@ -559,9 +557,8 @@ int pdscope_int4_pack(const void *codes, const void *scales, const void *zeros, 
 int pdscope_int4_quantize(const void *weight, int N, int K, int G, int zeros, void *out, void *stream);
 int pdscope_int4_dequantize(const void *w, int N, int K, int G, int zeros, int fp16_scales, void *weight,
                             void *stream);
-size_t pdscope_linear_int4_workspace_size(int T, int N, int K, int G);
 int pdscope_linear_int4(const void *x, const void *w, const void *bias, int T, int N, int K, int G, int zeros,
-                        int fp16_scales, void *y, void *workspace, void *stream);
+                        int fp16_scales, void *y, void *stream);
 
 /*
  * A7 demand staging: replaces the three per-projection non_blocking copies

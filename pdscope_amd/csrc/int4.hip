@@ -45,8 +45,8 @@ __global__ __launch_bounds__(256) void i4_pack_kernel(const uint8_t *__restrict_
     if (g < groups) {
         const int at = s.u * groups + g;
         const bool in = s.row < s.N && at < per_row;
-        reinterpret_cast<uint16_t *>(dst + kI4Codes)[lane] = in ? scales[s.row * per_row + at] : (uint16_t)0;
-        if (zeros) dst[kI4Codes + 32 * groups + lane] = in ? zeros[s.row * per_row + at] & 15 : 0;
+        *reinterpret_cast<uint16_t *>(dst + i4_scale_at(lane & 15, g, groups)) = in ? scales[s.row * per_row + at] : (uint16_t)0;
+        if (zeros) dst[i4_zero_at(lane & 15, g, groups)] = in ? zeros[s.row * per_row + at] & 15 : 0;
     }
 }
 
@@ -108,8 +108,8 @@ __global__ __launch_bounds__(256) void i4_quantize_kernel(const uint16_t *__rest
         }
         if (g == 0) {
             const bool in = s.row < s.N && s.u * kI4In + gi * G < s.K;
-            reinterpret_cast<uint16_t *>(dst + kI4Codes)[gi * 16 + lane] = in ? (uint16_t)s16 : (uint16_t)0;
-            if (ZEROS) dst[kI4Codes + 32 * GP + gi * 16 + lane] = in ? (uint8_t)z : 0;
+            *reinterpret_cast<uint16_t *>(dst + i4_scale_at(lane, gi, GP)) = in ? (uint16_t)s16 : (uint16_t)0;
+            if (ZEROS) dst[i4_zero_at(lane, gi, GP)] = in ? (uint8_t)z : 0;
         }
     }
     *reinterpret_cast<uint4 *>(dst + 16 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -130,8 +130,8 @@ __global__ __launch_bounds__(256) void i4_dequantize_kernel(const uint8_t *__res
         const int k = s.u * kI4In + 32 * j + 8 * g;
         if (k >= s.K) break;
         const int gi = 32 * j / G;
-        const float sc = i4_scale(reinterpret_cast<const uint16_t *>(src + kI4Codes)[gi * 16 + r], fp16);
-        const float z = has_zeros ? (float)src[kI4Codes + 32 * (kI4In / G) + gi * 16 + r] : 8.0f;
+        const float sc = i4_scale(*reinterpret_cast<const uint16_t *>(src + i4_scale_at(r, gi, kI4In / G)), fp16);
+        const float z = has_zeros ? (float)src[i4_zero_at(r, gi, kI4In / G)] : 8.0f;
         const bf16x8_t q = i4_decode(w[j]);
         uint32_t o[4];
 #pragma unroll

@@ -25,12 +25,11 @@ struct I4Linear {
 // What a wave holds of a unit: codes, its rows' scales and zero points (rows 4 g .. +
 // 3, a group each), and the inputs of MT tiles of 16 tokens (token r, inputs 8 g .. + 7
 // of each 32).
-template <int G, bool ZEROS, int MT>
+template <int G, bool ZEROS, bool FP16, int MT>
 struct I4Unit {
     static constexpr int GP = kI4In / G, JG = 4 / GP;  // groups of a unit, words of a group
     uint4 c;
-    uint2 s[GP];
-    uint32_t z[GP];
+    I4Side<G, ZEROS, FP16> side;
     uint4 x[MT][4];
 
     // KEEP: another workgroup reads the weights too.  Inputs past the end of a row
@@ -39,11 +38,7 @@ struct I4Unit {
     __device__ __forceinline__ void load(const uint8_t *unit, const uint16_t *const (&xr)[MT], int u, int K, int lane) {
         const int g = lane >> 4;
         c = KEEP ? ld_g(unit + 16 * lane) : ld_nt(unit + 16 * lane);
-#pragma unroll
-        for (int gi = 0; gi < GP; ++gi) {
-            s[gi] = *reinterpret_cast<const uint2 *>(unit + kI4Codes + gi * 32 + 8 * g);
-            if (ZEROS) z[gi] = *reinterpret_cast<const uint32_t *>(unit + kI4Codes + GP * 32 + gi * 16 + 4 * g);
-        }
+        side.load(unit, g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int k = min(u * kI4In + 32 * j + 8 * g, K - 8);
@@ -52,7 +47,6 @@ struct I4Unit {
         }
     }
 
-    template <bool FP16>
     __device__ __forceinline__ void add(f32x4_t (&tot)[MT]) const {
         const __bf16 one = (__bf16)1.0f;
         const bf16x8_t ones = {one, one, one, one, one, one, one, one};
@@ -74,8 +68,7 @@ struct I4Unit {
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float sc = i4_scale((i < 2 ? s[gi].x : s[gi].y) >> (16 * (i & 1)) & 0xffffu, FP16);
-                const float zp = ZEROS ? (float)(z[gi] >> (8 * i) & 255u) : 8.0f;
+                const float sc = side.scale(gi, i), zp = side.zero(gi, i);
 #pragma unroll
                 for (int m = 0; m < MT; ++m) tot[m][i] = fmaf(sc, fmaf(-zp, sx[m][i], acc[m][i]), tot[m][i]);
             }
@@ -119,9 +112,9 @@ __global__ __launch_bounds__(64 * WV) void i4_split_kernel(I4Linear p) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) tot[m] = f32x4_t{};
     for (int u = ks; u < KU; u += WV) {
-        I4Unit<G, ZEROS, MT> d;
+        I4Unit<G, ZEROS, FP16, MT> d;
         d.template load<KEEP>(wt + (size_t)u * UB, xr, u, p.K, lane);
-        d.template add<FP16>(tot);
+        d.add(tot);
     }
     // ---- the waves' parts, in order; lane l has token r and rows 4 g .. + 3
 #pragma unroll
@@ -151,8 +144,7 @@ __global__ __launch_bounds__(64 * WV) void i4_rows_kernel(I4Linear p) {
     const int tiles = (p.N + kI4Rows - 1) / kI4Rows, KU = (p.K + kI4In - 1) / kI4In, stride = gridDim.x;
     struct Held {
         u32x4_t c;
-        uint2 s[GP];
-        uint32_t z[GP];
+        I4Side<G, ZEROS, FP16> side;
     };
     // units past the end are read as the last one, with an x of 0; tiles past the end as
     // the first one, whose sums are not used: no branch round a load, whose registers would be
@@ -163,11 +155,7 @@ __global__ __launch_bounds__(64 * WV) void i4_rows_kernel(I4Linear p) {
         for (int i = 0; i < U; ++i) {
             const uint8_t *unit = at + (size_t)min(ks * U + i, KU - 1) * UB;
             d[i].c = __builtin_nontemporal_load(gptr(unit + 16 * lane));
-#pragma unroll
-            for (int gi = 0; gi < GP; ++gi) {
-                d[i].s[gi] = *reinterpret_cast<const uint2 *>(unit + kI4Codes + gi * 32 + 8 * g);
-                if (ZEROS) d[i].z[gi] = *reinterpret_cast<const uint32_t *>(unit + kI4Codes + GP * 32 + gi * 16 + 4 * g);
-            }
+            d[i].side.load(unit, g);
         }
     };
     Held d0[U], d1[U], d2[U];
@@ -215,9 +203,7 @@ __global__ __launch_bounds__(64 * WV) void i4_rows_kernel(I4Linear p) {
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(i4_decode(d[i].c[j]), x[i][j], acc, 0, 0, 0);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const float sc = i4_scale((q < 2 ? d[i].s[gi].x : d[i].s[gi].y) >> (16 * (q & 1)) & 0xffffu, FP16);
-                    const float zp = ZEROS ? (float)(d[i].z[gi] >> (8 * q) & 255u) : 8.0f;
-                    tot[q] = fmaf(sc, fmaf(-zp, sx[i][gi], acc[q]), tot[q]);
+                    tot[q] = fmaf(d[i].side.scale(gi, q), fmaf(-d[i].side.zero(gi, q), sx[i][gi], acc[q]), tot[q]);
                 }
             }
         // two buffers in turn: who sums tile it is at the barrier of it + 1 before
@@ -249,107 +235,116 @@ __global__ __launch_bounds__(64 * WV) void i4_rows_kernel(I4Linear p) {
 
 // ---- many tokens
 
-// Sums of each group's inputs, fp32 [T, K/G]: four lanes a group of 32 inputs.
-template <int G>
-__global__ __launch_bounds__(256) void i4_sums_kernel(const uint16_t *__restrict__ x, int64_t pieces, float *__restrict__ sums) {
-    constexpr int LG = G / 8;  // lanes of a group
-    const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t at = q < pieces ? q : pieces - 1;
-    const uint4 v = ld_g(x + 8 * at);
-    float s = ((lo_bf(v.x) + hi_bf(v.x)) + (lo_bf(v.y) + hi_bf(v.y))) + ((lo_bf(v.z) + hi_bf(v.z)) + (lo_bf(v.w) + hi_bf(v.w)));
-#pragma unroll
-    for (int d = 1; d < LG; d *= 2) s += __shfl_xor(s, d);
-    if (q < pieces && (q & (LG - 1)) == 0) sums[q / LG] = s;
-}
-
 constexpr int kI4GemmM = 64, kI4GemmN = 256;
-constexpr int kI4GemmStage = kI4GemmM * 256, kI4GemmOut = kI4GemmN * 2 + 16;
+constexpr int kI4GemmX = kI4GemmM * 256;           // a stage's x, behind it its scales:
+constexpr int kI4GemmStage = kI4GemmX + 4 * 512;  // 128 bytes at most for each of four tiles of four waves
+constexpr int kI4GemmSums = 16;                    // groups whose sums of x are kept at a time
+constexpr int kI4GemmOut = kI4GemmN * 2 + 16;
 
 // 64 tokens x 256 rows of W, K in steps of 128: a wave has four row tiles to
 // itself, whose codes go from memory to registers a step ahead; x streams through two LDS
 // stages in 256-byte rows whose 16-byte chunk c lies in slot c ^ (row % 16).
 template <int G, bool ZEROS, bool FP16>
-__global__ __launch_bounds__(256, 2) void i4_gemm_kernel(I4Linear p, const float *sums) {
+__global__ __launch_bounds__(256, 2) void i4_gemm_kernel(I4Linear p, int cut) {
     constexpr int UB = i4_unit_bytes(G, ZEROS), GP = kI4In / G, JG = 4 / GP;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[std::max(2 * kI4GemmStage, kI4GemmM * kI4GemmOut)];
+    __shared__ float s_sums[2][kI4GemmSums][kI4GemmM];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
     const int tiles = (p.N + kI4Rows - 1) / kI4Rows, KT = (p.K + kI4In - 1) / kI4In;
-    // eight contiguous pieces of the list, one per XCD, tokens fastest: an XCD's L2 holds its rows of W
-    const int TB = (p.T + kI4GemmM - 1) / kI4GemmM, total = TB * ((p.N + kI4GemmN - 1) / kI4GemmN);
-    const int per_xcd = (total + 7) >> 3, pos = blockIdx.x >> 3, t = (blockIdx.x & 7) * per_xcd + pos;
-    if (pos >= per_xcd || t >= total) return;
-    const int nb = t / TB, t0 = (t - nb * TB) * kI4GemmM, n0 = nb * kI4GemmN;
+    // the tiles in `cut` x 8 / `cut` rectangles, one per XCD: tokens and rows of W whose
+    // sum in bytes is least, for its L2; tokens fastest
+    const int TB = (p.T + kI4GemmM - 1) / kI4GemmM, NB = (p.N + kI4GemmN - 1) / kI4GemmN;
+    const int xcd = blockIdx.x & 7, pos = blockIdx.x >> 3, per_t = (TB + cut - 1) / cut, per_n = (NB * cut + 7) / 8;
+    const int tb = xcd % cut * per_t + pos % per_t, nb = xcd / cut * per_n + pos / per_t;
+    if (tb >= TB || nb >= NB) return;
+    const int t0 = tb * kI4GemmM, n0 = nb * kI4GemmN;
 
     const uint8_t *wt[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) wt[i] = p.w + (size_t)min(n0 / 16 + 4 * wave + i, tiles - 1) * KT * UB;
     // x loads: load q of wave w fills rows 16 q + 4 w .. + 3; lane l takes row + l / 16 and
     // the chunk that belongs in its slot
-    uint32_t xrow[4];
+    const uint16_t *xrow[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) xrow[q] = (uint32_t)min(t0 + 16 * q + 4 * wave + (lane >> 4), p.T - 1) * (uint32_t)(p.K / 8);
+    for (int q = 0; q < 4; ++q) xrow[q] = p.x + (size_t)min(t0 + 16 * q + 4 * wave + (lane >> 4), p.T - 1) * p.K;
     const int chunk = (lane & 15) ^ ((4 * wave + (lane >> 4)) & 15);
-    const uint32_t lds0 = lds_offset(smem);
 
-    auto issue_x = [&](int kt) __attribute__((always_inline)) {
+    // scales: lanes 2 GP i .. + 2 GP - 1 take row tile i's
+    const uint8_t *const scales =
+        p.w + (size_t)min(n0 / 16 + 4 * wave + min(lane / (2 * GP), 3), tiles - 1) * KT * UB + kI4Codes + lane % (2 * GP) * 16;
+
+    // Loads and reads of different stages go through __restrict__ pointers: the compiler
+    // lets no LDS read pass a direct-to-LDS load in flight that may write what it reads.
+    auto issue_x = [&](int kt, uint8_t *__restrict__ st) __attribute__((always_inline)) {
         // past the end of a row: its last inputs, whose scales are 0
         const uint32_t at = (uint32_t)min(kt * 16 + chunk, p.K / 8 - 1);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            load_lds_hidden<16>(reinterpret_cast<const uint8_t *>(p.x) + (size_t)(xrow[q] + at) * 16,
-                                lds0 + (kt & 1) * kI4GemmStage + (16 * q + 4 * wave) * 256);
+            load_lds16(xrow[q] + (size_t)at * 8, st + (16 * q + 4 * wave) * 256);
+        if (lane < 8 * GP) load_lds16(reinterpret_cast<const uint16_t *>(scales + (size_t)kt * UB), st + kI4GemmX + 512 * wave);
     };
+    const uint32_t lane16 = 16 * (uint32_t)lane;
     auto issue_w = [&](int kt, u32x4_t (&d)[4]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = *gptr(wt[i] + (size_t)kt * UB + 16 * lane);
+        for (int i = 0; i < 4; ++i) d[i] = *gptr(wt[i] + (size_t)kt * UB + lane16);
     };
-    u32x4_t w0[4], w1[4];
-    issue_w(0, w0);
-    issue_x(0);
+    u32x4_t ahead[4];
+    issue_w(0, ahead);
+    issue_x(0, smem);
 
-    // ---- what the zero points take off: tot = -sum over groups of (s z)[n] sums[t], an fp32
-    // product of four groups a step
     f32x4_t tot[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int m = 0; m < 4; ++m) tot[i][m] = f32x4_t{};
     const int groups = p.K / G;
-    for (int q = 0; q < groups; q += 4) {
-        const int gr = min(q + g, groups - 1);
-        float b[4];
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            b[m] = sums[(size_t)min(t0 + 16 * m + r, p.T - 1) * groups + gr];
-            if (q + g >= groups) b[m] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint8_t *side = wt[i] + (size_t)(gr / GP) * UB + kI4Codes;
-            const float s = i4_scale(*reinterpret_cast<const uint16_t *>(side + (gr % GP) * 32 + 2 * r), FP16);
-            const float z = ZEROS ? (float)side[GP * 32 + (gr % GP) * 16 + r] : 8.0f;
-#pragma unroll
-            for (int m = 0; m < 4; ++m) tot[i][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(-s * z, b[m], tot[i][m], 0, 0, 0);
-        }
-    }
+    const __bf16 one = (__bf16)1.0f;
+    const bf16x8_t ones = {one, one, one, one, one, one, one, one};
 
-    auto step = [&](auto more, int kt, u32x4_t (&d)[4], u32x4_t (&next)[4]) __attribute__((always_inline)) {
+    // What the zero points take off: tot -= sum of (s z)[n] sx[t] over up to 16 groups from
+    // q0 on, whose sums of x lie in s_sums: fp32 products of four groups at a time
+    auto take_off = [&](int q0) __attribute__((always_inline)) {
+        const float *const sums = &s_sums[q0 / kI4GemmSums & 1][0][0];
+        // (not unrolled: with more loads at a time their registers are spilled)
+#pragma unroll 1
+        for (int q = 0; q < kI4GemmSums; q += 4) {
+            const int gr = min(q0 + q + g, groups - 1);
+            const bool on = q0 + q + g < groups;
+            uint32_t sz[4], zz[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint8_t *unit = wt[i] + (size_t)((uint32_t)gr / GP * UB);
+                sz[i] = *reinterpret_cast<const uint16_t *>(unit + i4_scale_at(r, gr % GP, GP));
+                zz[i] = ZEROS ? unit[i4_zero_at(r, gr % GP, GP)] : 8;
+            }
+            float b[4];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) b[m] = on ? sums[(q + g) * kI4GemmM + 16 * m + r] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = on ? -i4_scale(sz[i], FP16) * (float)zz[i] : 0.0f;
+#pragma unroll
+                for (int m = 0; m < 4; ++m) tot[i][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b[m], tot[i][m], 0, 0, 0);
+            }
+        }
+    };
+
+    auto step = [&](int kt, const uint8_t *__restrict__ cur, uint8_t *__restrict__ nxt)
+        __attribute__((always_inline)) {
         wait_vm<0>();
         ring_barrier();
+        if (kt && kt * GP % kI4GemmSums == 0) take_off(kt * GP - kI4GemmSums);
+        u32x4_t d[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(d[i]));
-        uint2 s4[GP][4];
-#pragma unroll
-        for (int gi = 0; gi < GP; ++gi)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                s4[gi][i] = *reinterpret_cast<const uint2 *>(wt[i] + (size_t)kt * UB + kI4Codes + gi * 32 + 8 * g);
-        if constexpr (decltype(more)::value) {
-            issue_x(kt + 1);
-            issue_w(kt + 1, next);
+        for (int i = 0; i < 4; ++i) {
+            d[i] = ahead[i];
+            asm volatile("" : "+v"(d[i]));
         }
-        const uint8_t *st = smem + (kt & 1) * kI4GemmStage + r * 256;
+        issue_x(min(kt + 1, KT - 1), nxt);
+        issue_w(min(kt + 1, KT - 1), ahead);
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t *st = cur + r * 256, *sc = cur + kI4GemmX + 512 * wave + g * (8 * GP);
 #pragma unroll
         for (int gi = 0; gi < GP; ++gi) {
             bf16x8_t x[JG][4];
@@ -358,6 +353,15 @@ __global__ __launch_bounds__(256, 2) void i4_gemm_kernel(I4Linear p, const float
 #pragma unroll
                 for (int m = 0; m < 4; ++m)
                     x[j][m] = *reinterpret_cast<const bf16x8_t *>(st + m * 4096 + (((4 * (gi * JG + j) + g) ^ r) << 4));
+            // the group's sums of x, of the wave's own token tile
+            f32x4_t sx = {};
+#pragma unroll
+            for (int j = 0; j < JG; ++j)
+                sx = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    ones, *reinterpret_cast<const bf16x8_t *>(st + wave * 4096 + (((4 * (gi * JG + j) + g) ^ r) << 4)), sx, 0, 0, 0);
+            const int gr = kt * GP + gi;
+            // (of every g the same value: a branch round this store has registers spilled)
+            s_sums[gr / kI4GemmSums & 1][gr % kI4GemmSums][16 * wave + r] = sx[0];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 f32x4_t acc[4];
@@ -368,26 +372,22 @@ __global__ __launch_bounds__(256, 2) void i4_gemm_kernel(I4Linear p, const float
                     for (int m = 0; m < 4; ++m)
                         acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[j][m], j == 0 ? f32x4_t{} : acc[m], 0, 0, 0);
                 }
+                const uint2 s4 = *reinterpret_cast<const uint2 *>(sc + i * (32 * GP) + gi * 8);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const float s = i4_scale((q < 2 ? s4[gi][i].x : s4[gi][i].y) >> (16 * (q & 1)) & 0xffffu, FP16);
+                    const float s = i4_scale((q < 2 ? s4.x : s4.y) >> (16 * (q & 1)) & 0xffffu, FP16);
 #pragma unroll
                     for (int m = 0; m < 4; ++m) tot[i][m][q] = fmaf(s, acc[m][q], tot[i][m][q]);
                 }
             }
+            if (GP > 1) __builtin_amdgcn_sched_barrier(0);  // one group's registers at a time
         }
     };
-    int kt = 0;
-    for (; kt + 2 < KT; kt += 2) {
-        step(std::true_type{}, kt, w0, w1);
-        step(std::true_type{}, kt + 1, w1, w0);
-    }
-    if (KT - kt == 2) {
-        step(std::true_type{}, kt, w0, w1);
-        step(std::false_type{}, kt + 1, w1, w0);
-    } else {
-        step(std::false_type{}, kt, w0, w1);
-    }
+    // one body for every step: the last one asks for its own inputs again
+    for (int kt = 0; kt < KT; ++kt) step(kt, smem + (kt & 1) * kI4GemmStage, smem + (~kt & 1) * kI4GemmStage);
+    wait_vm<0>();
+    __syncthreads();
+    take_off((KT - 1) * GP / kI4GemmSums * kI4GemmSums);
 
     // ---- a lane holds token r of each tile and rows 4 g .. + 3 of each row tile: through
     // LDS, out in whole-row 16-byte stores
@@ -418,11 +418,15 @@ __global__ __launch_bounds__(256, 2) void i4_gemm_kernel(I4Linear p, const float
 }
 
 template <int G, bool ZEROS, bool FP16>
-static void i4_gemm_run(const I4Linear &a, float *sums, hipStream_t s) {
-    const int64_t pieces = (int64_t)a.T * a.K / 8;
-    i4_sums_kernel<G><<<(unsigned)((pieces + 255) / 256), 256, 0, s>>>(a.x, pieces, sums);
-    const int64_t total = (int64_t)((a.T + kI4GemmM - 1) / kI4GemmM) * ((a.N + kI4GemmN - 1) / kI4GemmN);
-    i4_gemm_kernel<G, ZEROS, FP16><<<(unsigned)((total + 7) / 8 * 8), 256, 0, s>>>(a, sums);
+static void i4_gemm_run(const I4Linear &a, hipStream_t s) {
+    const int TB = (a.T + kI4GemmM - 1) / kI4GemmM, NB = (a.N + kI4GemmN - 1) / kI4GemmN;
+    // bytes of x and of W that an XCD reads, with the tokens in `cut` parts and the rows in 8 / cut
+    int cut = 1;
+    auto read = [&](int c) { return 2.0 * a.T / c + 0.55 * a.N * c / 8; };
+    for (int c : {2, 4, 8})
+        if (c <= TB && read(c) < read(cut)) cut = c;
+    const int per_t = (TB + cut - 1) / cut, per_n = (NB * cut + 7) / 8;
+    i4_gemm_kernel<G, ZEROS, FP16><<<(unsigned)(8 * per_t * per_n), 256, 0, s>>>(a, cut);
 }
 
 template <int G, bool ZEROS, bool FP16, int MT, int WV, bool KEEP>
@@ -439,20 +443,20 @@ static bool i4_many(int T, int N) {
 }
 
 template <int G, bool ZEROS, bool FP16>
-static void i4_linear_launch(const I4Linear &a, float *sums, hipStream_t s) {
+static void i4_linear_launch(const I4Linear &a, hipStream_t s) {
     const int KU = (a.K + kI4In - 1) / kI4In, tiles = (a.N + kI4Rows - 1) / kI4Rows;
     if (i4_many(a.T, a.N)) {
-        i4_gemm_run<G, ZEROS, FP16>(a, sums, s);
+        i4_gemm_run<G, ZEROS, FP16>(a, s);
     } else if (a.T > 32) {
-        i4_split_run<G, ZEROS, FP16, 4, 4, true>(a, s);
+        i4_split_run<G, ZEROS, FP16, 4, 8, true>(a, s);
     } else if (a.T > 16) {
-        i4_split_run<G, ZEROS, FP16, 2, 4, true>(a, s);
+        i4_split_run<G, ZEROS, FP16, 2, 8, true>(a, s);
     } else if (KU > 8 && KU <= 16) {
         if (tiles <= 1024) i4_rows_kernel<G, ZEROS, FP16, 8, 2, true><<<(unsigned)tiles, 512, 0, s>>>(a);
         else i4_rows_kernel<G, ZEROS, FP16, 8, 2, false><<<G == 32 ? 256 : 512, 512, 0, s>>>(a);
     } else if (KU > 24 && KU <= 32 && tiles <= 256) {
         i4_rows_kernel<G, ZEROS, FP16, 8, 4, true><<<(unsigned)tiles, 512, 0, s>>>(a);
-    } else if (KU > 16 && tiles <= 512) {
+    } else if (KU > 32 && tiles <= 512) {
         i4_split_run<G, ZEROS, FP16, 1, 16, false>(a, s);
     } else {
         i4_split_run<G, ZEROS, FP16, 1, 8, false>(a, s);
@@ -463,36 +467,23 @@ static void i4_linear_launch(const I4Linear &a, float *sums, hipStream_t s) {
 
 using namespace pd;
 
-static bool i4_linear_ok(int T, int N, int K, int G) {
-    return i4_shape_ok(N, K, G) && i4_units(N, K) <= ((int64_t)1 << 26) - 4 && T >= 1;
-}
-
-PD_API size_t pdscope_linear_int4_workspace_size(int T, int N, int K, int G) {
-    return i4_linear_ok(T, N, K, G) && i4_many(T, N) ? (size_t)T * (K / G) * sizeof(float) : 0;
-}
-
 PD_API int pdscope_linear_int4(const void *x, const void *w, const void *bias, int T, int N, int K, int G, int zeros,
-                               int fp16_scales, void *y, void *workspace, void *stream) {
+                               int fp16_scales, void *y, void *stream) {
     if (!x || !w || !y) return fail(kEInval, "linear_int4: null pointer");
     if (!i4_shape_ok(N, K, G) || i4_units(N, K) > ((int64_t)1 << 26) - 4)
         return fail(kEInval, "linear_int4: need 1 <= N <= 2^24, G of 32, 64 or 128 and K % G == 0, K <= 2^20");
     if (T < 1) return fail(kEInval, "linear_int4: need T >= 1");
     for (const void *p : {x, w})
         if (reinterpret_cast<uintptr_t>(p) % 16) return fail(kEInval, "linear_int4: x and w need 16-byte alignment");
-    // launches have fewer than 2^32 threads (at most 1024 for 16 rows of W and 16 of x, and one for
-    // eight inputs), and 16-byte pieces of x are counted in 32 bits
+    // a launch has fewer than 2^32 threads: at most 1024 for 16 rows of W and 16 of x
     if ((((int64_t)N + 15) / 16) * (((int64_t)T + 15) / 16) > ((int64_t)1 << 22) - 1)
         return fail(kEInval, "linear_int4: too many outputs for one launch");
-    if ((int64_t)T * K > ((int64_t)1 << 35) - 4096) return fail(kEInval, "linear_int4: too many inputs for one launch");
-    if (pdscope_linear_int4_workspace_size(T, N, K, G) && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4))
-        return fail(kEInval, "linear_int4: this many rows need a workspace");
     const I4Linear a{(const uint8_t *)w, (const uint16_t *)x, (const uint16_t *)bias, (uint16_t *)y, T, N, K};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     auto group = [&](auto g) {
         constexpr int GG = decltype(g)::value;
-        auto *sums = (float *)workspace;
-        if (zeros) fp16_scales ? i4_linear_launch<GG, true, true>(a, sums, s) : i4_linear_launch<GG, true, false>(a, sums, s);
-        else fp16_scales ? i4_linear_launch<GG, false, true>(a, sums, s) : i4_linear_launch<GG, false, false>(a, sums, s);
+        if (zeros) fp16_scales ? i4_linear_launch<GG, true, true>(a, s) : i4_linear_launch<GG, true, false>(a, s);
+        else fp16_scales ? i4_linear_launch<GG, false, true>(a, s) : i4_linear_launch<GG, false, false>(a, s);
     };
     if (G == 32) group(std::integral_constant<int, 32>{});
     else if (G == 64) group(std::integral_constant<int, 64>{});

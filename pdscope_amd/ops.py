@@ -998,15 +998,9 @@ def int4_dequantize(w: Int4Weight, out=None) -> torch.Tensor:
     return out
 
 
-def linear_int4_workspace_size(T, N, K, group) -> int:
-    """Bytes of linear_int4's workspace: 0 for few rows."""
-    return int(_lib.load().pdscope_linear_int4_workspace_size(int(T), int(N), int(K), int(group)))
-
-
-def linear_int4(x, w: Int4Weight, bias=None, out=None, workspace=None) -> torch.Tensor:
+def linear_int4(x, w: Int4Weight, bias=None, out=None) -> torch.Tensor:
     """x [T, K] bf16 times a 4-bit matrix: bf16 [T, N] = x W^T + bias ([N] bf16 or
-    None), rounded once; any T (see pdscope_linear_int4).  workspace: uint8 of
-    linear_int4_workspace_size bytes, allocated where it is needed and left out."""
+    None), rounded once; any T (see pdscope_linear_int4)."""
     _need(x, "x", BF16, 2)
     dev = x.device
     _need_int4(w, dev)
@@ -1020,15 +1014,8 @@ def linear_int4(x, w: Int4Weight, bias=None, out=None, workspace=None) -> torch.
     elif not _fits(out, BF16, (T, w.N), dev):
         _refuse(out, "out", BF16, (T, w.N), dev)
     if T:
-        need = linear_int4_workspace_size(T, w.N, K, w.group) if T > 16 else 0
-        if workspace is not None:
-            _need(workspace, "workspace", torch.uint8, 1, dev)
-            if workspace.numel() < need:
-                raise ValueError(f"workspace must hold {need} bytes, got {workspace.numel()}")
-        elif need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         _call_on(dev, "pdscope_linear_int4", _p(x), _p(w.units), _p(bias), T, w.N, K, w.group, int(w.zeros),
-                 int(w.scale_dtype is torch.float16), _p(out), _p(workspace))
+                 int(w.scale_dtype is torch.float16), _p(out))
     return out
 
 
