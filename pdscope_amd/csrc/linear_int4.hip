@@ -132,14 +132,17 @@ __global__ __launch_bounds__(64 * WV) void i4_split_kernel(I4Linear p) {
     }
 }
 
-// Up to 16 tokens.  Each of the WV waves keeps U units' worth of x (and its groups'
+constexpr int kI4RowsWaves = 8, kI4RowsUnits = 2;
+
+// Up to 16 tokens, K up to 2048.  Each wave keeps two units' worth of x (and its groups'
 // sums, which do not depend on the row) in registers and takes these units of
 // one row tile after the other, the tiles ahead on their way while it works on one; the
-// waves' parts meet in LDS.  ONE: a workgroup has a single tile.
-template <int G, bool ZEROS, bool FP16, int WV, int U, bool ONE>
-__global__ __launch_bounds__(64 * WV) void i4_rows_kernel(I4Linear p) {
+// waves' parts meet in LDS.
+template <int G, bool ZEROS, bool FP16>
+__global__ __launch_bounds__(64 * kI4RowsWaves) void i4_rows_kernel(I4Linear p) {
+    constexpr int WV = kI4RowsWaves, U = kI4RowsUnits;
     constexpr int UB = i4_unit_bytes(G, ZEROS), GP = kI4In / G, JG = 4 / GP;
-    __shared__ f32x4_t s_part[ONE ? 1 : 2][WV][64];
+    __shared__ f32x4_t s_part[2][WV][64];
     const int lane = lane_id(), ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int tiles = (p.N + kI4Rows - 1) / kI4Rows, KU = (p.K + kI4In - 1) / kI4In, stride = gridDim.x;
     struct Held {
@@ -175,7 +178,7 @@ __global__ __launch_bounds__(64 * WV) void i4_rows_kernel(I4Linear p) {
             if (k >= p.K) v = make_uint4(0, 0, 0, 0);
             x[i][j] = __builtin_bit_cast(bf16x8_t, v);
         }
-    if (!ONE) load(blockIdx.x + stride, d1);
+    load(blockIdx.x + stride, d1);
 #pragma unroll
     for (int i = 0; i < U; ++i)
 #pragma unroll
@@ -191,7 +194,7 @@ __global__ __launch_bounds__(64 * WV) void i4_rows_kernel(I4Linear p) {
         const bool mine = ks == it % WV;
         float bias[4];
         if (mine) i4_bias(p, tile * 16 + 4 * g, bias);
-        if (!ONE) load(tile + 2 * stride, ahead);
+        load(tile + 2 * stride, ahead);
         f32x4_t tot = {};
 #pragma unroll
         for (int i = 0; i < U; ++i)
@@ -208,7 +211,7 @@ __global__ __launch_bounds__(64 * WV) void i4_rows_kernel(I4Linear p) {
             }
         // two buffers in turn: who sums tile it is at the barrier of it + 1 before
         // anyone writes the same buffer for it + 2
-        f32x4_t(&part)[WV][64] = s_part[ONE ? 0 : it & 1];
+        f32x4_t(&part)[WV][64] = s_part[it & 1];
         if (r < p.T) part[ks][lane] = tot;
         ring_barrier();
         if (mine && r < p.T) {
@@ -219,10 +222,6 @@ __global__ __launch_bounds__(64 * WV) void i4_rows_kernel(I4Linear p) {
         }
     };
     int tile = blockIdx.x;
-    if (ONE) {
-        step(tile, 0, d0, d2);
-        return;
-    }
     for (int it = 0;; it += 3) {
         step(tile, it, d0, d2);
         if ((tile += stride) >= tiles) break;
@@ -235,34 +234,38 @@ __global__ __launch_bounds__(64 * WV) void i4_rows_kernel(I4Linear p) {
 
 // ---- many tokens
 
-constexpr int kI4GemmM = 64, kI4GemmN = 256;
+constexpr int kI4GemmM = 64;
 constexpr int kI4GemmX = kI4GemmM * 256;           // a stage's x, behind it its scales:
 constexpr int kI4GemmStage = kI4GemmX + 4 * 512;  // 128 bytes at most for each of four tiles of four waves
 constexpr int kI4GemmSums = 16;                    // groups whose sums of x are kept at a time
-constexpr int kI4GemmOut = kI4GemmN * 2 + 16;
 
 // 64 tokens x 256 rows of W, K in steps of 128: a wave has four row tiles to
 // itself, whose codes go from memory to registers a step ahead; x streams through two LDS
 // stages in 256-byte rows whose 16-byte chunk c lies in slot c ^ (row % 16).
-template <int G, bool ZEROS, bool FP16>
-__global__ __launch_bounds__(256, 2) void i4_gemm_kernel(I4Linear p, int cut) {
+template <int G, bool ZEROS, bool FP16, int RT, int KS>
+__global__ __launch_bounds__(256 * KS, 2) void i4_gemm_kernel(I4Linear p, int cut) {
     constexpr int UB = i4_unit_bytes(G, ZEROS), GP = kI4In / G, JG = 4 / GP;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[std::max(2 * kI4GemmStage, kI4GemmM * kI4GemmOut)];
-    __shared__ float s_sums[2][kI4GemmSums][kI4GemmM];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int kN = 64 * RT, kOut = kN * 2 + 16;       // rows of W, bytes of a staged output row
+    constexpr int kParts = (KS - 1) * 4 * RT * 4 * 64 * 16;  // fp32 totals of the waves of the other parts of K
+    __shared__ __attribute__((aligned(1024))) uint8_t smem_all[std::max({KS * 2 * kI4GemmStage, kParts, kI4GemmM * kOut})];
+    __shared__ float s_sums_all[KS][2][kI4GemmSums][kI4GemmM];
+    const int tid = threadIdx.x, lane = tid & 63, wave_all = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int part = wave_all >> 2, wave = wave_all & 3;  // its part of the steps, its four row tiles
+    uint8_t *const smem = smem_all + part * (2 * kI4GemmStage);
+    float(&s_sums)[2][kI4GemmSums][kI4GemmM] = s_sums_all[part];
     const int r = lane & 15, g = lane >> 4;
     const int tiles = (p.N + kI4Rows - 1) / kI4Rows, KT = (p.K + kI4In - 1) / kI4In;
     // the tiles in `cut` x 8 / `cut` rectangles, one per XCD: tokens and rows of W whose
     // sum in bytes is least, for its L2; tokens fastest
-    const int TB = (p.T + kI4GemmM - 1) / kI4GemmM, NB = (p.N + kI4GemmN - 1) / kI4GemmN;
+    const int TB = (p.T + kI4GemmM - 1) / kI4GemmM, NB = (p.N + kN - 1) / kN;
     const int xcd = blockIdx.x & 7, pos = blockIdx.x >> 3, per_t = (TB + cut - 1) / cut, per_n = (NB * cut + 7) / 8;
     const int tb = xcd % cut * per_t + pos % per_t, nb = xcd / cut * per_n + pos / per_t;
     if (tb >= TB || nb >= NB) return;
-    const int t0 = tb * kI4GemmM, n0 = nb * kI4GemmN;
+    const int t0 = tb * kI4GemmM, n0 = nb * kN;
 
-    const uint8_t *wt[4];
+    const uint8_t *wt[RT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) wt[i] = p.w + (size_t)min(n0 / 16 + 4 * wave + i, tiles - 1) * KT * UB;
+    for (int i = 0; i < RT; ++i) wt[i] = p.w + (size_t)min(n0 / 16 + RT * wave + i, tiles - 1) * KT * UB;
     // x loads: load q of wave w fills rows 16 q + 4 w .. + 3; lane l takes row + l / 16 and
     // the chunk that belongs in its slot
     const uint16_t *xrow[4];
@@ -272,7 +275,7 @@ __global__ __launch_bounds__(256, 2) void i4_gemm_kernel(I4Linear p, int cut) {
 
     // scales: lanes 2 GP i .. + 2 GP - 1 take row tile i's
     const uint8_t *const scales =
-        p.w + (size_t)min(n0 / 16 + 4 * wave + min(lane / (2 * GP), 3), tiles - 1) * KT * UB + kI4Codes + lane % (2 * GP) * 16;
+        p.w + (size_t)min(n0 / 16 + RT * wave + min(lane / (2 * GP), RT - 1), tiles - 1) * KT * UB + kI4Codes + lane % (2 * GP) * 16;
 
     // Loads and reads of different stages go through __restrict__ pointers: the compiler
     // lets no LDS read pass a direct-to-LDS load in flight that may write what it reads.
@@ -282,20 +285,20 @@ __global__ __launch_bounds__(256, 2) void i4_gemm_kernel(I4Linear p, int cut) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             load_lds16(xrow[q] + (size_t)at * 8, st + (16 * q + 4 * wave) * 256);
-        if (lane < 8 * GP) load_lds16(reinterpret_cast<const uint16_t *>(scales + (size_t)kt * UB), st + kI4GemmX + 512 * wave);
+        if (lane < 2 * RT * GP) load_lds16(reinterpret_cast<const uint16_t *>(scales + (size_t)kt * UB), st + kI4GemmX + 512 * wave);
     };
     const uint32_t lane16 = 16 * (uint32_t)lane;
-    auto issue_w = [&](int kt, u32x4_t (&d)[4]) __attribute__((always_inline)) {
+    auto issue_w = [&](int kt, u32x4_t (&d)[RT]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = *gptr(wt[i] + (size_t)kt * UB + lane16);
+        for (int i = 0; i < RT; ++i) d[i] = *gptr(wt[i] + (size_t)kt * UB + lane16);
     };
-    u32x4_t ahead[4];
-    issue_w(0, ahead);
-    issue_x(0, smem);
+    u32x4_t ahead[RT];
+    issue_w(min(part, KT - 1), ahead);
+    issue_x(min(part, KT - 1), smem);
 
-    f32x4_t tot[4][4];
+    f32x4_t tot[RT][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int m = 0; m < 4; ++m) tot[i][m] = f32x4_t{};
     const int groups = p.K / G;
@@ -306,44 +309,49 @@ __global__ __launch_bounds__(256, 2) void i4_gemm_kernel(I4Linear p, int cut) {
     // q0 on, whose sums of x lie in s_sums: fp32 products of four groups at a time
     auto take_off = [&](int q0) __attribute__((always_inline)) {
         const float *const sums = &s_sums[q0 / kI4GemmSums & 1][0][0];
-        // (not unrolled: with more loads at a time their registers are spilled)
-#pragma unroll 1
-        for (int q = 0; q < kI4GemmSums; q += 4) {
-            const int gr = min(q0 + q + g, groups - 1);
-            const bool on = q0 + q + g < groups;
-            uint32_t sz[4], zz[4];
+        uint32_t sz[kI4GemmSums / 4][RT], zz[kI4GemmSums / 4][RT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint8_t *unit = wt[i] + (size_t)((uint32_t)gr / GP * UB);
-                sz[i] = *reinterpret_cast<const uint16_t *>(unit + i4_scale_at(r, gr % GP, GP));
-                zz[i] = ZEROS ? unit[i4_zero_at(r, gr % GP, GP)] : 8;
+        for (int q = 0; q < kI4GemmSums / 4; ++q) {
+            const uint32_t own = q0 + 4 * q + g, gr = min((own / GP * KS + part) * GP + own % GP, (uint32_t)groups - 1);
+            const uint32_t at = gr / GP * UB + i4_scale_at<uint32_t>(r, gr % GP, GP), zt = gr / GP * UB + i4_zero_at<uint32_t>(r, gr % GP, GP);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                sz[q][i] = *reinterpret_cast<const uint16_t *>(wt[i] + at);
+                zz[q][i] = ZEROS ? wt[i][zt] : 8;
             }
+        }
+#pragma unroll
+        for (int q = 0; q < kI4GemmSums / 4; ++q) {
+            const uint32_t own = q0 + 4 * q + g;  // the part's group; the row's:
+            const bool on = (own / GP * KS + part) * GP + own % GP < (uint32_t)groups;
             float b[4];
 #pragma unroll
-            for (int m = 0; m < 4; ++m) b[m] = on ? sums[(q + g) * kI4GemmM + 16 * m + r] : 0.0f;
+            for (int m = 0; m < 4; ++m) b[m] = on ? sums[(4 * q + g) * kI4GemmM + 16 * m + r] : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = on ? -i4_scale(sz[i], FP16) * (float)zz[i] : 0.0f;
+            for (int i = 0; i < RT; ++i) {
+                const float a = on ? -i4_scale(sz[q][i], FP16) * (float)zz[q][i] : 0.0f;
 #pragma unroll
                 for (int m = 0; m < 4; ++m) tot[i][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b[m], tot[i][m], 0, 0, 0);
             }
         }
     };
 
-    auto step = [&](int kt, const uint8_t *__restrict__ cur, uint8_t *__restrict__ nxt)
+    auto step = [&](int it, const uint8_t *__restrict__ cur, uint8_t *__restrict__ nxt)
         __attribute__((always_inline)) {
+        const int kt = it * KS + part;
         wait_vm<0>();
         ring_barrier();
-        if (kt && kt * GP % kI4GemmSums == 0) take_off(kt * GP - kI4GemmSums);
-        u32x4_t d[4];
+        if (it && it * GP % kI4GemmSums == 0) take_off(it * GP - kI4GemmSums);
+        u32x4_t d[RT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < RT; ++i) {
             d[i] = ahead[i];
             asm volatile("" : "+v"(d[i]));
         }
-        issue_x(min(kt + 1, KT - 1), nxt);
-        issue_w(min(kt + 1, KT - 1), ahead);
+        issue_x(min(kt + KS, KT - 1), nxt);
+        issue_w(min(kt + KS, KT - 1), ahead);
         __builtin_amdgcn_sched_barrier(0);
+        if (KS > 1 && kt >= KT) return;
         const uint8_t *st = cur + r * 256, *sc = cur + kI4GemmX + 512 * wave + g * (8 * GP);
 #pragma unroll
         for (int gi = 0; gi < GP; ++gi) {
@@ -359,11 +367,11 @@ __global__ __launch_bounds__(256, 2) void i4_gemm_kernel(I4Linear p, int cut) {
             for (int j = 0; j < JG; ++j)
                 sx = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                     ones, *reinterpret_cast<const bf16x8_t *>(st + wave * 4096 + (((4 * (gi * JG + j) + g) ^ r) << 4)), sx, 0, 0, 0);
-            const int gr = kt * GP + gi;
+            const int gr = it * GP + gi;
             // (of every g the same value: a branch round this store has registers spilled)
             s_sums[gr / kI4GemmSums & 1][gr % kI4GemmSums][16 * wave + r] = sx[0];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < RT; ++i) {
                 f32x4_t acc[4];
 #pragma unroll
                 for (int j = 0; j < JG; ++j) {
@@ -384,30 +392,49 @@ __global__ __launch_bounds__(256, 2) void i4_gemm_kernel(I4Linear p, int cut) {
         }
     };
     // one body for every step: the last one asks for its own inputs again
-    for (int kt = 0; kt < KT; ++kt) step(kt, smem + (kt & 1) * kI4GemmStage, smem + (~kt & 1) * kI4GemmStage);
+    const int IT = (KT + KS - 1) / KS;
+    for (int it = 0; it < IT; ++it) step(it, smem + (it & 1) * kI4GemmStage, smem + (~it & 1) * kI4GemmStage);
     wait_vm<0>();
     __syncthreads();
-    take_off((KT - 1) * GP / kI4GemmSums * kI4GemmSums);
+    take_off((IT - 1) * GP / kI4GemmSums * kI4GemmSums);
+    if constexpr (KS > 1) {
+        // the second part's totals, to the first
+        f32x4_t *const parts = reinterpret_cast<f32x4_t *>(smem_all) + wave * (4 * RT * 64) + lane;
+        if (part) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) parts[(4 * i + m) * 64] = tot[i][m];
+        }
+        __syncthreads();
+        if (!part) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) tot[i][m] += parts[(4 * i + m) * 64];
+        }
+    }
 
     // ---- a lane holds token r of each tile and rows 4 g .. + 3 of each row tile: through
     // LDS, out in whole-row 16-byte stores
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RT; ++i) {
+        if (KS > 1 && part) break;
         float bias[4];
-        i4_bias(p, n0 + 64 * wave + 16 * i + 4 * g, bias);
+        i4_bias(p, n0 + 16 * (RT * wave + i) + 4 * g, bias);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const f32x4_t v = tot[i][m];
-            *reinterpret_cast<uint2 *>(smem + (16 * m + r) * kI4GemmOut + (64 * wave + 16 * i + 4 * g) * 2) =
+            *reinterpret_cast<uint2 *>(smem_all + (16 * m + r) * kOut + (16 * (RT * wave + i) + 4 * g) * 2) =
                 make_uint2(f2bf2_hw(v[0] + bias[0], v[1] + bias[1]), f2bf2_hw(v[2] + bias[2], v[3] + bias[3]));
         }
     }
     __syncthreads();
-    const int rows = min(kI4GemmM, p.T - t0), cols = min(kI4GemmN, p.N - n0);
-    for (int c = tid; c < rows * (kI4GemmN / 8); c += 256) {
-        const int row = c / (kI4GemmN / 8), col = c % (kI4GemmN / 8) * 8;
-        const uint8_t *from = smem + row * kI4GemmOut + col * 2;
+    const int rows = min(kI4GemmM, p.T - t0), cols = min(kN, p.N - n0);
+    for (int c = tid; c < rows * (kN / 8); c += 256 * KS) {
+        const int row = c / (kN / 8), col = c % (kN / 8) * 8;
+        const uint8_t *from = smem_all + row * kOut + col * 2;
         uint16_t *to = p.y + (size_t)(t0 + row) * p.N + n0 + col;
         if (col + 8 <= cols && p.N % 8 == 0) {
             st_through(to, *reinterpret_cast<const uint4 *>(from));
@@ -417,16 +444,19 @@ __global__ __launch_bounds__(256, 2) void i4_gemm_kernel(I4Linear p, int cut) {
     }
 }
 
-template <int G, bool ZEROS, bool FP16>
+template <int G, bool ZEROS, bool FP16, int RT, int KS>
 static void i4_gemm_run(const I4Linear &a, hipStream_t s) {
-    const int TB = (a.T + kI4GemmM - 1) / kI4GemmM, NB = (a.N + kI4GemmN - 1) / kI4GemmN;
-    // bytes of x and of W that an XCD reads, with the tokens in `cut` parts and the rows in 8 / cut
+    const int TB = (a.T + kI4GemmM - 1) / kI4GemmM, NB = (a.N + 64 * RT - 1) / (64 * RT);
+    // the tokens in `cut` parts and the rows in 8 / cut: by the rounds of the XCD with most
+    // tiles (eight waves of a CU at a time), then by the bytes of x and of W that one reads (T =
+    // 300, N = 2816, K = 2048 12.4 us, by the bytes alone 22.0)
     int cut = 1;
+    auto rounds = [&](int c) { return ((TB + c - 1) / c * ((NB * c + 7) / 8) * KS + 63) / 64; };
     auto read = [&](int c) { return 2.0 * a.T / c + 0.55 * a.N * c / 8; };
     for (int c : {2, 4, 8})
-        if (c <= TB && read(c) < read(cut)) cut = c;
+        if (c <= TB && (rounds(c) < rounds(cut) || (rounds(c) == rounds(cut) && read(c) < read(cut)))) cut = c;
     const int per_t = (TB + cut - 1) / cut, per_n = (NB * cut + 7) / 8;
-    i4_gemm_kernel<G, ZEROS, FP16><<<(unsigned)(8 * per_t * per_n), 256, 0, s>>>(a, cut);
+    i4_gemm_kernel<G, ZEROS, FP16, RT, KS><<<(unsigned)(8 * per_t * per_n), 256 * KS, 0, s>>>(a, cut);
 }
 
 template <int G, bool ZEROS, bool FP16, int MT, int WV, bool KEEP>
@@ -435,31 +465,53 @@ static void i4_split_run(const I4Linear &a, hipStream_t s) {
     i4_split_kernel<G, ZEROS, FP16, MT, WV, KEEP><<<(unsigned)(tiles * down), 64 * WV, 0, s>>>(a);
 }
 
-// Whether T rows take the launch for many tokens: from 48 of its 64 x 256 tiles on (N =
-// 4096, K = 2048: T = 128 19.4 us split and 31.0 there, T = 192 28 and 31; a tile's time
-// is that of its K axis, however few there are).
-static bool i4_many(int T, int N) {
-    return T > 16 && (int64_t)((T + kI4GemmM - 1) / kI4GemmM) * ((N + kI4GemmN - 1) / kI4GemmN) >= 48;
+// A launch by token tiles of a workgroup, in the time of one that has a single one, over
+// two: workgroups come 256 at a time, and one of MT tiles takes about as long as
+// MT + 1.  N = 1024, K = 2048: T = 64 4.6 / 7.1 / 10.6 us for MT = 1 / 2 / 4; N = 4096, K = 2048:
+// T = 17 6.1 / 5.7 / 6.7, T = 48 - / 10.0 / 9.8; N = 2048, K = 4096: T = 32 6.9 / 10.3 / 12.5,
+// T = 64 - / 11.1 / 17.9, T = 192 - / 26.6 / 32.5.
+static int64_t i4_split_cost(int T, int tiles, int MT) {
+    return ((int64_t)tiles * ((T + 16 * MT - 1) / (16 * MT)) + 255) / 256 * (MT + 1);
 }
 
 template <int G, bool ZEROS, bool FP16>
 static void i4_linear_launch(const I4Linear &a, hipStream_t s) {
     const int KU = (a.K + kI4In - 1) / kI4In, tiles = (a.N + kI4Rows - 1) / kI4Rows;
-    if (i4_many(a.T, a.N)) {
-        i4_gemm_run<G, ZEROS, FP16>(a, s);
-    } else if (a.T > 32) {
-        i4_split_run<G, ZEROS, FP16, 4, 8, true>(a, s);
-    } else if (a.T > 16) {
+    if (a.T <= 16) {
+        // x in registers where a wave has many tiles to read with it: from 24576 units on, or
+        // 16384 where x is most of a tile's reading (K = 2048, G = 128: N = 16384 8.0 us and 7.3
+        // without, 24576 9.2 and 9.4, 49152 12.9 and 15.8, 151936 29.5 and 42.8; T = 16: 16384 10.2
+        // and 11.2, 151936 35 and 80).  G = 32 has registers for one workgroup per CU.
+        if (KU > kI4RowsWaves && KU <= kI4RowsWaves * kI4RowsUnits && (int64_t)tiles * KU > (a.T > 4 ? 16384 : 24576)) {
+            const int blocks = std::min(tiles, G == 32 ? 256 : 512);
+            i4_rows_kernel<G, ZEROS, FP16><<<(unsigned)blocks, 64 * kI4RowsWaves, 0, s>>>(a);
+        } else if (a.T <= 4 && KU > 16 && tiles <= 512) {
+            // 16 waves where there are few workgroups and little of x (K = 2816, N = 2048, T = 1 4.5 us
+            // against 4.7 with eight, K = 8192, N = 4096 8.3 against 9.2; T = 16 5.9 against 5.7)
+            i4_split_run<G, ZEROS, FP16, 1, 16, false>(a, s);
+        } else {
+            i4_split_run<G, ZEROS, FP16, 1, 8, false>(a, s);
+        }
+        return;
+    }
+    const int64_t one = i4_split_cost(a.T, tiles, 1), two = i4_split_cost(a.T, tiles, 2), four = i4_split_cost(a.T, tiles, 4);
+    // The tiled launch takes the time of about seven such units (K = 2048: N = 4096, T = 64 12.0
+    // us against 11.0 split, T = 128 12.0 and 17.8; N = 16384, T = 24 12.1 and 15.7; K = 4096: N =
+    // 2048, T = 128 19.3 and 18.1, T = 192 19.4 and 26.6).  With few tiles a step's time is that
+    // of its loads, and small ones that share the K axis have fewer steps: N = 4096,
+    // K = 2048, tiles of 64 tokens x 64 rows in two parts / x 128 in two / x 256: T = 256 12.2 / 15.6 /
+    // 24.7 us, T = 512 22.4 / 15.7 / 24.6, T = 1024 42 / 29 / 25.5, T = 2048 83 / 57 / 37.3.
+    if (std::min({one, two, four}) >= 7) {
+        const int64_t down = (a.T + kI4GemmM - 1) / kI4GemmM;
+        if (down * ((a.N + 63) / 64) <= 256) i4_gemm_run<G, ZEROS, FP16, 1, 2>(a, s);
+        else if (down * ((a.N + 127) / 128) <= 256) i4_gemm_run<G, ZEROS, FP16, 2, 2>(a, s);
+        else i4_gemm_run<G, ZEROS, FP16, 4, 1>(a, s);
+    } else if (one <= two && one <= four) {
+        i4_split_run<G, ZEROS, FP16, 1, 8, true>(a, s);
+    } else if (two <= four) {
         i4_split_run<G, ZEROS, FP16, 2, 8, true>(a, s);
-    } else if (KU > 8 && KU <= 16) {
-        if (tiles <= 1024) i4_rows_kernel<G, ZEROS, FP16, 8, 2, true><<<(unsigned)tiles, 512, 0, s>>>(a);
-        else i4_rows_kernel<G, ZEROS, FP16, 8, 2, false><<<G == 32 ? 256 : 512, 512, 0, s>>>(a);
-    } else if (KU > 24 && KU <= 32 && tiles <= 256) {
-        i4_rows_kernel<G, ZEROS, FP16, 8, 4, true><<<(unsigned)tiles, 512, 0, s>>>(a);
-    } else if (KU > 32 && tiles <= 512) {
-        i4_split_run<G, ZEROS, FP16, 1, 16, false>(a, s);
     } else {
-        i4_split_run<G, ZEROS, FP16, 1, 8, false>(a, s);
+        i4_split_run<G, ZEROS, FP16, 4, 8, true>(a, s);
     }
 }
 

@@ -90,6 +90,9 @@ SIZES = [(1, 1, 32, 32), (1, 16, 128, 128), (2, 15, 64, 64), (1, 4096, 2048, 128
          # the launch for many rows: one step of the K axis, two, odd ones, ragged edges of every kind
          (800, 1000, 96, 32), (800, 1000, 128, 128), (3100, 257, 352, 32), (3071, 255, 192, 64), (1500, 520, 1408, 128),
          (1025, 771, 4096, 64), (2049, 513, 1056, 32),
+         # smaller tiles, whose steps two halves of a workgroup share: one step, an odd count of them
+         (70, 2100, 128, 128), (200, 1030, 1056, 32), (130, 4100, 640, 64), (513, 2048, 4096, 128), (512, 4095, 352, 32),
+         (449, 4096, 128, 64), (700, 1500, 2048, 128), (24, 16384, 1408, 128),
          # many row tiles for one workgroup
          (1, 20000, 2048, 128), (3, 16401, 1152, 32), (16, 33000, 1984, 64), (2, 9000, 8192, 128), (4, 5000, 4096, 128)]
 
