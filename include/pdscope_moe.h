@@ -548,7 +548,7 @@ int pdscope_swiglu_grouped_mxfp8(const void *x, const void *x_scales, const int3
  * infinity or NaN gives NaN, and a row of W with an infinite or NaN scale NaN or
  * infinities.  y may overlap nothing.
  * Limits: 1 <= N <= 2^24, K % G == 0, K <= 2^20, fewer than 2^37 - 2^13 weights in whole
- * 16 x 128 units; T >= 1, (N/16) * (T/16), each rounded up, below 2^22; x, w,
+ * 16 x 128 units; 1 <= T <= 2^24, (N/256) * (T/64), each rounded up, at most 2^23; x, w,
  * codes and weight 16-byte aligned.
  */
 size_t pdscope_int4_bytes(int N, int K, int G, int zeros);

@@ -7,6 +7,13 @@
 //
 // The whole numbers q are bf16 exactly, so the products with x are exact and a
 // group's two sums are held in fp32; the scale enters once a group, in fp32.
+//
+// Three launches: up to 16 rows of x against many of W with x in registers
+// (i4_rows_kernel), few rows with the K axis split over the waves of a workgroup
+// (i4_split_kernel), many in tiles through LDS (i4_gemm_kernel).  The first two are
+// bound by W's bytes or, for small matrices, by a launch's start, one load and one join: N = 151936, K
+// = 2048, G = 64 with zero points, one row 36 us (4.7 TB/s); N = 2048, K = 4096, G = 128 4.8 us (0.9).
+// With 16 rows x's bytes cost as much, read again for every row tile: N = 4096, K = 2048 5.1 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -239,9 +246,18 @@ constexpr int kI4GemmX = kI4GemmM * 256;           // a stage's x, behind it its
 constexpr int kI4GemmStage = kI4GemmX + 4 * 512;  // 128 bytes at most for each of four tiles of four waves
 constexpr int kI4GemmSums = 16;                    // groups whose sums of x are kept at a time
 
-// 64 tokens x 256 rows of W, K in steps of 128: a wave has four row tiles to
+// 64 tokens x 64 RT rows of W, K in steps of 128: a wave has RT row tiles to
 // itself, whose codes go from memory to registers a step ahead; x streams through two LDS
-// stages in 256-byte rows whose 16-byte chunk c lies in slot c ^ (row % 16).
+// stages in 256-byte rows whose 16-byte chunk c lies in slot c ^ (row % 16).  The
+// steps are dealt to KS parts of the workgroup, whose totals meet in LDS.
+//
+// A step of RT = 4 issues 64 products and 4 for the sums, and some 220 other vector
+// instructions (112 decode, 64 scale) through the same port, so two waves take about 3100 cycles
+// where the products alone need 2200.  N = 4096, K = 2048, G = 128, T = 2048 37.3 us,
+// 0.92 PFLOP/s (G = 64 43, G = 32 56: more scalings), of which the loop 26, what is before and behind it
+// 4.3; without the loop's loads 33.6, without decoding 35.8, without reading x from LDS 30.4.  T = 4096 and
+// K = 4096 1.0 PFLOP/s.  Held back by neither alone; reading x 32 inputs ahead of the products or
+// another order of them changed nothing.
 template <int G, bool ZEROS, bool FP16, int RT, int KS>
 __global__ __launch_bounds__(256 * KS, 2) void i4_gemm_kernel(I4Linear p, int cut) {
     constexpr int UB = i4_unit_bytes(G, ZEROS), GP = kI4In / G, JG = 4 / GP;
@@ -451,7 +467,7 @@ static void i4_gemm_run(const I4Linear &a, hipStream_t s) {
     // tiles (eight waves of a CU at a time), then by the bytes of x and of W that one reads (T =
     // 300, N = 2816, K = 2048 12.4 us, by the bytes alone 22.0)
     int cut = 1;
-    auto rounds = [&](int c) { return ((TB + c - 1) / c * ((NB * c + 7) / 8) * KS + 63) / 64; };
+    auto rounds = [&](int c) { return ((int64_t)((TB + c - 1) / c) * ((NB * c + 7) / 8) * KS + 63) / 64; };
     auto read = [&](int c) { return 2.0 * a.T / c + 0.55 * a.N * c / 8; };
     for (int c : {2, 4, 8})
         if (c <= TB && (rounds(c) < rounds(cut) || (rounds(c) == rounds(cut) && read(c) < read(cut)))) cut = c;
@@ -524,11 +540,12 @@ PD_API int pdscope_linear_int4(const void *x, const void *w, const void *bias, i
     if (!x || !w || !y) return fail(kEInval, "linear_int4: null pointer");
     if (!i4_shape_ok(N, K, G) || i4_units(N, K) > ((int64_t)1 << 26) - 4)
         return fail(kEInval, "linear_int4: need 1 <= N <= 2^24, G of 32, 64 or 128 and K % G == 0, K <= 2^20");
-    if (T < 1) return fail(kEInval, "linear_int4: need T >= 1");
+    if (T < 1 || T > (1 << 24)) return fail(kEInval, "linear_int4: need 1 <= T <= 2^24");
     for (const void *p : {x, w})
         if (reinterpret_cast<uintptr_t>(p) % 16) return fail(kEInval, "linear_int4: x and w need 16-byte alignment");
-    // a launch has fewer than 2^32 threads: at most 1024 for 16 rows of W and 16 of x
-    if ((((int64_t)N + 15) / 16) * (((int64_t)T + 15) / 16) > ((int64_t)1 << 22) - 1)
+    // a launch has fewer than 2^32 threads: 256 a tile of the tiled one, whose rectangles
+    // may add 8 tiles a row and a column of them
+    if (((int64_t)N + 255) / 256 * (((int64_t)T + kI4GemmM - 1) / kI4GemmM) > (int64_t)1 << 23)
         return fail(kEInval, "linear_int4: too many outputs for one launch");
     const I4Linear a{(const uint8_t *)w, (const uint16_t *)x, (const uint16_t *)bias, (uint16_t *)y, T, N, K};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);

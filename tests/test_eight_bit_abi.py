@@ -118,6 +118,6 @@ def test_products():
         call("null", **{p: None})
     for p in ("x", "w"):
         call("16-byte", **{p: ODD})
-    for T in (0, -5):
-        call("T >= 1", T=T)
-    call("too many outputs", T=1 << 20, N=1 << 16)
+    for T in (0, -5, (1 << 24) + 1):
+        call("1 <= T", T=T)
+    call("too many outputs", T=1 << 24, N=1 << 16)

@@ -162,6 +162,18 @@ def test_a_matrix_past_2_to_the_31_bytes():
             check(y[:, a:a + 100].contiguous(), x, codes[a:a + 100], scales[a:a + 100], None, G)
 
 
+def test_more_than_2_to_the_31_outputs():
+    T, N, K, G = 16_400, 140_000, 64, 64
+    codes, scales, _ = make(N, K, G, seed=11)
+    w = ops.int4_pack(codes, scales)
+    x = torch.randn((T, K), device=DEV).to(BF16)
+    y = ops.linear_int4(x, w)
+    rows = torch.tensor([0, 63, 64, T // 2, T - 1], device=DEV)
+    check(y[rows], x[rows], codes, scales, None, G)
+    for at in (0, N - 3):
+        check(y[:, at:at + 3].contiguous(), x, codes[at:at + 3], scales[at:at + 3], None, G)
+
+
 @pytest.mark.parametrize("T", [2, 40, 1700])
 def test_replay_and_another_stream(T):
     N, K, G = 300, 2048, 128
