@@ -27,6 +27,7 @@ struct I4Linear {
     const uint16_t *x, *bias;
     uint16_t *y;
     int T, N, K;
+    bool wide;  // every 8 outputs of a row from its start on lie at a multiple of 16 bytes
 };
 
 // What a wave holds of a unit: codes, its rows' scales and zero points (rows 4 g .. +
@@ -87,7 +88,7 @@ struct I4Unit {
 __device__ __forceinline__ void i4_store(const I4Linear &p, int t, int n, f32x4_t v, const float (&bias)[4]) {
     const uint32_t lo = f2bf2_hw(v[0] + bias[0], v[1] + bias[1]), hi = f2bf2_hw(v[2] + bias[2], v[3] + bias[3]);
     uint16_t *y = p.y + (size_t)t * p.N + n;
-    if (n + 3 < p.N && p.N % 4 == 0) {
+    if (n + 3 < p.N && p.wide) {
         *reinterpret_cast<uint2 *>(y) = make_uint2(lo, hi);
     } else {
         if (n < p.N) y[0] = (uint16_t)lo;
@@ -452,7 +453,7 @@ __global__ __launch_bounds__(256 * KS, 2) void i4_gemm_kernel(I4Linear p, int cu
         const int row = c / (kN / 8), col = c % (kN / 8) * 8;
         const uint8_t *from = smem_all + row * kOut + col * 2;
         uint16_t *to = p.y + (size_t)(t0 + row) * p.N + n0 + col;
-        if (col + 8 <= cols && p.N % 8 == 0) {
+        if (col + 8 <= cols && p.wide) {
             st_through(to, *reinterpret_cast<const uint4 *>(from));
         } else {
             for (int i = 0; i < 8 && col + i < cols; ++i) to[i] = reinterpret_cast<const uint16_t *>(from)[i];
@@ -547,7 +548,8 @@ PD_API int pdscope_linear_int4(const void *x, const void *w, const void *bias, i
     // may add 8 tiles a row and a column of them
     if (((int64_t)N + 255) / 256 * (((int64_t)T + kI4GemmM - 1) / kI4GemmM) > (int64_t)1 << 23)
         return fail(kEInval, "linear_int4: too many outputs for one launch");
-    const I4Linear a{(const uint8_t *)w, (const uint16_t *)x, (const uint16_t *)bias, (uint16_t *)y, T, N, K};
+    const I4Linear a{(const uint8_t *)w, (const uint16_t *)x, (const uint16_t *)bias, (uint16_t *)y, T, N, K,
+                     N % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     auto group = [&](auto g) {
         constexpr int GG = decltype(g)::value;

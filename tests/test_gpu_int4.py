@@ -162,6 +162,21 @@ def test_a_matrix_past_2_to_the_31_bytes():
             check(y[:, a:a + 100].contiguous(), x, codes[a:a + 100], scales[a:a + 100], None, G)
 
 
+@pytest.mark.parametrize("T", [1, 20, 60, 200, 900, 2300])
+def test_outputs_at_addresses_that_16_bytes_do_not_divide(T):
+    N, K, G = 1040, 384, 128
+    codes, scales, z = make(N, K, G, zeros=True, seed=12)
+    w = ops.int4_pack(codes, scales, z)
+    x = torch.randn((T, K), device=DEV).to(BF16)
+    want = ops.linear_int4(x, w)
+    for off in (1, 2, 4):
+        room = torch.full((T * N + 16,), 7.0, dtype=BF16, device=DEV)
+        ops.linear_int4(x, w, out=room[off:off + T * N].view(T, N))
+        assert torch.equal(room[off:off + T * N].view(T, N), want)
+        assert (room[:off] == 7).all() and (room[off + T * N:] == 7).all()
+    check(want, x, codes, scales, z, G)
+
+
 def test_more_than_2_to_the_31_outputs():
     T, N, K, G = 16_400, 140_000, 64, 64
     codes, scales, _ = make(N, K, G, seed=11)
