@@ -245,7 +245,6 @@ __global__ __launch_bounds__(64 * kI4RowsWaves) void i4_rows_kernel(I4Linear p) 
 constexpr int kI4GemmM = 64;
 constexpr int kI4GemmX = kI4GemmM * 256;           // a stage's x, behind it its scales:
 constexpr int kI4GemmStage = kI4GemmX + 4 * 512;  // 128 bytes at most for each of four tiles of four waves
-constexpr int kI4GemmSums = 16;                    // groups whose sums of x are kept at a time
 
 // 64 tokens x 64 RT rows of W, K in steps of 128: a wave has RT row tiles to
 // itself, whose codes go from memory to registers a step ahead; x streams through two LDS
@@ -260,16 +259,17 @@ constexpr int kI4GemmSums = 16;                    // groups whose sums of x are
 // K = 4096 1.0 PFLOP/s.  Held back by neither alone; reading x 32 inputs ahead of the products or
 // another order of them changed nothing.
 template <int G, bool ZEROS, bool FP16, int RT, int KS>
-__global__ __launch_bounds__(256 * KS, 2) void i4_gemm_kernel(I4Linear p, int cut) {
+__global__ __launch_bounds__(256 * KS, std::max(KS, 2)) void i4_gemm_kernel(I4Linear p, int cut) {
     constexpr int UB = i4_unit_bytes(G, ZEROS), GP = kI4In / G, JG = 4 / GP;
-    constexpr int kN = 64 * RT, kOut = kN * 2 + 16;       // rows of W, bytes of a staged output row
+    constexpr int kN = 64 * RT, kOut = kN * 2 + 16;          // rows of W, bytes of a staged output row
+    constexpr int kSums = KS > 2 ? 8 : 16;                   // groups whose sums of x are kept at a time
     constexpr int kParts = (KS - 1) * 4 * RT * 4 * 64 * 16;  // fp32 totals of the waves of the other parts of K
     __shared__ __attribute__((aligned(1024))) uint8_t smem_all[std::max({KS * 2 * kI4GemmStage, kParts, kI4GemmM * kOut})];
-    __shared__ float s_sums_all[KS][2][kI4GemmSums][kI4GemmM];
+    __shared__ float s_sums_all[KS][2][kSums][kI4GemmM];
     const int tid = threadIdx.x, lane = tid & 63, wave_all = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int part = wave_all >> 2, wave = wave_all & 3;  // its part of the steps, its four row tiles
+    const int part = wave_all >> 2, wave = wave_all & 3;  // its part of the steps, its row tiles
     uint8_t *const smem = smem_all + part * (2 * kI4GemmStage);
-    float(&s_sums)[2][kI4GemmSums][kI4GemmM] = s_sums_all[part];
+    float(&s_sums)[2][kSums][kI4GemmM] = s_sums_all[part];
     const int r = lane & 15, g = lane >> 4;
     const int tiles = (p.N + kI4Rows - 1) / kI4Rows, KT = (p.K + kI4In - 1) / kI4In;
     // the tiles in `cut` x 8 / `cut` rectangles, one per XCD: tokens and rows of W whose
@@ -322,13 +322,13 @@ __global__ __launch_bounds__(256 * KS, 2) void i4_gemm_kernel(I4Linear p, int cu
     const __bf16 one = (__bf16)1.0f;
     const bf16x8_t ones = {one, one, one, one, one, one, one, one};
 
-    // What the zero points take off: tot -= sum of (s z)[n] sx[t] over up to 16 groups from
+    // What the zero points take off: tot -= sum of (s z)[n] sx[t] over up to kSums groups from
     // q0 on, whose sums of x lie in s_sums: fp32 products of four groups at a time
     auto take_off = [&](int q0) __attribute__((always_inline)) {
-        const float *const sums = &s_sums[q0 / kI4GemmSums & 1][0][0];
-        uint32_t sz[kI4GemmSums / 4][RT], zz[kI4GemmSums / 4][RT];
+        const float *const sums = &s_sums[q0 / kSums & 1][0][0];
+        uint32_t sz[kSums / 4][RT], zz[kSums / 4][RT];
 #pragma unroll
-        for (int q = 0; q < kI4GemmSums / 4; ++q) {
+        for (int q = 0; q < kSums / 4; ++q) {
             const uint32_t own = q0 + 4 * q + g, gr = min((own / GP * KS + part) * GP + own % GP, (uint32_t)groups - 1);
             const uint32_t at = gr / GP * UB + i4_scale_at<uint32_t>(r, gr % GP, GP), zt = gr / GP * UB + i4_zero_at<uint32_t>(r, gr % GP, GP);
 #pragma unroll
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(256 * KS, 2) void i4_gemm_kernel(I4Linear p, int cu
             }
         }
 #pragma unroll
-        for (int q = 0; q < kI4GemmSums / 4; ++q) {
+        for (int q = 0; q < kSums / 4; ++q) {
             const uint32_t own = q0 + 4 * q + g;  // the part's group; the row's:
             const bool on = (own / GP * KS + part) * GP + own % GP < (uint32_t)groups;
             float b[4];
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(256 * KS, 2) void i4_gemm_kernel(I4Linear p, int cu
         const int kt = it * KS + part;
         wait_vm<0>();
         ring_barrier();
-        if (it && it * GP % kI4GemmSums == 0) take_off(it * GP - kI4GemmSums);
+        if (it && it * GP % kSums == 0) take_off(it * GP - kSums);
         u32x4_t d[RT];
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -386,7 +386,7 @@ __global__ __launch_bounds__(256 * KS, 2) void i4_gemm_kernel(I4Linear p, int cu
                     ones, *reinterpret_cast<const bf16x8_t *>(st + wave * 4096 + (((4 * (gi * JG + j) + g) ^ r) << 4)), sx, 0, 0, 0);
             const int gr = it * GP + gi;
             // (of every g the same value: a branch round this store has registers spilled)
-            s_sums[gr / kI4GemmSums & 1][gr % kI4GemmSums][16 * wave + r] = sx[0];
+            s_sums[gr / kSums & 1][gr % kSums][16 * wave + r] = sx[0];
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
                 f32x4_t acc[4];
@@ -413,22 +413,24 @@ __global__ __launch_bounds__(256 * KS, 2) void i4_gemm_kernel(I4Linear p, int cu
     for (int it = 0; it < IT; ++it) step(it, smem + (it & 1) * kI4GemmStage, smem + (~it & 1) * kI4GemmStage);
     wait_vm<0>();
     __syncthreads();
-    take_off((IT - 1) * GP / kI4GemmSums * kI4GemmSums);
+    take_off((IT - 1) * GP / kSums * kSums);
     if constexpr (KS > 1) {
-        // the second part's totals, to the first
+        // the other parts' totals, to the first, which adds them in order
         f32x4_t *const parts = reinterpret_cast<f32x4_t *>(smem_all) + wave * (4 * RT * 64) + lane;
         if (part) {
 #pragma unroll
             for (int i = 0; i < RT; ++i)
 #pragma unroll
-                for (int m = 0; m < 4; ++m) parts[(4 * i + m) * 64] = tot[i][m];
+                for (int m = 0; m < 4; ++m) parts[((part - 1) * 16 * RT + 4 * i + m) * 64] = tot[i][m];
         }
         __syncthreads();
         if (!part) {
 #pragma unroll
-            for (int i = 0; i < RT; ++i)
+            for (int k = 0; k < KS - 1; ++k)
 #pragma unroll
-                for (int m = 0; m < 4; ++m) tot[i][m] += parts[(4 * i + m) * 64];
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) tot[i][m] += parts[(k * 16 * RT + 4 * i + m) * 64];
         }
     }
 
@@ -465,10 +467,12 @@ template <int G, bool ZEROS, bool FP16, int RT, int KS>
 static void i4_gemm_run(const I4Linear &a, hipStream_t s) {
     const int TB = (a.T + kI4GemmM - 1) / kI4GemmM, NB = (a.N + 64 * RT - 1) / (64 * RT);
     // the tokens in `cut` parts and the rows in 8 / cut: by the rounds of the XCD with most
-    // tiles (eight waves of a CU at a time), then by the bytes of x and of W that one reads (T =
-    // 300, N = 2816, K = 2048 12.4 us, by the bytes alone 22.0)
+    // tiles (two workgroups a CU at a time, one where parts share the K axis), then by the bytes
+    // of x and of W that one reads (T = 300, N = 2816, K = 2048 in two parts 12.4 us, by the bytes
+    // alone 22.0)
     int cut = 1;
-    auto rounds = [&](int c) { return ((int64_t)((TB + c - 1) / c) * ((NB * c + 7) / 8) * KS + 63) / 64; };
+    constexpr int per_xcd = KS == 1 ? 64 : 32;
+    auto rounds = [&](int c) { return ((int64_t)((TB + c - 1) / c) * ((NB * c + 7) / 8) + per_xcd - 1) / per_xcd; };
     auto read = [&](int c) { return 2.0 * a.T / c + 0.55 * a.N * c / 8; };
     for (int c : {2, 4, 8})
         if (c <= TB && (rounds(c) < rounds(cut) || (rounds(c) == rounds(cut) && read(c) < read(cut)))) cut = c;
@@ -512,15 +516,16 @@ static void i4_linear_launch(const I4Linear &a, hipStream_t s) {
         return;
     }
     const int64_t one = i4_split_cost(a.T, tiles, 1), two = i4_split_cost(a.T, tiles, 2), four = i4_split_cost(a.T, tiles, 4);
-    // The tiled launch takes the time of about seven such units (K = 2048: N = 4096, T = 64 12.0
-    // us against 11.0 split, T = 128 12.0 and 17.8; N = 16384, T = 24 12.1 and 15.7; K = 4096: N =
-    // 2048, T = 128 19.3 and 18.1, T = 192 19.4 and 26.6).  With few tiles a step's time is that
+    // The tiled launch takes the time of about seven such units (K = 2048: N = 4096, T = 64 10.9
+    // us against 10.3 split, T = 128 11.0 and 17.8; N = 16384, T = 24 11.1 and 15.7; K = 4096: N =
+    // 2048, T = 128 16.6 and 17.3, T = 192 16.8 and 26.6).  With few tiles a step's time is that
     // of its loads, and small ones that share the K axis have fewer steps: N = 4096,
-    // K = 2048, tiles of 64 tokens x 64 rows in two parts / x 128 in two / x 256: T = 256 12.2 / 15.6 /
-    // 24.7 us, T = 512 22.4 / 15.7 / 24.6, T = 1024 42 / 29 / 25.5, T = 2048 83 / 57 / 37.3.
+    // K = 2048, tiles of 64 tokens x 64 rows in four parts / in two / x 128 in two / x 256: T = 256 11.1 / 12.0
+    // / 15.6 / 24.7 us, T = 512 - / 22.4 / 15.7 / 24.6, T = 1024 - / 42 / 29 / 25.5, T = 2048 - / 83 / 57 /
+    // 37.3; K = 4096, N = 2048, T = 512 16.9 / 19.4 / 24.9 / 44.6.
     if (std::min({one, two, four}) >= 7) {
         const int64_t down = (a.T + kI4GemmM - 1) / kI4GemmM;
-        if (down * ((a.N + 63) / 64) <= 256) i4_gemm_run<G, ZEROS, FP16, 1, 2>(a, s);
+        if (down * ((a.N + 63) / 64) <= 256) i4_gemm_run<G, ZEROS, FP16, 1, 4>(a, s);
         else if (down * ((a.N + 127) / 128) <= 256) i4_gemm_run<G, ZEROS, FP16, 2, 2>(a, s);
         else i4_gemm_run<G, ZEROS, FP16, 4, 1>(a, s);
     } else if (one <= two && one <= four) {
