@@ -56,6 +56,7 @@ class MoEWorkspace:
         # 8-bit rows of x for moe_forward(activations="mxfp8") without rows of the caller's
         self.x_rows = ops.mxfp8_empty(max_tokens, H, device) if mxfp8 else None
         self._h_rows = None
+        self._packed = None
         # always-on shared experts (one fused MLP of intermediate shared_I over every token)
         self.shared_I = shared_I
         if shared_I:
@@ -105,8 +106,12 @@ class MoEWorkspace:
         """What pack writes for T tokens."""
         if not 0 < T <= self.max_tokens:
             raise ValueError(f"token count {T} outside workspace capacity {self.max_tokens}")
-        n = T * self.k
-        return ops.Packed(self.counts, self.offsets, self.perm_token[:n], self.perm_pos[:n], self.row_of[:n])
+        # (the views of the last T: their three slices take 4 us of a call)
+        if self._packed is None or self._packed[0] != T:
+            n = T * self.k
+            self._packed = T, ops.Packed(self.counts, self.offsets, self.perm_token[:n], self.perm_pos[:n],
+                                         self.row_of[:n])
+        return self._packed[1]
 
     def views(self, T: int):
         packed = self.packed(T)

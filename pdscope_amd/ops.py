@@ -183,6 +183,7 @@ class Packed:
     row_of: torch.Tensor      # int32 [T*k]
 
 
+@functools.lru_cache(maxsize=256)
 def pack_workspace_size(T: int, k: int, E: int) -> int:
     return int(_lib.load().pdscope_pack_workspace_size(int(T), int(k), int(E)))
 
@@ -206,20 +207,24 @@ def pack(ids, E, out: Packed | None = None, workspace=None, *, schedule=None) ->
     args = (_p(ids), T, k, E, _p(out.counts), _p(out.offsets), _p(out.perm_token), _p(out.perm_pos), _p(out.row_of),
             _p(workspace) if need else None)
     if schedule is None:
-        _lib.call("pdscope_pack", *args, _stream(dev))
+        _call_on(dev, "pdscope_pack", *args)
         return out
     sel, block_m, order, tile_start, *second = schedule
     block_m2, tile_start2 = second if second else (0, None)
-    for t, name, size in ((sel, "sel", 0), (order, "order", sel.numel()), (tile_start, "tile_start", sel.numel() + 1)):
-        _need(t, name, torch.int32, 1, dev)
-        if t.numel() < size:
+    if not _line(sel, torch.int32, dev):
+        _need(sel, "sel", torch.int32, 1, dev)
+    nsel = sel.shape[0]
+    for t, name, size in ((order, "order", nsel), (tile_start, "tile_start", nsel + 1)):
+        if not _line(t, torch.int32, dev):
+            _need(t, name, torch.int32, 1, dev)
+        if t.shape[0] < size:
             raise ValueError(f"{name} smaller than sel needs")
     if tile_start2 is not None:
         _need(tile_start2, "tile_start2", torch.int32, 1, dev)
-        if tile_start2.numel() < sel.numel() + 1:
+        if tile_start2.numel() < nsel + 1:
             raise ValueError("tile_start2 smaller than sel needs")
-    _lib.call("pdscope_pack_schedule_balanced", *args, _p(sel), sel.numel(), block_m, block_m2, _p(order),
-              _p(tile_start), _p(tile_start2), _stream(dev))
+    _call_on(dev, "pdscope_pack_schedule_balanced", *args, _p(sel), nsel, block_m, block_m2, _p(order), _p(tile_start),
+             _p(tile_start2))
     return out
 
 
@@ -689,15 +694,17 @@ class DecodeBinding:
 def merge(y, row_of, w, out, add_in=None, *, mode="fused"):
     _need(w, "weights", BF16, 2)
     dev = w.device
-    _need(y, "y", BF16, None, dev)
-    _need(row_of, "row_of", torch.int32, 1, dev)
+    if not _line(y, BF16, dev):
+        _need(y, "y", BF16, None, dev)
+    if not _line(row_of, torch.int32, dev):
+        _need(row_of, "row_of", torch.int32, 1, dev)
     _need(out, "out", BF16, 2, dev)
     T, k = w.shape
     H = out.shape[1]
     if add_in is not None:
         _need(add_in, "add_in", BF16, 2, dev)
     name = "pdscope_merge_ordered" if merge_mode(mode) else "pdscope_merge"
-    _lib.call(name, _p(y), _p(row_of), _p(w), T, k, H, _p(add_in), _p(out), _stream(dev))
+    _call_on(dev, name, _p(y), _p(row_of), _p(w), T, k, H, _p(add_in), _p(out))
     return out
 
 
@@ -876,6 +883,7 @@ def mxfp8_dequantize(rows: MxRows, out=None) -> torch.Tensor:
     return out
 
 
+@functools.lru_cache(maxsize=256)
 def grouped_mxfp8_block_m(rows_hint: int) -> int:
     """Row tile of swiglu_grouped_mxfp8 for rows_hint mean rows per expert."""
     return int(_lib.load().pdscope_grouped_mxfp8_block_m(int(rows_hint)))
@@ -893,7 +901,8 @@ def swiglu_grouped_mxfp8(x: MxRows, perm_token, offsets, sel, tile_start, max_ti
     if not _line(slots, torch.int64, dev):
         _need(slots, "slots", torch.int64, 1, dev)
     _need_rows(h_ws, "h_ws", None, I, dev)
-    _need(y, "y", BF16, None, dev)
+    if not _line(y, BF16, dev):
+        _need(y, "y", BF16, None, dev)
     check_slots(slots, H, I, "mxfp4")
     rows, nsel = perm_token.shape[0], sel.shape[0]
     if h_ws.codes.shape[0] < rows or y.numel() < rows * H:
