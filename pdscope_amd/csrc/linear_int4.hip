@@ -12,8 +12,9 @@
 // (i4_rows_kernel), few rows with the K axis split over the waves of a workgroup
 // (i4_split_kernel), many in tiles through LDS (i4_gemm_kernel).  The first two are
 // bound by W's bytes or, for small matrices, by a launch's start, one load and one join: N = 151936, K
-// = 2048, G = 64 with zero points, one row 36 us (4.7 TB/s); N = 2048, K = 4096, G = 128 4.8 us (0.9).
-// With 16 rows x's bytes cost as much, read again for every row tile: N = 4096, K = 2048 5.1 us.
+// = 2048, G = 64 with zero points, one row 36 us (4.7 TB/s); K = 4096, G = 128 64 us (5.3); N = 2048,
+// K = 4096 4.8 us (0.9).  With 16 rows x's bytes cost as much, read again by every workgroup: N = 4096, K
+// = 2048 5.1 us, N = 151936, K = 4096 82.
 #include <algorithm>
 #include <type_traits>
 
@@ -30,55 +31,41 @@ struct I4Linear {
     bool wide;  // every 8 outputs of a row from its start on lie at a multiple of 16 bytes
 };
 
-// What a wave holds of a unit: codes, its rows' scales and zero points (rows 4 g .. +
-// 3, a group each), and the inputs of MT tiles of 16 tokens (token r, inputs 8 g .. + 7
-// of each 32).
-template <int G, bool ZEROS, bool FP16, int MT>
+// What a wave holds of a unit: codes, and its rows' scales and zero points (rows 4 g .. +
+// 3, a group each).
+template <int G, bool ZEROS, bool FP16>
 struct I4Unit {
     static constexpr int GP = kI4In / G, JG = 4 / GP;  // groups of a unit, words of a group
     uint4 c;
     I4Side<G, ZEROS, FP16> side;
-    uint4 x[MT][4];
 
-    // KEEP: another workgroup reads the weights too.  Inputs past the end of a row
-    // are read as its last ones: their scales are 0.
+    // KEEP: another workgroup reads the weights too.
     template <bool KEEP>
-    __device__ __forceinline__ void load(const uint8_t *unit, const uint16_t *const (&xr)[MT], int u, int K, int lane) {
-        const int g = lane >> 4;
+    __device__ __forceinline__ void load(const uint8_t *unit, int lane) {
         c = KEEP ? ld_g(unit + 16 * lane) : ld_nt(unit + 16 * lane);
-        side.load(unit, g);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = min(u * kI4In + 32 * j + 8 * g, K - 8);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) x[m][j] = ld_g(xr[m] + k);
-        }
+        side.load(unit, lane >> 4);
     }
 
-    __device__ __forceinline__ void add(f32x4_t (&tot)[MT]) const {
-        const __bf16 one = (__bf16)1.0f;
-        const bf16x8_t ones = {one, one, one, one, one, one, one, one};
+    // sx: the groups' sums of x, the same in every register of a column
+    template <int MT>
+    __device__ __forceinline__ void add(const bf16x8_t (&x)[MT][4], const float (&sx)[MT][GP], f32x4_t (&tot)[MT]) const {
         const uint32_t words[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
         for (int gi = 0; gi < GP; ++gi) {
-            f32x4_t acc[MT], sx[MT];
+            f32x4_t acc[MT];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m] = sx[m] = f32x4_t{};
+            for (int m = 0; m < MT; ++m) acc[m] = f32x4_t{};
 #pragma unroll
             for (int j = gi * JG; j < (gi + 1) * JG; ++j) {
                 const bf16x8_t w = i4_decode(words[j]);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const bf16x8_t v = __builtin_bit_cast(bf16x8_t, x[m][j]);
-                    acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, v, acc[m], 0, 0, 0);
-                    sx[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, v, sx[m], 0, 0, 0);
-                }
+                for (int m = 0; m < MT; ++m) acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[m][j], acc[m], 0, 0, 0);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float sc = side.scale(gi, i), zp = side.zero(gi, i);
 #pragma unroll
-                for (int m = 0; m < MT; ++m) tot[m][i] = fmaf(sc, fmaf(-zp, sx[m][i], acc[m][i]), tot[m][i]);
+                for (int m = 0; m < MT; ++m) tot[m][i] = fmaf(sc, fmaf(-zp, sx[m][gi], acc[m][i]), tot[m][i]);
             }
         }
     }
@@ -102,40 +89,69 @@ __device__ __forceinline__ void i4_bias(const I4Linear &p, int n, float (&bias)[
     for (int q = 0; q < 4; ++q) bias[q] = p.bias ? bf2f(p.bias[min(n + q, p.N - 1)]) : 0.0f;
 }
 
-// A workgroup: one tile of 16 rows of W x MT tiles of 16 tokens, the units of the K
+// A workgroup: RT tiles of 16 rows of W x MT tiles of 16 tokens, the units of the K
 // axis dealt to WV waves, whose parts meet in LDS.
-template <int G, bool ZEROS, bool FP16, int MT, int WV, bool KEEP>
+template <int G, bool ZEROS, bool FP16, int RT, int MT, int WV, bool KEEP>
 __global__ __launch_bounds__(64 * WV) void i4_split_kernel(I4Linear p) {
-    constexpr int UB = i4_unit_bytes(G, ZEROS);
-    __shared__ f32x4_t s_part[WV][MT][64];
-    const int lane = lane_id(), ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15;
-    const int tiles = (p.N + kI4Rows - 1) / kI4Rows, KU = (p.K + kI4In - 1) / kI4In;
-    const int tb = blockIdx.x / tiles, n0 = blockIdx.x - tb * tiles;
-    const uint8_t *const wt = p.w + (size_t)n0 * KU * UB;
+    constexpr int UB = i4_unit_bytes(G, ZEROS), GP = kI4In / G, JG = 4 / GP;
+    __shared__ f32x4_t s_part[WV][RT * MT][64];
+    const int lane = lane_id(), ks = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int tiles = (p.N + kI4Rows - 1) / kI4Rows, KU = (p.K + kI4In - 1) / kI4In, across = (tiles + RT - 1) / RT;
+    const int tb = blockIdx.x / across, n0 = (blockIdx.x - tb * across) * RT;
+    const uint8_t *wt[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) wt[i] = p.w + (size_t)min(n0 + i, tiles - 1) * KU * UB;
     const uint16_t *xr[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) xr[m] = p.x + (size_t)min((tb * MT + m) * 16 + r, p.T - 1) * p.K;
+    const __bf16 one = (__bf16)1.0f;
+    const bf16x8_t ones = {one, one, one, one, one, one, one, one};
 
-    f32x4_t tot[MT];
+    f32x4_t tot[RT][MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) tot[m] = f32x4_t{};
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) tot[i][m] = f32x4_t{};
     for (int u = ks; u < KU; u += WV) {
-        I4Unit<G, ZEROS, FP16, MT> d;
-        d.template load<KEEP>(wt + (size_t)u * UB, xr, u, p.K, lane);
-        d.add(tot);
+        I4Unit<G, ZEROS, FP16> d[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) d[i].template load<KEEP>(wt[i] + (size_t)u * UB, lane);
+        // inputs past the end of a row are read as its last ones: their scales are 0
+        bf16x8_t x[MT][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = min(u * kI4In + 32 * j + 8 * g, p.K - 8);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) x[m][j] = __builtin_bit_cast(bf16x8_t, ld_g(xr[m] + k));
+        }
+        if (RT > 1) __builtin_amdgcn_sched_barrier(0);  // all loads before the first wait
+        float sx[MT][GP];
+#pragma unroll
+        for (int gi = 0; gi < GP; ++gi)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                f32x4_t a = {};
+#pragma unroll
+                for (int j = gi * JG; j < (gi + 1) * JG; ++j) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, x[m][j], a, 0, 0, 0);
+                sx[m][gi] = a[0];
+            }
+#pragma unroll
+        for (int i = 0; i < RT; ++i) d[i].add(x, sx, tot[i]);
     }
     // ---- the waves' parts, in order; lane l has token r and rows 4 g .. + 3
 #pragma unroll
-    for (int m = 0; m < MT; ++m) s_part[ks][m][lane] = tot[m];
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) s_part[ks][i * MT + m][lane] = tot[i][m];
     __syncthreads();
-    for (int q = threadIdx.x; q < MT * 64; q += 64 * WV) {
-        const int m = q >> 6, l = q & 63, t = (tb * MT + m) * 16 + (l & 15), n = n0 * 16 + 4 * (l >> 4);
+    for (int q = threadIdx.x; q < RT * MT * 64; q += 64 * WV) {
+        const int at = q >> 6, l = q & 63, t = (tb * MT + at % MT) * 16 + (l & 15), n = (n0 + at / MT) * 16 + 4 * (l >> 4);
         if (t >= p.T) continue;
         float bias[4];
         i4_bias(p, n, bias);
-        f32x4_t v = s_part[0][m][l];
+        f32x4_t v = s_part[0][at][l];
 #pragma unroll
-        for (int w = 1; w < WV; ++w) v += s_part[w][m][l];
+        for (int w = 1; w < WV; ++w) v += s_part[w][at][l];
         i4_store(p, t, n, v, bias);
     }
 }
@@ -480,10 +496,10 @@ static void i4_gemm_run(const I4Linear &a, hipStream_t s) {
     i4_gemm_kernel<G, ZEROS, FP16, RT, KS><<<(unsigned)(8 * per_t * per_n), 256 * KS, 0, s>>>(a, cut);
 }
 
-template <int G, bool ZEROS, bool FP16, int MT, int WV, bool KEEP>
+template <int G, bool ZEROS, bool FP16, int RT, int MT, int WV, bool KEEP>
 static void i4_split_run(const I4Linear &a, hipStream_t s) {
-    const int64_t tiles = (a.N + 15) / 16, down = (a.T + 16 * MT - 1) / (16 * MT);
-    i4_split_kernel<G, ZEROS, FP16, MT, WV, KEEP><<<(unsigned)(tiles * down), 64 * WV, 0, s>>>(a);
+    const int64_t across = ((a.N + 15) / 16 + RT - 1) / RT, down = (a.T + 16 * MT - 1) / (16 * MT);
+    i4_split_kernel<G, ZEROS, FP16, RT, MT, WV, KEEP><<<(unsigned)(across * down), 64 * WV, 0, s>>>(a);
 }
 
 // A launch by token tiles of a workgroup, in the time of one that has a single one, over
@@ -499,19 +515,28 @@ template <int G, bool ZEROS, bool FP16>
 static void i4_linear_launch(const I4Linear &a, hipStream_t s) {
     const int KU = (a.K + kI4In - 1) / kI4In, tiles = (a.N + kI4Rows - 1) / kI4Rows;
     if (a.T <= 16) {
-        // x in registers where a wave has many tiles to read with it: from 24576 units on, or
-        // 16384 where x is most of a tile's reading (K = 2048, G = 128: N = 16384 8.0 us and 7.3
-        // without, 24576 9.2 and 9.4, 49152 12.9 and 15.8, 151936 29.5 and 42.8; T = 16: 16384 10.2
-        // and 11.2, 151936 35 and 80).  G = 32 has registers for one workgroup per CU.
-        if (KU > kI4RowsWaves && KU <= kI4RowsWaves * kI4RowsUnits && (int64_t)tiles * KU > (a.T > 4 ? 16384 : 24576)) {
+        // x in registers where a wave has very many tiles to read with it (K = 2048, G = 128: N =
+        // 98304 21.3 us against 20.8 with four row tiles a workgroup, T = 16 25.0 and 27.5; N = 151936
+        // 29.6 and 30.7, T = 16 35.0 and 40.7; K = 1536 26.7 and 25.4).  G = 32 has registers for one
+        // workgroup per CU.
+        if (KU > 12 && KU <= kI4RowsWaves * kI4RowsUnits && (int64_t)tiles * KU > 65536) {
             const int blocks = std::min(tiles, G == 32 ? 256 : 512);
             i4_rows_kernel<G, ZEROS, FP16><<<(unsigned)blocks, 64 * kI4RowsWaves, 0, s>>>(a);
-        } else if (a.T <= 4 && KU > 16 && tiles <= 512) {
+        } else if (G > 32 && tiles > 512) {
+            // As many row tiles a workgroup, up to four, as leave one per CU: x is read once for all
+            // of them, and each has more loads on its way.  G = 128, K = 4096, one / two / four: N = 4096
+            // 5.6 / 6.6 / 8.8 us, N = 8192 8.3 / 7.7 / 9.6, N = 16384 12.7 / 11.1 / 10.1, N = 151936 90 / 70 / 64;
+            // T = 16 7.2 / 7.8 / 9.6, 12.4 / 8.6 / 10.5, 20.2 / 14.1 / 11.3, 162 / 103 / 82.  G = 32: N =
+            // 40000 31.4 / 27.9 / 33.5, T = 16 48.6 / 33.3 / 35.3.
+            i4_split_run<G, ZEROS, FP16, 4, 1, 8, false>(a, s);
+        } else if (tiles > 256) {
+            i4_split_run<G, ZEROS, FP16, 2, 1, 8, false>(a, s);
+        } else if (a.T <= 4 && KU > 16) {
             // 16 waves where there are few workgroups and little of x (K = 2816, N = 2048, T = 1 4.5 us
             // against 4.7 with eight, K = 8192, N = 4096 8.3 against 9.2; T = 16 5.9 against 5.7)
-            i4_split_run<G, ZEROS, FP16, 1, 16, false>(a, s);
+            i4_split_run<G, ZEROS, FP16, 1, 1, 16, false>(a, s);
         } else {
-            i4_split_run<G, ZEROS, FP16, 1, 8, false>(a, s);
+            i4_split_run<G, ZEROS, FP16, 1, 1, 8, false>(a, s);
         }
         return;
     }
@@ -529,11 +554,11 @@ static void i4_linear_launch(const I4Linear &a, hipStream_t s) {
         else if (down * ((a.N + 127) / 128) <= 256) i4_gemm_run<G, ZEROS, FP16, 2, 2>(a, s);
         else i4_gemm_run<G, ZEROS, FP16, 4, 1>(a, s);
     } else if (one <= two && one <= four) {
-        i4_split_run<G, ZEROS, FP16, 1, 8, true>(a, s);
+        i4_split_run<G, ZEROS, FP16, 1, 1, 8, true>(a, s);
     } else if (two <= four) {
-        i4_split_run<G, ZEROS, FP16, 2, 8, true>(a, s);
+        i4_split_run<G, ZEROS, FP16, 1, 2, 8, true>(a, s);
     } else {
-        i4_split_run<G, ZEROS, FP16, 4, 8, true>(a, s);
+        i4_split_run<G, ZEROS, FP16, 1, 4, 8, true>(a, s);
     }
 }
 

@@ -94,7 +94,8 @@ SIZES = [(1, 1, 32, 32), (1, 16, 128, 128), (2, 15, 64, 64), (1, 4096, 2048, 128
          (70, 2100, 128, 128), (200, 1030, 1056, 32), (130, 4100, 640, 64), (513, 2048, 4096, 128), (512, 4095, 352, 32),
          (449, 4096, 128, 64), (700, 1500, 2048, 128), (24, 16384, 1408, 128),
          # many row tiles for one workgroup
-         (1, 20000, 2048, 128), (3, 16401, 1152, 32), (16, 33000, 1984, 64), (2, 9000, 8192, 128), (4, 5000, 4096, 128)]
+         (1, 20000, 2048, 128), (3, 16401, 1152, 32), (16, 33000, 1984, 64), (2, 9000, 8192, 128), (4, 5000, 4096, 128),
+         (1, 70000, 2048, 128), (9, 66001, 2016, 32), (16, 80000, 1984, 64), (2, 5000, 352, 32), (13, 8193, 1088, 64), (16, 4113, 96, 32)]
 
 
 @pytest.mark.parametrize("T,N,K,G", SIZES)
