@@ -53,20 +53,24 @@ struct Mx8Grouped {
     uint8_t *out, *out_scales;  // gate/up: h codes and scales; down: y bf16 [rows, H], null
 };
 
+// Waves of a workgroup, a row group each.  Eight in the down half of BM = 32, two workgroups a CU: Qwen
+// shape T = 33 18.5 us against 19.4, T = 8 14.5 against 12.2; DeepSeek-V2-Lite shape T = 33 22.0 against
+// 18.6, T = 128 22.9 against 19.4; of BM = 64 at T = 1303 of the Qwen shape 78 and 49 us against 65 and 39.
+constexpr int kMx8Waves = 4;
 // bytes of a staged output row: 32 columns of h codes or 64 of bf16 y per wave, off the bank line
-template <int NW, bool GATEUP>
-constexpr int kMx8OutRow = NW * (GATEUP ? 32 : 128) + 16;
+template <bool GATEUP>
+constexpr int kMx8OutRow = kMx8Waves * (GATEUP ? 32 : 128) + 16;
 template <int BM>
 constexpr int kMx8Stage = BM * 128 + 256;  // codes and scales of a step's 128 inputs
-template <int BM, int NW, bool GATEUP>
-constexpr int kMx8Lds = std::max(2 * kMx8Stage<BM>, BM * kMx8OutRow<NW, GATEUP> + (GATEUP ? BM * NW : 0));
+template <int BM, bool GATEUP>
+constexpr int kMx8Lds = std::max(2 * kMx8Stage<BM>, BM * kMx8OutRow<GATEUP> + (GATEUP ? BM * kMx8Waves : 0));
 
 // BM rows x four groups (128 h columns or 256 y columns), K in steps of 128, two
 // stages of activations; at least OCC workgroups per CU.
-template <int BM, int NW, bool GATEUP, int OCC>
-__global__ __launch_bounds__(64 * NW, OCC * NW / 4) void mx8_grouped_kernel(Mx8Grouped p) {
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[kMx8Lds<BM, NW, GATEUP>];
-    constexpr int TM = BM / 16;
+template <int BM, bool GATEUP, int OCC>
+__global__ __launch_bounds__(64 * kMx8Waves, OCC) void mx8_grouped_kernel(Mx8Grouped p) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kMx8Lds<BM, GATEUP>];
+    constexpr int TM = BM / 16, NW = kMx8Waves;
     const int H = p.H, I = p.I;
     const int K = GATEUP ? H : I, KT = K / kGroupIn;
     const int groups = GATEUP ? I / 32 : H / kGroupRows, NT = (groups + NW - 1) / NW;
@@ -101,8 +105,8 @@ __global__ __launch_bounds__(64 * NW, OCC * NW / 4) void mx8_grouped_kernel(Mx8G
     // ---- activation loads: load q of wave w fills rows 8 (NW q + w) .. + 7 of 128
     // bytes, whose 16-byte chunk c lies in slot c ^ (row / 2 % 8); lane l takes row + l /
     // 8 and the chunk that belongs in its slot
-    constexpr int RQ = 8 * NW, AL = (BM + RQ - 1) / RQ;  // rows per load of all waves, loads of a wave
-    static_assert(BM % RQ == 0 || BM < RQ, "activation loads");
+    constexpr int RQ = 8 * NW, AL = BM / RQ;  // rows per load of all waves, loads of a wave
+    static_assert(BM % RQ == 0, "activation loads");
     const uint8_t *arow[AL];
     const int lrow = 8 * wave + (lane >> 3);  // in its load's rows
     const uint32_t achunk = (uint32_t)((lane & 7) ^ ((lrow >> 1) & 7));
@@ -198,7 +202,9 @@ __global__ __launch_bounds__(64 * NW, OCC * NW / 4) void mx8_grouped_kernel(Mx8G
         step(std::false_type{}, KT - 1);
     };
     // one straight-line loop for each number of 16-row tiles that hold rows, and for
-    // weights that no other tile reads, which are not kept in the caches
+    // weights that no other tile reads, which are not kept in the caches (Qwen shape, T = 33 gate/up
+    // 31.5 us against 35.8 kept, down 18.5 and 19.1; T = 1303, where most are read by two, nothing kept
+    // 77 and 44 against 65 and 39)
     const int live = (min(BM, row_end - m0) + 15) / 16;
     auto run = [&](auto once) __attribute__((always_inline)) {
         if (live == 1) kloop(std::integral_constant<int, 1>{}, once);
@@ -214,7 +220,7 @@ __global__ __launch_bounds__(64 * NW, OCC * NW / 4) void mx8_grouped_kernel(Mx8G
     // ---- epilogue: a lane holds token row r of each tile and weight rows 4 g ..
     // + 3 of each 16-row tile; through LDS, out in whole-row 16-byte stores.  The 32
     // columns of h that a wave has of a row are one scale block, in four lanes.
-    constexpr int OB = kMx8OutRow<NW, GATEUP>;
+    constexpr int OB = kMx8OutRow<GATEUP>;
     uint8_t *const out_s = smem + BM * OB;
     __syncthreads();
 #pragma unroll
@@ -272,16 +278,16 @@ struct Mx8Call {
     hipStream_t s;
 };
 
-// NWG / NWD waves and OCCG / OCCD workgroups per CU of the gate/up and down halves
-template <int BM, int NWG, int OCCG, int NWD, int OCCD>
+template <int BM, int OCC>
 static int mx8_grouped_launch(const Mx8Call &c, const uint8_t *x, const uint8_t *xs, const int32_t *perm, uint8_t *h,
                               uint8_t *hs, uint8_t *y) {
+    constexpr int NW = kMx8Waves;
     auto grid = [&](int nt) { return (unsigned)(((size_t)c.max_tiles * nt + 7) / 8 * 8); };
-    mx8_grouped_kernel<BM, NWG, true, OCCG><<<grid((c.I / 32 + NWG - 1) / NWG), 64 * NWG, 0, c.s>>>(
+    mx8_grouped_kernel<BM, true, OCC><<<grid((c.I / 32 + NW - 1) / NW), 64 * NW, 0, c.s>>>(
         Mx8Grouped{x, xs, perm, c.offsets, c.sel, c.nsel, c.tile_start, c.slots, c.H, c.I, h, hs});
     const int rc = check_launch("mx8_grouped_kernel<gateup>");
     if (rc) return rc;
-    mx8_grouped_kernel<BM, NWD, false, OCCD><<<grid((c.H / kGroupRows + NWD - 1) / NWD), 64 * NWD, 0, c.s>>>(
+    mx8_grouped_kernel<BM, false, OCC><<<grid((c.H / kGroupRows + NW - 1) / NW), 64 * NW, 0, c.s>>>(
         Mx8Grouped{h, hs, nullptr, c.offsets, c.sel, c.nsel, c.tile_start, c.slots, c.H, c.I, y, nullptr});
     return check_launch("mx8_grouped_kernel<down>");
 }
@@ -309,14 +315,13 @@ PD_API int pdscope_swiglu_grouped_mxfp8(const void *x, const void *x_scales, con
         if (reinterpret_cast<uintptr_t>(p) % 16) return fail(kEInval, "grouped_mxfp8: x, h and y need 16-byte alignment");
     for (const void *p : {x_scales, (const void *)h_scales})
         if (reinterpret_cast<uintptr_t>(p) % 4) return fail(kEInval, "grouped_mxfp8: scales need 4-byte alignment");
-    // a launch has fewer than 2^32 threads: at least 128 columns of h or 256 of y a workgroup
-    // of 256, or 512 of y one of 512
+    // a launch has fewer than 2^32 threads: 128 columns of h or 256 of y a workgroup of 256
     if ((int64_t)max_tiles * ((std::max(I, H / 2) + 127) / 128) * 256 > ((int64_t)1 << 32) - 8192)
         return fail(kEInval, "grouped_mxfp8: too many tiles for one launch");
     const Mx8Call c{offsets, sel, nsel, tile_start, max_tiles, (const uint8_t *const *)slots, H, I,
                     reinterpret_cast<hipStream_t>(stream)};
     auto *xc = (const uint8_t *)x, *xs = (const uint8_t *)x_scales;
     auto *hc = (uint8_t *)h, *hs = (uint8_t *)h_scales, *out = (uint8_t *)y;
-    if (block_m == 32) return mx8_grouped_launch<32, 4, 4, 8, 2>(c, xc, xs, perm_token, hc, hs, out);
-    return mx8_grouped_launch<64, 4, 2, 4, 2>(c, xc, xs, perm_token, hc, hs, out);
+    if (block_m == 32) return mx8_grouped_launch<32, 4>(c, xc, xs, perm_token, hc, hs, out);
+    return mx8_grouped_launch<64, 2>(c, xc, xs, perm_token, hc, hs, out);
 }
