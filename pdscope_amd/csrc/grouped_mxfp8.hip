@@ -21,8 +21,8 @@
 // Wave tile: 64 rows of weights x BM rows of x.  Weights go from memory to registers,
 // where a wave is the only one that needs them, a step of 128 inputs ahead; x through two
 // LDS stages, which all waves read.  Few rows (BM = 32) are bound by the weights' bytes: 33
-// tokens of the Qwen shape (H 2048, I 768, 128 experts, 8 a token), gate/up 32 us and down 17,
-// 5.9 and 5.6 TB/s.  Many are bound by the time that a step's loads take under load, and by
+// tokens of the Qwen shape (H 2048, I 768, 128 experts, 8 a token), gate/up 32 us and down 18,
+// 5.9 and 5.2 TB/s.  Many are bound by the time that a step's loads take under load, and by
 // what a tile does before and after its K loop: 4096 tokens of the DeepSeek-V2-Lite shape (H 2048, I
 // 1408, 64 experts, 6 a token) gate/up 156 us and down 89, 1.8 and 1.6 PFLOP/s, the matrix
 // units busy 45% of the time; of a gate/up tile's 26 us 3.6 are spent before its loop (where it

@@ -823,6 +823,11 @@ class MxRows:
     scales: torch.Tensor  # uint8 [T, n / 32]
 
 
+def _rows_of(T, n, dtype, dev) -> torch.Tensor:
+    """torch.empty((T, n), dtype=dtype, device=dev), whose arguments take 0.4 us longer to read."""
+    return torch.empty_strided((T, n), (n, 1), dtype=dtype, device=dev)
+
+
 def _line(t, dtype, dev) -> bool:
     """Whether _need(t, ..., dtype, 1, dev) passes."""
     return isinstance(t, torch.Tensor) and t.dtype is dtype and t.ndim == 1 and t.device == dev and t.is_contiguous()
@@ -833,12 +838,12 @@ def _need_rows(rows, name, T, n, device):
     if not isinstance(rows, MxRows):
         raise ValueError(f"{name} must be MxRows")
     c, s = rows.codes, rows.scales
-    if (isinstance(c, torch.Tensor) and isinstance(s, torch.Tensor) and c.dtype is F8 and s.dtype is torch.uint8
-            and c.ndim == 2 and c.shape[1] % 32 == 0 and s.shape == (c.shape[0], c.shape[1] // 32)
-            and (T is None or c.shape[0] == T) and (n is None or c.shape[1] == n) and c.device.type == "cuda"
-            and s.device == c.device and (device is None or c.device == device) and c.is_contiguous()
-            and s.is_contiguous()):
-        return
+    if isinstance(c, torch.Tensor) and isinstance(s, torch.Tensor) and c.ndim == 2 and c.is_cuda:
+        shape, dev = c.shape, c.device
+        if (c.dtype is F8 and s.dtype is torch.uint8 and shape[1] % 32 == 0 and s.shape == (shape[0], shape[1] // 32)
+                and (T is None or shape[0] == T) and (n is None or shape[1] == n) and s.device == dev
+                and (device is None or dev == device) and c.is_contiguous() and s.is_contiguous()):
+            return
     _need(rows.codes, f"{name}.codes", F8, 2, device)
     _need(rows.scales, f"{name}.scales", torch.uint8, 2, rows.codes.device)
     shape = tuple(rows.codes.shape)
@@ -853,8 +858,7 @@ def mxfp8_empty(T, n, device) -> MxRows:
     """8-bit rows to be written: codes [T, n], scales [T, n / 32]."""
     if n % 32:
         raise ValueError(f"8-bit rows need a length of whole blocks of 32, got {n}")
-    return MxRows(torch.empty((T, n), dtype=F8, device=device),
-                  torch.empty((T, n // 32), dtype=torch.uint8, device=device))
+    return MxRows(_rows_of(T, n, F8, device), _rows_of(T, n // 32, torch.uint8, device))
 
 
 def mxfp8_quantize(x, out: MxRows | None = None) -> MxRows:
@@ -875,7 +879,7 @@ def mxfp8_dequantize(rows: MxRows, out=None) -> torch.Tensor:
     _need_rows(rows, "rows", None, None, None)
     T, n = rows.codes.shape
     if out is None:
-        out = torch.empty((T, n), dtype=BF16, device=rows.codes.device)
+        out = _rows_of(T, n, BF16, rows.codes.device)
     elif not _fits(out, BF16, (T, n), rows.codes.device):
         _refuse(out, "out", BF16, (T, n), rows.codes.device)
     if T:
@@ -1019,7 +1023,7 @@ def linear_int4(x, w: Int4Weight, bias=None, out=None) -> torch.Tensor:
     if bias is not None and not _fits(bias, BF16, (w.N,), dev):
         _refuse(bias, "bias", BF16, (w.N,), dev)
     if out is None:
-        out = torch.empty((T, w.N), dtype=BF16, device=dev)
+        out = _rows_of(T, w.N, BF16, dev)
     elif not _fits(out, BF16, (T, w.N), dev):
         _refuse(out, "out", BF16, (T, w.N), dev)
     if T:
