@@ -111,6 +111,21 @@ def test_every_row_tile_and_merge(block_m, T, used):
     assert torch.equal(out, again)
 
 
+def test_an_expert_picked_twice_by_a_token():
+    """Rows of one expert that come from the same row of x, and a batch padded with copies of a token."""
+    T, H, I, E, k = 70, 384, 256, 6, 3
+    rows, ids, w, blocks, slots = make(T, H, I, E, k, seed=8)
+    ids[::2, 1] = ids[::2, 0]
+    ids[5] = 4
+    rows.codes.view(torch.uint8)[40:] = rows.codes.view(torch.uint8)[39]
+    rows.scales[40:] = rows.scales[39]
+    ids[40:], w[40:] = ids[39], w[39]
+    ws = layer.MoEWorkspace(T, H, I, E, k, DEV)
+    out = layer.experts_resident(rows, ids, w, slots, ws, representation="mxfp4")
+    check(out, ws, rows, ids, w, blocks)
+    assert torch.equal(out[39:], out[39].expand(T - 39, H))
+
+
 def test_rows_counts_of_one_expert():
     """One expert with every count of rows around the tiles' edges."""
     H, I = 256, 128
