@@ -937,6 +937,7 @@ class Int4Weight:
     scale_dtype: torch.dtype = BF16
 
 
+@functools.lru_cache(maxsize=256)
 def int4_bytes(N: int, K: int, group: int, zeros: bool = False) -> int:
     """Bytes of a laid-out 4-bit matrix."""
     n = int(_lib.load().pdscope_int4_bytes(int(N), int(K), int(group), int(bool(zeros))))
@@ -991,7 +992,8 @@ def int4_quantize(weight, group=128, zeros=False, out=None) -> Int4Weight:
 def _need_int4(w, device=None):
     if not isinstance(w, Int4Weight):
         raise ValueError("weight must be an Int4Weight")
-    _need(w.units, "weight.units", torch.uint8, 1, device)
+    if device is None or not _line(w.units, torch.uint8, device):
+        _need(w.units, "weight.units", torch.uint8, 1, device)
     if w.units.numel() != int4_bytes(w.N, w.K, w.group, w.zeros):
         raise ValueError("weight.units is not of the size of its shape")
     if w.scale_dtype not in (BF16, torch.float16):
