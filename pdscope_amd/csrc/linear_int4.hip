@@ -273,9 +273,10 @@ constexpr int kI4GemmStage = kI4GemmX + 4 * 512;  // 128 bytes at most for each 
 // 0.92 PFLOP/s (G = 64 43, G = 32 56: more scalings), of which the loop 26, what is before and behind it
 // 4.3; without the loop's loads 33.6, without decoding 35.8, without reading x from LDS 30.4.  T = 4096 and
 // K = 4096 1.0 PFLOP/s.  Held back by neither alone; reading x 32 inputs ahead of the products or
-// another order of them changed nothing.
+// another order of them changed nothing.  RT = 2 without parts has 168 registers, for three workgroups a
+// CU (T = 1100 30.5 us against 34.5 with two).
 template <int G, bool ZEROS, bool FP16, int RT, int KS>
-__global__ __launch_bounds__(256 * KS, std::max(KS, 2)) void i4_gemm_kernel(I4Linear p, int cut) {
+__global__ __launch_bounds__(256 * KS, KS > 2 ? KS : KS == 1 && RT == 2 ? 3 : 2) void i4_gemm_kernel(I4Linear p, int cut) {
     constexpr int UB = i4_unit_bytes(G, ZEROS), GP = kI4In / G, JG = 4 / GP;
     constexpr int kN = 64 * RT, kOut = kN * 2 + 16;          // rows of W, bytes of a staged output row
     constexpr int kSums = KS > 2 ? 8 : 16;                   // groups whose sums of x are kept at a time
@@ -483,11 +484,11 @@ template <int G, bool ZEROS, bool FP16, int RT, int KS>
 static void i4_gemm_run(const I4Linear &a, hipStream_t s) {
     const int TB = (a.T + kI4GemmM - 1) / kI4GemmM, NB = (a.N + 64 * RT - 1) / (64 * RT);
     // the tokens in `cut` parts and the rows in 8 / cut: by the rounds of the XCD with most
-    // tiles (two workgroups a CU at a time, one where parts share the K axis), then by the bytes
+    // tiles (two workgroups a CU at a time, three of RT = 2, one where parts share the K axis), then by the bytes
     // of x and of W that one reads (T = 300, N = 2816, K = 2048 in two parts 12.4 us, by the bytes
     // alone 22.0)
     int cut = 1;
-    constexpr int per_xcd = KS == 1 ? 64 : 32;
+    constexpr int per_xcd = KS > 1 ? 32 : RT == 2 ? 96 : 64;
     auto rounds = [&](int c) { return ((int64_t)((TB + c - 1) / c) * ((NB * c + 7) / 8) + per_xcd - 1) / per_xcd; };
     auto read = [&](int c) { return 2.0 * a.T / c + 0.55 * a.N * c / 8; };
     for (int c : {2, 4, 8})
@@ -547,11 +548,14 @@ static void i4_linear_launch(const I4Linear &a, hipStream_t s) {
     // of its loads, and small ones that share the K axis have fewer steps: N = 4096,
     // K = 2048, tiles of 64 tokens x 64 rows in four parts / in two / x 128 in two / x 256: T = 256 11.1 / 12.0
     // / 15.6 / 24.7 us, T = 512 - / 22.4 / 15.7 / 24.6, T = 1024 - / 42 / 29 / 25.5, T = 2048 - / 83 / 57 /
-    // 37.3; K = 4096, N = 2048, T = 512 16.9 / 19.4 / 24.9 / 44.6.
+    // 37.3; K = 4096, N = 2048, T = 512 16.9 / 19.4 / 24.9 / 44.6.  Tiles of 128 rows without
+    // parts fill the card up to three a CU (against 256 rows, G = 128 / 32: T = 640 23.5 / 33.6 us and
+    // 24.8 / 38.2, T = 1300 32.3 / 45.0 and 36.0 / 55.0, T = 1600 42.7 / 58.4 and 35.9 / 55.7).
     if (std::min({one, two, four}) >= 7) {
         const int64_t down = (a.T + kI4GemmM - 1) / kI4GemmM;
         if (down * ((a.N + 63) / 64) <= 256) i4_gemm_run<G, ZEROS, FP16, 1, 4>(a, s);
         else if (down * ((a.N + 127) / 128) <= 256) i4_gemm_run<G, ZEROS, FP16, 2, 2>(a, s);
+        else if (down * ((a.N + 127) / 128) <= 768) i4_gemm_run<G, ZEROS, FP16, 2, 1>(a, s);
         else i4_gemm_run<G, ZEROS, FP16, 4, 1>(a, s);
     } else if (one <= two && one <= four) {
         i4_split_run<G, ZEROS, FP16, 1, 1, 8, true>(a, s);
