@@ -28,7 +28,7 @@ struct I4Linear {
     const uint16_t *x, *bias;
     uint16_t *y;
     int T, N, K;
-    bool wide;  // every 8 outputs of a row from its start on lie at a multiple of 16 bytes
+    int piece;  // outputs that one store takes: 8, 2 or 1, of whose size every row's start is a multiple
 };
 
 // What a wave holds of a unit: codes, and its rows' scales and zero points (rows 4 g .. +
@@ -75,7 +75,7 @@ struct I4Unit {
 __device__ __forceinline__ void i4_store(const I4Linear &p, int t, int n, f32x4_t v, const float (&bias)[4]) {
     const uint32_t lo = f2bf2_hw(v[0] + bias[0], v[1] + bias[1]), hi = f2bf2_hw(v[2] + bias[2], v[3] + bias[3]);
     uint16_t *y = p.y + (size_t)t * p.N + n;
-    if (n + 3 < p.N && p.wide) {
+    if (n + 3 < p.N && p.piece == 8) {
         *reinterpret_cast<uint2 *>(y) = make_uint2(lo, hi);
     } else {
         if (n < p.N) y[0] = (uint16_t)lo;
@@ -468,16 +468,22 @@ __global__ __launch_bounds__(256 * KS, KS > 2 ? KS : KS == 1 && RT == 2 ? 3 : 2)
     }
     __syncthreads();
     const int rows = min(kI4GemmM, p.T - t0), cols = min(kN, p.N - n0);
-    for (int c = tid; c < rows * (kN / 8); c += 256 * KS) {
-        const int row = c / (kN / 8), col = c % (kN / 8) * 8;
-        const uint8_t *from = smem_all + row * kOut + col * 2;
-        uint16_t *to = p.y + (size_t)(t0 + row) * p.N + n0 + col;
-        if (col + 8 <= cols && p.wide) {
-            st_through(to, *reinterpret_cast<const uint4 *>(from));
-        } else {
-            for (int i = 0; i < 8 && col + i < cols; ++i) to[i] = reinterpret_cast<const uint16_t *>(from)[i];
+    uint16_t *const y = p.y + (size_t)t0 * p.N + n0;
+    // neighbouring lanes beside one another, as wide as every row's start allows
+    auto put = [&](auto piece) {
+        using Piece = decltype(piece);
+        constexpr int PW = sizeof(Piece) / 2, PR = kN / PW;  // values of a piece, pieces of a row
+        for (int c = tid; c < rows * PR; c += 256 * KS) {
+            const int row = c / PR, col = c % PR * PW;
+            if (col >= cols) continue;
+            const Piece v = *reinterpret_cast<const Piece *>(smem_all + row * kOut + col * 2);
+            if constexpr (PW == 8) st_through(y + (size_t)row * p.N + col, v);
+            else *reinterpret_cast<Piece *>(y + (size_t)row * p.N + col) = v;
         }
-    }
+    };
+    if (p.piece == 8) put(uint4{});
+    else if (p.piece == 2) put(uint32_t{});
+    else put(uint16_t{});
 }
 
 template <int G, bool ZEROS, bool FP16, int RT, int KS>
@@ -549,13 +555,16 @@ static void i4_linear_launch(const I4Linear &a, hipStream_t s) {
     // K = 2048, tiles of 64 tokens x 64 rows in four parts / in two / x 128 in two / x 256: T = 256 11.1 / 12.0
     // / 15.6 / 24.7 us, T = 512 - / 22.4 / 15.7 / 24.6, T = 1024 - / 42 / 29 / 25.5, T = 2048 - / 83 / 57 /
     // 37.3; K = 4096, N = 2048, T = 512 16.9 / 19.4 / 24.9 / 44.6.  Tiles of 128 rows without
-    // parts fill the card up to three a CU (against 256 rows, G = 128 / 32: T = 640 23.5 / 33.6 us and
-    // 24.8 / 38.2, T = 1300 32.3 / 45.0 and 36.0 / 55.0, T = 1600 42.7 / 58.4 and 35.9 / 55.7).
+    // parts go by up to three a CU, those of 256 by two; a round of 256 of the former counts as 10, one
+    // of 256 of the latter as 24, of 512 as 34 (against 256 rows, G = 128 / 32: T = 640 23.5 / 33.6 us
+    // and 24.8 / 38.2, T = 1300 32.3 / 45.0 and 36.0 / 55.0, T = 1600 42.7 / 58.4 and 35.9 / 55.7, N = 4097,
+    // T = 2048 57.6 / 74.9 and 64.8 / 91.7).
     if (std::min({one, two, four}) >= 7) {
-        const int64_t down = (a.T + kI4GemmM - 1) / kI4GemmM;
+        const int64_t down = (a.T + kI4GemmM - 1) / kI4GemmM, narrow = down * ((a.N + 127) / 128);
+        const int64_t n2 = (narrow + 255) / 256, n4 = (down * ((a.N + 255) / 256) + 255) / 256;
         if (down * ((a.N + 63) / 64) <= 256) i4_gemm_run<G, ZEROS, FP16, 1, 4>(a, s);
-        else if (down * ((a.N + 127) / 128) <= 256) i4_gemm_run<G, ZEROS, FP16, 2, 2>(a, s);
-        else if (down * ((a.N + 127) / 128) <= 768) i4_gemm_run<G, ZEROS, FP16, 2, 1>(a, s);
+        else if (n2 == 1) i4_gemm_run<G, ZEROS, FP16, 2, 2>(a, s);
+        else if (10 * n2 < 34 * (n4 / 2) + 24 * (n4 % 2)) i4_gemm_run<G, ZEROS, FP16, 2, 1>(a, s);
         else i4_gemm_run<G, ZEROS, FP16, 4, 1>(a, s);
     } else if (one <= two && one <= four) {
         i4_split_run<G, ZEROS, FP16, 1, 1, 8, true>(a, s);
@@ -582,8 +591,9 @@ PD_API int pdscope_linear_int4(const void *x, const void *w, const void *bias, i
     // may add 8 tiles a row and a column of them
     if (((int64_t)N + 255) / 256 * (((int64_t)T + kI4GemmM - 1) / kI4GemmM) > (int64_t)1 << 23)
         return fail(kEInval, "linear_int4: too many outputs for one launch");
+    const uintptr_t at = reinterpret_cast<uintptr_t>(y);
     const I4Linear a{(const uint8_t *)w, (const uint16_t *)x, (const uint16_t *)bias, (uint16_t *)y, T, N, K,
-                     N % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0};
+                     N % 8 == 0 && at % 16 == 0 ? 8 : N % 2 == 0 && at % 4 == 0 ? 2 : 1};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     auto group = [&](auto g) {
         constexpr int GG = decltype(g)::value;

@@ -95,6 +95,7 @@ SIZES = [(1, 1, 32, 32), (1, 16, 128, 128), (2, 15, 64, 64), (1, 4096, 2048, 128
          (449, 4096, 128, 64), (700, 1500, 2048, 128), (24, 16384, 1408, 128),
          # tiles of 128 rows without parts: one step, an odd count of them, ragged edges
          (700, 4000, 128, 64), (1300, 4097, 352, 32), (650, 3900, 1408, 128), (1111, 2500, 2048, 32),
+         (2048, 4097, 160, 32), (2500, 4100, 256, 128), (1800, 2222, 192, 64), (1601, 4098, 128, 32),
          # many row tiles for one workgroup
          (1, 20000, 2048, 128), (3, 16401, 1152, 32), (16, 33000, 1984, 64), (2, 9000, 8192, 128), (4, 5000, 4096, 128),
          (1, 70000, 2048, 128), (9, 66001, 2016, 32), (16, 80000, 1984, 64), (2, 5000, 352, 32), (13, 8193, 1088, 64), (16, 4113, 96, 32)]
