@@ -29,9 +29,9 @@
 // finds its expert and its rows) and 3.0 behind it, three tiles a CU at a time.  Without
 // the loop's loads the layer's products take 95 us for 153, with weights from the L2 128.  Tried and
 // not kept, all within 5% or slower: 128 rows a tile, two waves on the same weights through
-// LDS with two to four stages (154 to 190 and 84 to 101 us), eight waves a tile, weights two
-// steps ahead in registers, four workgroups a CU (194 and 118 us, spilled), a list of experts
-// read beside their tiles before the loop.
+// LDS with two to four stages (154 to 190 and 84 to 101 us), each wave's own weights two steps ahead
+// through LDS (155 and 87) or in registers, eight waves a tile, four workgroups a CU (194 and 118 us,
+// spilled), a list of experts read beside their tiles before the loop.
 #include <algorithm>
 #include <type_traits>
 
