@@ -1,0 +1,26 @@
+"""Linear modules on 4-bit weights in the place of a model's own: what is refused before a
+module is replaced, and the inputs that a plain linear module takes."""
+import pytest
+import torch
+
+from pdscope_amd import ops
+from pdscope_amd.hf import Int4Linear, install_int4_linears
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16 = torch.bfloat16
+
+
+def linear(k, n, bias=False, seed=1):
+    torch.manual_seed(seed)
+    return torch.nn.Linear(k, n, bias=bias).to(BF16).to(DEV)
+
+
+def test_a_bias_of_another_type_or_device_is_refused_before_anything_is_replaced():
+    for change in (lambda b: b.float(), lambda b: b.cpu(), lambda b: b.half()):
+        model = torch.nn.Sequential(linear(128, 64, True), linear(64, 32, True))
+        model[1].bias = torch.nn.Parameter(change(model[1].bias.detach()))
+        before = list(model)
+        with pytest.raises(ValueError, match="bias"):
+            install_int4_linears(model, 64)
+        assert all(a is b for a, b in zip(model, before))
