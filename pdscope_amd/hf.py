@@ -24,6 +24,7 @@ that a decoded token reads of them in bf16 (the reference keeps them as they are
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
 from .cache import ExpertKey
@@ -66,7 +67,7 @@ def install_expert_blocks(model, forward_layer, *, return_router_logits=None):
 class Int4Linear(torch.nn.Module):
     """A linear module over a 4-bit matrix (ops.Int4Weight): bf16 inputs [..., K] on the
     matrix' device to bf16 outputs [..., N].  Inference only: ops.linear_int4 has no
-    gradient."""
+    gradient, of reverse or forward mode."""
 
     def __init__(self, weight: ops.Int4Weight, bias=None):
         super().__init__()
@@ -86,7 +87,7 @@ class Int4Linear(torch.nn.Module):
         return ops.Int4Weight(self.units, *self._shape)
 
     def forward(self, x):
-        if torch.is_grad_enabled() and x.requires_grad:
+        if torch.is_grad_enabled() and x.requires_grad or forward_ad.unpack_dual(x).tangent is not None:
             raise RuntimeError("Int4Linear has no gradient: run it under torch.no_grad() or inference_mode()")
         out = ops.linear_int4(x.reshape(-1, x.shape[-1]).contiguous(), self.weight4, bias=self.bias)
         return out.view(*x.shape[:-1], self.out_features)

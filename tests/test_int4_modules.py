@@ -1,0 +1,23 @@
+"""CPU checks of the linear modules on 4-bit weights: refusals that come before a launch."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from pdscope_amd import ops
+from pdscope_amd.hf import Int4Linear
+
+
+def module(N=16, K=128, G=64):
+    return Int4Linear(ops.Int4Weight(torch.zeros(ops.int4_bytes(N, K, G), dtype=torch.uint8), N, K, G, False))
+
+
+def test_no_gradient_of_either_mode():
+    q, x = module(), torch.zeros((2, 128), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        q(x.clone().requires_grad_())
+    for grad in (True, False):  # no_grad() does not leave tangents out
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="no gradient"):
+                q(forward_ad.make_dual(x, torch.ones_like(x)))
+            with pytest.raises(ValueError, match="on the GPU"):  # as without a level: its own refusal
+                q(x)
