@@ -89,7 +89,10 @@ class Int4Linear(torch.nn.Module):
     def forward(self, x):
         if torch.is_grad_enabled() and x.requires_grad or forward_ad.unpack_dual(x).tangent is not None:
             raise RuntimeError("Int4Linear has no gradient: run it under torch.no_grad() or inference_mode()")
-        out = ops.linear_int4(x.reshape(-1, x.shape[-1]).contiguous(), self.weight4, bias=self.bias)
+        rows = x.reshape(-1, x.shape[-1]).contiguous()
+        if rows.data_ptr() % 16:  # the kernels read 16 bytes at a time
+            rows = rows.clone()
+        out = ops.linear_int4(rows, self.weight4, bias=self.bias)
         return out.view(*x.shape[:-1], self.out_features)
 
     def extra_repr(self):

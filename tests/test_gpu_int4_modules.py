@@ -24,3 +24,17 @@ def test_a_bias_of_another_type_or_device_is_refused_before_anything_is_replaced
         with pytest.raises(ValueError, match="bias"):
             install_int4_linears(model, 64)
         assert all(a is b for a, b in zip(model, before))
+
+
+def test_contiguous_inputs_at_addresses_that_16_bytes_do_not_divide():
+    q = Int4Linear.of(linear(128, 48, True), 64)
+    for shape in ((3, 128), (2, 40, 128)):
+        n = torch.Size(shape).numel()
+        x = torch.randn(n, device=DEV).to(BF16)
+        want = q(x.view(shape))
+        for off in (1, 2, 4):
+            room = torch.empty(n + off, dtype=BF16, device=DEV)
+            room[off:] = x
+            at = room[off:].view(shape)
+            assert at.is_contiguous() and at.data_ptr() % 16
+            assert torch.equal(q(at), want)
