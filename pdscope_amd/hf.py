@@ -66,8 +66,9 @@ def install_expert_blocks(model, forward_layer, *, return_router_logits=None):
 
 class Int4Linear(torch.nn.Module):
     """A linear module over a 4-bit matrix (ops.Int4Weight): bf16 inputs [..., K] on the
-    matrix' device to bf16 outputs [..., N].  Inference only: ops.linear_int4 has no
-    gradient, of reverse or forward mode."""
+    matrix' device (under autocast to bf16 fp32 and fp16 ones too) to bf16 outputs
+    [..., N].  Inference only: ops.linear_int4 has no gradient, of reverse or forward
+    mode."""
 
     def __init__(self, weight: ops.Int4Weight, bias=None):
         super().__init__()
@@ -89,6 +90,10 @@ class Int4Linear(torch.nn.Module):
     def forward(self, x):
         if torch.is_grad_enabled() and x.requires_grad or forward_ad.unpack_dual(x).tangent is not None:
             raise RuntimeError("Int4Linear has no gradient: run it under torch.no_grad() or inference_mode()")
+        # under autocast to bf16 the inputs that it casts for a plain linear module
+        if x.dtype in (torch.float32, torch.float16) and x.is_cuda and torch.is_autocast_enabled("cuda") \
+                and torch.get_autocast_dtype("cuda") is torch.bfloat16:
+            x = x.to(torch.bfloat16)
         rows = x.reshape(-1, x.shape[-1]).contiguous()
         if rows.data_ptr() % 16:  # the kernels read 16 bytes at a time
             rows = rows.clone()

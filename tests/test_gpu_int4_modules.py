@@ -38,3 +38,27 @@ def test_contiguous_inputs_at_addresses_that_16_bytes_do_not_divide():
             at = room[off:].view(shape)
             assert at.is_contiguous() and at.data_ptr() % 16
             assert torch.equal(q(at), want)
+
+
+def test_autocast():
+    """Where autocast makes bf16 of a linear module's inputs, so it does of this one's; elsewhere
+    inputs of other types are refused as they are without it."""
+    q = Int4Linear.of(linear(128, 48, True), 64)
+    x = torch.randn((5, 128), device=DEV)
+    want = q(x.to(BF16))
+    with torch.autocast("cuda", dtype=BF16):
+        for t in (x, x.to(BF16), x.to(BF16).float()):
+            y = q(t)
+            assert y.dtype is BF16 and torch.equal(y, want)
+        y = q(x.half())
+        assert y.dtype is BF16 and torch.equal(y, q(x.half().to(BF16)))
+        with pytest.raises(ValueError, match="bfloat16"):
+            q(x.double())  # a plain module leaves 64 bits as they are too, and refuses the mixture
+        with torch.autocast("cuda", enabled=False), pytest.raises(ValueError, match="bfloat16"):
+            q(x)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            q(x.clone().requires_grad_())
+    with torch.autocast("cuda", dtype=torch.float16), pytest.raises(ValueError, match="bfloat16"):
+        q(x)
+    with pytest.raises(ValueError, match="bfloat16"):
+        q(x)
