@@ -107,11 +107,16 @@ class Int4Linear(torch.nn.Module):
 def install_int4_linears(model, group=128, zeros=False, keep=()):
     """Replace every torch.nn.Linear of a model that is on the GPU, but for routers and
     experts (modules below a `mlp` with a `gate`) and the names in `keep`, by its
-    4-bit form; returns the replaced modules' names.  Their bf16 weights are freed
+    4-bit form; returns the replaced modules' names.  A module that the model has under
+    several names gets one 4-bit form for all of them, or stays under all where one is
+    an expert block's or in `keep`.  Their bf16 weights are freed
     where nothing else holds them (a tied embedding does)."""
-    inside = [n + "." for n, m in model.named_modules() if hasattr(m, "gate") and n.rsplit(".", 1)[-1] == "mlp"]
-    found = [(n, m) for n, m in model.named_modules()
-             if type(m) is torch.nn.Linear and n not in keep and not any(n.startswith(p) for p in inside)]
+    named = list(model.named_modules(remove_duplicate=False))
+    kept = {id(m) for n, m in named if n in keep}
+    for n, m in named:
+        if hasattr(m, "gate") and n.rsplit(".", 1)[-1] == "mlp":
+            kept.update(id(part) for part in m.modules())
+    found = [(n, m) for n, m in named if type(m) is torch.nn.Linear and id(m) not in kept]
     for name, m in found:  # before anything is replaced
         if m.weight.dtype != torch.bfloat16 or m.weight.device.type != "cuda":
             raise ValueError(f"{name} must be bf16 on the GPU, got {m.weight.dtype} on {m.weight.device}")
@@ -119,9 +124,12 @@ def install_int4_linears(model, group=128, zeros=False, keep=()):
             raise ValueError(f"{name}'s bias must be as its weight, bf16 on {m.weight.device}, got {m.bias.dtype} on {m.bias.device}")
         if m.in_features % group:
             raise ValueError(f"{name} has {m.in_features} inputs, not whole groups of {group}: keep it or take smaller groups")
+    forms = {}
     for name, m in found:
+        if id(m) not in forms:
+            forms[id(m)] = Int4Linear.of(m, group, zeros)
         parent, _, leaf = name.rpartition(".")
-        setattr(model.get_submodule(parent) if parent else model, leaf, Int4Linear.of(m, group, zeros))
+        setattr(model.get_submodule(parent) if parent else model, leaf, forms[id(m)])
     return [n for n, _ in found]
 
 

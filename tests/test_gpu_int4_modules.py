@@ -62,3 +62,26 @@ def test_autocast():
         q(x)
     with pytest.raises(ValueError, match="bfloat16"):
         q(x)
+
+
+class Shared(torch.nn.Module):
+    def __init__(self, shared):
+        super().__init__()
+        self.first, self.inner = shared, torch.nn.Sequential(linear(64, 64, seed=2), shared)
+        self.mlp = torch.nn.Module()
+        self.mlp.gate, self.mlp.up = linear(64, 32, seed=3), linear(64, 32, seed=4)
+        self.up_again = self.mlp.up
+
+
+def test_a_module_under_two_names():
+    """Both names get the one 4-bit form; a module that one name keeps, or that an expert block has
+    too, stays under all of its names."""
+    model = Shared(linear(64, 64))
+    up, gate = model.mlp.up, model.mlp.gate
+    assert sorted(install_int4_linears(model, 64)) == ["first", "inner.0", "inner.1"]
+    assert type(model.first) is Int4Linear and model.first is model.inner[1] and model.inner[0] is not model.first
+    assert model.mlp.up is up and model.up_again is up and model.mlp.gate is gate
+    model = Shared(linear(64, 64))
+    first = model.first
+    assert install_int4_linears(model, 64, keep=("inner.1",)) == ["inner.0"]
+    assert model.first is first and model.inner[1] is first
