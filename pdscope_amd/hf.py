@@ -111,6 +111,8 @@ def install_int4_linears(model, group=128, zeros=False, keep=()):
     several names gets one 4-bit form for all of them, or stays under all where one is
     an expert block's or in `keep`.  Their bf16 weights are freed
     where nothing else holds them (a tied embedding does)."""
+    if type(model) is torch.nn.Linear:
+        raise ValueError("the model is a linear module itself, which no parent holds: take Int4Linear.of")
     named = list(model.named_modules(remove_duplicate=False))
     kept = {id(m) for n, m in named if n in keep}
     for n, m in named:

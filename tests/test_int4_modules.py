@@ -4,7 +4,7 @@ import torch
 from torch.autograd import forward_ad
 
 from pdscope_amd import ops
-from pdscope_amd.hf import Int4Linear
+from pdscope_amd.hf import Int4Linear, install_int4_linears
 
 
 def module(N=16, K=128, G=64):
@@ -21,3 +21,9 @@ def test_no_gradient_of_either_mode():
                 q(forward_ad.make_dual(x, torch.ones_like(x)))
             with pytest.raises(ValueError, match="on the GPU"):  # as without a level: its own refusal
                 q(x)
+
+
+def test_a_model_that_is_a_linear_module_itself_is_refused():
+    """No parent holds it, so nothing could be replaced."""
+    with pytest.raises(ValueError, match="itself"):
+        install_int4_linears(torch.nn.Linear(128, 48), 64)
