@@ -111,6 +111,8 @@ def install_int4_linears(model, group=128, zeros=False, keep=()):
     several names gets one 4-bit form for all of them, or stays under all where one is
     an expert block's or in `keep`.  Their bf16 weights are freed
     where nothing else holds them (a tied embedding does)."""
+    if group not in (32, 64, 128):
+        raise ValueError(f"group must be 32, 64 or 128, got {group}")
     if type(model) is torch.nn.Linear:
         raise ValueError("the model is a linear module itself, which no parent holds: take Int4Linear.of")
     named = list(model.named_modules(remove_duplicate=False))

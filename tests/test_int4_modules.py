@@ -27,3 +27,11 @@ def test_a_model_that_is_a_linear_module_itself_is_refused():
     """No parent holds it, so nothing could be replaced."""
     with pytest.raises(ValueError, match="itself"):
         install_int4_linears(torch.nn.Linear(128, 48), 64)
+
+
+@pytest.mark.parametrize("group", [0, -64, 16, 48, 256])
+def test_groups_that_a_matrix_cannot_have(group):
+    """Before any module is looked at: a model without linear modules has its answer too."""
+    for model in (torch.nn.Sequential(torch.nn.Linear(768, 48)), torch.nn.Sequential()):
+        with pytest.raises(ValueError, match="32, 64 or 128"):
+            install_int4_linears(model, group)
