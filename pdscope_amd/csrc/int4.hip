@@ -93,7 +93,8 @@ __global__ __launch_bounds__(256) void i4_quantize_kernel(const uint16_t *__rest
             }
         top = max_quarters(top);
         bottom = max_quarters(bottom);
-        const uint32_t s16 = f2bf(ZEROS ? (top + bottom) / 15.0f : top / 7.0f);
+        // halves, which bf16 values have exactly: the span itself may be past fp32's largest number
+        const uint32_t s16 = f2bf(ZEROS ? (0.5f * top + 0.5f * bottom) / 7.5f : top / 7.0f);
         const float sc = bf2f(s16);
         const float z = !ZEROS ? 8.0f : sc > 0.0f ? fminf(rintf(bottom / sc), 15.0f) : 0.0f;
 #pragma unroll
