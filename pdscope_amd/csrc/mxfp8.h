@@ -58,9 +58,14 @@ __device__ __forceinline__ uint2 mx8_encode8(const float (&v)[8], uint32_t byte)
 
 // A 64-bit value cut to 32 bits, with the last bit set where anything was cut
 // off: rounding it further to a type of fewer bits gives what rounding the
-// value itself would.
+// value itself would.  Below fp32's normal numbers the last bit is a step of 2^-149.
 __device__ __forceinline__ float round_to_odd(double v) {
     const uint64_t u = (uint64_t)__double_as_longlong(v);
+    if (fabs(v) < 0x1p-126) {
+        const double steps = fabs(v) * 0x1p149;
+        const uint32_t whole = (uint32_t)steps;
+        return __uint_as_float(whole | (uint32_t)((double)whole != steps) | (uint32_t)(u >> 32 & 0x80000000u));
+    }
     const uint64_t cut = u & 0x1fffffffull;
     return (float)__longlong_as_double((long long)((u - cut) | (cut ? 0x20000000ull : 0ull)));
 }
