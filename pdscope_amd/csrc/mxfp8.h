@@ -56,18 +56,33 @@ __device__ __forceinline__ uint2 mx8_encode8(const float (&v)[8], uint32_t byte)
     return make_uint2((uint32_t)lo, (uint32_t)hi);
 }
 
-// A 64-bit value cut to 32 bits, with the last bit set where anything was cut
-// off: rounding it further to a type of fewer bits gives what rounding the
-// value itself would.  Below fp32's normal numbers the last bit is a step of 2^-149.
-__device__ __forceinline__ float round_to_odd(double v) {
-    const uint64_t u = (uint64_t)__double_as_longlong(v);
-    if (fabs(v) < 0x1p-126) {
-        const double steps = fabs(v) * 0x1p149;
-        const uint32_t whole = (uint32_t)steps;
-        return __uint_as_float(whole | (uint32_t)((double)whole != steps) | (uint32_t)(u >> 32 & 0x80000000u));
+// Eight 64-bit values cut to 32 bits, with the last bit set where anything was cut
+// off: rounding them further to a type of fewer bits gives what rounding the
+// values themselves would.  Below fp32's normal numbers the last bit is a step of
+// 2^-149; one branch for all eight (4096 rows of 2048 with the merge and the way back
+// 45.6 us, 47.9 with a choice for each value).
+__device__ __forceinline__ void round_to_odd8(const double (&v)[8], float (&o)[8]) {
+    uint64_t u[8];
+    uint32_t least = ~0u;  // the upper halves without their signs, whose order is that of the magnitudes
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        u[i] = (uint64_t)__double_as_longlong(v[i]);
+        least = min(least, (uint32_t)(u[i] >> 32) & 0x7fffffffu);
     }
-    const uint64_t cut = u & 0x1fffffffull;
-    return (float)__longlong_as_double((long long)((u - cut) | (cut ? 0x20000000ull : 0ull)));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint64_t cut = u[i] & 0x1fffffffull;
+        o[i] = (float)__longlong_as_double((long long)((u[i] - cut) | (cut ? 0x20000000ull : 0ull)));
+    }
+    if (least < 0x38100000u) {  // of 2^-126
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const double steps = fabs(v[i]) * 0x1p149;
+            const uint32_t whole = (uint32_t)steps;
+            const uint32_t odd = whole | (uint32_t)((double)whole != steps) | (uint32_t)(u[i] >> 32 & 0x80000000u);
+            if (fabs(v[i]) < 0x1p-126) o[i] = __uint_as_float(odd);
+        }
+    }
 }
 
 }  // namespace pd

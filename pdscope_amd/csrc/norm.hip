@@ -127,10 +127,13 @@ __device__ __forceinline__ F block_sum(F v, F *s_sum) {
 __device__ __forceinline__ float inv_rms(float sum, int H, float eps) { return 1.0f / sqrtf(sum / (float)H + eps); }
 __device__ __forceinline__ double inv_rms(double sum, int H, float eps) { return 1.0 / sqrt(sum / (double)H + (double)eps); }
 
-// What is stored of a value: itself, or the 32-bit value that keeps for any
-// shorter type on which side of its borders a 64-bit one lies.
-__device__ __forceinline__ float narrow(float v) { return v; }
-__device__ __forceinline__ float narrow(double v) { return round_to_odd(v); }
+// What is stored of eight values: themselves, or the 32-bit values that keep for any
+// shorter type on which side of its borders 64-bit ones lie.
+__device__ __forceinline__ void narrow8(const float (&v)[8], float (&o)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = v[i];
+}
+__device__ __forceinline__ void narrow8(const double (&v)[8], float (&o)[8]) { round_to_odd8(v, o); }
 
 // NV: eights of a row per thread; MX: 8-bit rows as well.
 template <bool VEC, bool R32, bool P32, int NV, bool MX>
@@ -211,8 +214,12 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
         }
         if (a.out_resid) {
             float r[8];
+            if constexpr (R32) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[i] = R32 ? (float)v[j][i] : narrow(v[j][i]);
+                for (int i = 0; i < 8; ++i) r[i] = (float)v[j][i];
+            } else {
+                narrow8(v[j], r);
+            }
             store8<VEC, R32>((char *)a.out_resid + (size_t)t * H * (R32 ? 4 : 2), at[j], H, r);
         }
     }
@@ -231,8 +238,7 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
             for (int i = 0; i < 8; ++i) v[j][i] *= rs;
         }
         float o[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = narrow(v[j][i]);
+        narrow8(v[j], o);
         if (!MX || a.out_norm) store8<VEC, false>(a.out_norm + (size_t)t * H, at[j], H, o);
         if constexpr (MX) {
             const uint32_t byte = mx8_scale_byte(max_over_quad(top_magnitude8(o)));
