@@ -550,6 +550,9 @@ int pdscope_swiglu_grouped_mxfp8(const void *x, const void *x_scales, const int3
  * Limits: 1 <= N <= 2^24, K % G == 0, K <= 2^20, fewer than 2^37 - 2^13 weights in whole
  * 16 x 128 units; 1 <= T <= 2^24, (N/256) * (T/64), each rounded up, at most 2^23; x, w,
  * codes and weight 16-byte aligned.
+ * pdscope_linear_int4_launch: the launch that these sizes take: 1 up to 16 rows with x in
+ * registers, 2 few rows with the K axis split over waves, 3 to 6 tiles of 64 rows of x and
+ * 64 (four parts of the K axis), 128 (two), 128 or 256 rows of W; 0 outside the limits of T, N, K and G.
  */
 size_t pdscope_int4_bytes(int N, int K, int G, int zeros);
 int pdscope_int4_pack(const void *codes, const void *scales, const void *zeros, int N, int K, int G, void *out,
@@ -559,6 +562,7 @@ int pdscope_int4_dequantize(const void *w, int N, int K, int G, int zeros, int f
                             void *stream);
 int pdscope_linear_int4(const void *x, const void *w, const void *bias, int T, int N, int K, int G, int zeros,
                         int fp16_scales, void *y, void *stream);
+int pdscope_linear_int4_launch(int T, int N, int K, int G);
 
 /*
  * A7 demand staging: replaces the three per-projection non_blocking copies

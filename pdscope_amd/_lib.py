@@ -88,6 +88,7 @@ SIGNATURES = {
     "pdscope_int4_quantize": ([_vp, _i32, _i32, _i32, _i32, _vp, _vp], _i32),
     "pdscope_int4_dequantize": ([_vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp], _i32),
     "pdscope_linear_int4": ([_vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp], _i32),
+    "pdscope_linear_int4_launch": ([_i32, _i32, _i32, _i32], _i32),
     "pdscope_stage_expert": ([_vp, _vp, _sz, _vp, _vp], _i32),
     "pdscope_stage_merge": ([_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp], _i32),
     "pdscope_dispatch_pack": ([_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp], _i32),

@@ -509,6 +509,14 @@ static void i4_split_run(const I4Linear &a, hipStream_t s) {
     i4_split_kernel<G, ZEROS, FP16, RT, MT, WV, KEEP><<<(unsigned)(across * down), 64 * WV, 0, s>>>(a);
 }
 
+// The launches, by what pdscope_linear_int4_launch calls them.
+enum I4Launch { kI4Rows16 = 1, kI4Split = 2, kI4Tiles64 = 3, kI4Tiles128Halves = 4, kI4Tiles128 = 5, kI4Tiles256 = 6 };
+
+struct I4Plan {
+    I4Launch launch;
+    int tiles = 0, tokens = 0, waves = 0;  // kI4Split: row tiles of W, tiles of 16 tokens and waves of a workgroup
+};
+
 // A launch by token tiles of a workgroup, in the time of one that has a single one, over
 // two: workgroups come 256 at a time, and one of MT tiles takes about as long as
 // MT + 1.  N = 1024, K = 2048: T = 64 4.6 / 7.1 / 10.6 us for MT = 1 / 2 / 4; N = 4096, K = 2048:
@@ -518,36 +526,31 @@ static int64_t i4_split_cost(int T, int tiles, int MT) {
     return ((int64_t)tiles * ((T + 16 * MT - 1) / (16 * MT)) + 255) / 256 * (MT + 1);
 }
 
-template <int G, bool ZEROS, bool FP16>
-static void i4_linear_launch(const I4Linear &a, hipStream_t s) {
-    const int KU = (a.K + kI4In - 1) / kI4In, tiles = (a.N + kI4Rows - 1) / kI4Rows;
-    if (a.T <= 16) {
-        // x in registers where a wave has very many tiles to read with it (K = 2048, G = 128: N =
-        // 98304 21.3 us against 20.8 with four row tiles a workgroup, T = 16 25.0 and 27.5; N = 151936
-        // 29.6 and 30.7, T = 16 35.0 and 40.7; K = 1536 26.7 and 25.4).  G = 32 has registers for one
+static I4Plan i4_plan(int T, int N, int K, int G) {
+    const int KU = (K + kI4In - 1) / kI4In, tiles = (N + kI4Rows - 1) / kI4Rows;
+    if (T <= 16) {
+        // x in registers where a wave has very many tiles to read with it, and either many rows of x,
+        // whose bytes count, or two whole units of it a wave.  us there / in the launch below: N =
+        // 151936, K = 2048, G = 128 T = 1 28.4 / 29.0, T = 8 30.7 / 31.9, T = 16 33.5 / 39.7; G = 64 with zero
+        // points 33.5 / 34.9, 36.0 / 37.9, 39.0 / 44.2; G = 32 48.5 / 48.4, 49.2 / 52.2, 50.1 / 57.5; K = 1664,
+        // G = 64 32.8 / 30.8, 35.0 / 32.9, 37.2 / 39.1; N = 98304, K = 2048, G = 128 20.3 / 20.0, 21.8 / 20.9,
+        // 24.0 / 26.4; N = 80000, K = 1664, G = 64 T = 14 22.4 / 21.1.  G = 32 has registers for one
         // workgroup per CU.
-        if (KU > 12 && KU <= kI4RowsWaves * kI4RowsUnits && (int64_t)tiles * KU > 65536) {
-            const int blocks = std::min(tiles, G == 32 ? 256 : 512);
-            i4_rows_kernel<G, ZEROS, FP16><<<(unsigned)blocks, 64 * kI4RowsWaves, 0, s>>>(a);
-        } else if (G > 32 && tiles > 512) {
-            // As many row tiles a workgroup, up to four, as leave one per CU: x is read once for all
-            // of them, and each has more loads on its way.  G = 128, K = 4096, one / two / four: N = 4096
-            // 5.6 / 6.6 / 8.8 us, N = 8192 8.3 / 7.7 / 9.6, N = 16384 12.7 / 11.1 / 10.1, N = 151936 90 / 70 / 64;
-            // T = 16 7.2 / 7.8 / 9.6, 12.4 / 8.6 / 10.5, 20.2 / 14.1 / 11.3, 162 / 103 / 82.  G = 32: N =
-            // 40000 31.4 / 27.9 / 33.5, T = 16 48.6 / 33.3 / 35.3.
-            i4_split_run<G, ZEROS, FP16, 4, 1, 8, false>(a, s);
-        } else if (tiles > 256) {
-            i4_split_run<G, ZEROS, FP16, 2, 1, 8, false>(a, s);
-        } else if (a.T <= 4 && KU > 16) {
-            // 16 waves where there are few workgroups and little of x (K = 2816, N = 2048, T = 1 4.5 us
-            // against 4.7 with eight, K = 8192, N = 4096 8.3 against 9.2; T = 16 5.9 against 5.7)
-            i4_split_run<G, ZEROS, FP16, 1, 1, 16, false>(a, s);
-        } else {
-            i4_split_run<G, ZEROS, FP16, 1, 1, 8, false>(a, s);
-        }
-        return;
+        const int64_t units = (int64_t)tiles * KU;
+        const int full = kI4RowsWaves * kI4RowsUnits;
+        if (KU > 12 && KU <= full && (T > 12 ? units > 98304 : KU == full && units > 131072)) return {kI4Rows16};
+        // As many row tiles a workgroup, up to four, as leave one per CU: x is read once for all
+        // of them, and each has more loads on its way.  G = 128, K = 4096, one / two / four: N = 4096
+        // 5.6 / 6.6 / 8.8 us, N = 8192 8.3 / 7.7 / 9.6, N = 16384 12.7 / 11.1 / 10.1, N = 151936 90 / 70 / 64;
+        // T = 16 7.2 / 7.8 / 9.6, 12.4 / 8.6 / 10.5, 20.2 / 14.1 / 11.3, 162 / 103 / 82.  G = 32: N =
+        // 40000 31.4 / 27.9 / 33.5, T = 16 48.6 / 33.3 / 35.3.
+        if (G > 32 && tiles > 512) return {kI4Split, 4, 1, 8};
+        if (tiles > 256) return {kI4Split, 2, 1, 8};
+        // 16 waves where there are few workgroups and little of x (K = 2816, N = 2048, T = 1 4.5 us
+        // against 4.7 with eight, K = 8192, N = 4096 8.3 against 9.2; T = 16 5.9 against 5.7)
+        return {kI4Split, 1, 1, T <= 4 && KU > 16 ? 16 : 8};
     }
-    const int64_t one = i4_split_cost(a.T, tiles, 1), two = i4_split_cost(a.T, tiles, 2), four = i4_split_cost(a.T, tiles, 4);
+    const int64_t one = i4_split_cost(T, tiles, 1), two = i4_split_cost(T, tiles, 2), four = i4_split_cost(T, tiles, 4);
     // The tiled launch takes the time of about seven such units (K = 2048: N = 4096, T = 64 10.9
     // us against 10.3 split, T = 128 11.0 and 17.8; N = 16384, T = 24 11.1 and 15.7; K = 4096: N =
     // 2048, T = 128 16.6 and 17.3, T = 192 16.8 and 26.6).  With few tiles a step's time is that
@@ -560,19 +563,39 @@ static void i4_linear_launch(const I4Linear &a, hipStream_t s) {
     // and 24.8 / 38.2, T = 1300 32.3 / 45.0 and 36.0 / 55.0, T = 1600 42.7 / 58.4 and 35.9 / 55.7, N = 4097,
     // T = 2048 57.6 / 74.9 and 64.8 / 91.7).
     if (std::min({one, two, four}) >= 7) {
-        const int64_t down = (a.T + kI4GemmM - 1) / kI4GemmM, narrow = down * ((a.N + 127) / 128);
-        const int64_t n2 = (narrow + 255) / 256, n4 = (down * ((a.N + 255) / 256) + 255) / 256;
-        if (down * ((a.N + 63) / 64) <= 256) i4_gemm_run<G, ZEROS, FP16, 1, 4>(a, s);
-        else if (n2 == 1) i4_gemm_run<G, ZEROS, FP16, 2, 2>(a, s);
-        else if (10 * n2 < 34 * (n4 / 2) + 24 * (n4 % 2)) i4_gemm_run<G, ZEROS, FP16, 2, 1>(a, s);
-        else i4_gemm_run<G, ZEROS, FP16, 4, 1>(a, s);
-    } else if (one <= two && one <= four) {
-        i4_split_run<G, ZEROS, FP16, 1, 1, 8, true>(a, s);
-    } else if (two <= four) {
-        i4_split_run<G, ZEROS, FP16, 1, 2, 8, true>(a, s);
-    } else {
-        i4_split_run<G, ZEROS, FP16, 1, 4, 8, true>(a, s);
+        const int64_t down = (T + kI4GemmM - 1) / kI4GemmM, narrow = down * ((N + 127) / 128);
+        const int64_t n2 = (narrow + 255) / 256, n4 = (down * ((N + 255) / 256) + 255) / 256;
+        if (down * ((N + 63) / 64) <= 256) return {kI4Tiles64};
+        if (n2 == 1) return {kI4Tiles128Halves};
+        if (10 * n2 < 34 * (n4 / 2) + 24 * (n4 % 2)) return {kI4Tiles128};
+        return {kI4Tiles256};
     }
+    return {kI4Split, 1, one <= two && one <= four ? 1 : two <= four ? 2 : 4, 8};
+}
+
+template <int G, bool ZEROS, bool FP16>
+static void i4_linear_launch(const I4Linear &a, hipStream_t s) {
+    const I4Plan p = i4_plan(a.T, a.N, a.K, G);
+    switch (p.launch) {
+        case kI4Rows16: {
+            const int blocks = std::min((a.N + kI4Rows - 1) / kI4Rows, G == 32 ? 256 : 512);
+            i4_rows_kernel<G, ZEROS, FP16><<<(unsigned)blocks, 64 * kI4RowsWaves, 0, s>>>(a);
+            return;
+        }
+        case kI4Tiles64: return i4_gemm_run<G, ZEROS, FP16, 1, 4>(a, s);
+        case kI4Tiles128Halves: return i4_gemm_run<G, ZEROS, FP16, 2, 2>(a, s);
+        case kI4Tiles128: return i4_gemm_run<G, ZEROS, FP16, 2, 1>(a, s);
+        case kI4Tiles256: return i4_gemm_run<G, ZEROS, FP16, 4, 1>(a, s);
+        case kI4Split: break;
+    }
+    if constexpr (G > 32)
+        if (p.tiles == 4) return i4_split_run<G, ZEROS, FP16, 4, 1, 8, false>(a, s);
+    if (p.tiles == 2) return i4_split_run<G, ZEROS, FP16, 2, 1, 8, false>(a, s);
+    if (p.tokens == 4) return i4_split_run<G, ZEROS, FP16, 1, 4, 8, true>(a, s);
+    if (p.tokens == 2) return i4_split_run<G, ZEROS, FP16, 1, 2, 8, true>(a, s);
+    if (a.T > 16) return i4_split_run<G, ZEROS, FP16, 1, 1, 8, true>(a, s);
+    if (p.waves == 16) return i4_split_run<G, ZEROS, FP16, 1, 1, 16, false>(a, s);
+    return i4_split_run<G, ZEROS, FP16, 1, 1, 8, false>(a, s);
 }
 
 }  // namespace pd
@@ -604,4 +627,9 @@ PD_API int pdscope_linear_int4(const void *x, const void *w, const void *bias, i
     else if (G == 64) group(std::integral_constant<int, 64>{});
     else group(std::integral_constant<int, 128>{});
     return check_launch("linear_int4");
+}
+
+PD_API int pdscope_linear_int4_launch(int T, int N, int K, int G) {
+    if (!i4_shape_ok(N, K, G) || i4_units(N, K) > ((int64_t)1 << 26) - 4 || T < 1 || T > (1 << 24)) return 0;
+    return i4_plan(T, N, K, G).launch;
 }
