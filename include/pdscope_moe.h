@@ -546,7 +546,8 @@ int pdscope_swiglu_grouped_mxfp8(const void *x, const void *x_scales, const int3
  * pdscope_linear_int4: y [T,N] = bf16(x [T,K] . W^T + bias), bias [N] bf16 or NULL,
  * with exact products of x and q, fp32 sums and fp32 scales; a row of x with an
  * infinity or NaN gives NaN, and a row of W with an infinite or NaN scale NaN or
- * infinities.  y may overlap nothing.
+ * infinities.  A group's sum of q x has to be a number of fp32: |x| < 2^117 is enough
+ * for every G; beyond it a row may give NaN.  y may overlap nothing.
  * Limits: 1 <= N <= 2^24, K % G == 0, K <= 2^20, fewer than 2^37 - 2^13 weights in whole
  * 16 x 128 units; 1 <= T <= 2^24, (N/256) * (T/64), each rounded up, at most 2^23; x, w,
  * codes and weight 16-byte aligned.
