@@ -237,6 +237,9 @@ int pdscope_swiglu_grouped_layer(const void *x, const int32_t *perm_token, const
  */
 int pdscope_merge(const void *y, const int32_t *row_of, const void *w, int T, int k, int H,
                   const void *add_in, void *out, void *stream);
+/* The same of fp32 rows y (pdscope_swiglu_grouped_mxfp8_y32 leaves such). */
+int pdscope_merge_y32(const void *y, const int32_t *row_of, const void *w, int T, int k, int H,
+                      const void *add_in, void *out, void *stream);
 
 /*
  * A8 in the arithmetic of the reference's default merge (merge='reference',
@@ -514,10 +517,17 @@ int pdscope_merge_norm_residual_mxfp8(const void *y, int64_t y_rows, const int32
                                       const void *gate, int gate_rows, int gate_cols, float scale, const void *pre_w,
                                       int params_f32, float eps, int T, int H, void *out_resid, void *out_norm,
                                       void *out_codes, void *out_scales, void *stream);
+/* pdscope_merge_norm_residual (codes and scales NULL) and the call above over fp32 rows y. */
+int pdscope_merge_norm_residual_y32(const void *y, int64_t y_rows, const int32_t *row_of, const void *w, int k,
+                                    const void *add_in, const void *resid, int resid_f32, const void *post_w,
+                                    const void *gate, int gate_rows, int gate_cols, float scale, const void *pre_w,
+                                    int params_f32, float eps, int T, int H, void *out_resid, void *out_norm,
+                                    void *out_codes, void *out_scales, void *stream);
 
 /*
  * pdscope_swiglu_grouped_mxfp4 over 8-bit rows x [T,H] (codes and scales):
- *   h[r] = rows8(silu(x . gate_e^T) * (x . up_e^T)),  y[r] = bf16(h[r] . down_e^T)
+ *   h[r] = rows8(silu(x . gate_e^T) * (x . up_e^T)),  y[r] = bf16(h[r] . down_e^T), or
+ *   (pdscope_swiglu_grouped_mxfp8_y32) y[r] = h[r] . down_e^T in fp32, whose merge rounds once,
  * with exact products of the codes' values and fp32 sums; h [rows,I] and h_scales
  * [rows,I/32] are 8-bit rows by the rule above, from the unrounded product.  A
  * row of h with an infinity or NaN makes its row of y NaN.  block_m: 32 or 64, the row
@@ -531,6 +541,10 @@ int pdscope_swiglu_grouped_mxfp8(const void *x, const void *x_scales, const int3
                                  const int32_t *offsets, const int32_t *sel, int nsel, const int32_t *tile_start,
                                  int max_tiles, int block_m, const void *const *slots, int H, int I, void *h,
                                  void *h_scales, void *y, void *stream);
+int pdscope_swiglu_grouped_mxfp8_y32(const void *x, const void *x_scales, const int32_t *perm_token,
+                                     const int32_t *offsets, const int32_t *sel, int nsel, const int32_t *tile_start,
+                                     int max_tiles, int block_m, const void *const *slots, int H, int I, void *h,
+                                     void *h_scales, void *y, void *stream);
 
 /*
  * 4-bit matrices with group scales, W[n,k] = s[n,k/G] * (q[n,k] - z[n,k/G]): q and z

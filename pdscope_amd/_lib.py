@@ -44,6 +44,7 @@ SIGNATURES = {
     "pdscope_swiglu_grouped_layer": ([_vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _i32, _i32,
                                       _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp], _i32),
     "pdscope_merge": ([_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp], _i32),
+    "pdscope_merge_y32": ([_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp], _i32),
     "pdscope_merge_ordered": ([_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp], _i32),
     "pdscope_swiglu_decode": ([_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp], _i32),
     "pdscope_swiglu_decode_shared": ([_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i32,
@@ -80,8 +81,12 @@ SIGNATURES = {
                                      _vp, _vp, _vp], _i32),
     "pdscope_merge_norm_residual_mxfp8": ([_vp, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _f32, _vp,
                                            _i32, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _vp], _i32),
+    "pdscope_merge_norm_residual_y32": ([_vp, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _f32, _vp,
+                                           _i32, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _vp], _i32),
     "pdscope_grouped_mxfp8_block_m": ([_i32], _i32),
     "pdscope_swiglu_grouped_mxfp8": ([_vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp,
+                                      _vp], _i32),
+    "pdscope_swiglu_grouped_mxfp8_y32": ([_vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp,
                                       _vp], _i32),
     "pdscope_int4_bytes": ([_i32, _i32, _i32, _i32], _sz),
     "pdscope_int4_pack": ([_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp], _i32),

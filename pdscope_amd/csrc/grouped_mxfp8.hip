@@ -3,7 +3,7 @@
 // routed to it.
 //
 //   gate/up : h[r,:] = rows8(silu(x_r . gate) * (x_r . up))
-//   down    : y[r,n] = bf16(h_r . down_n)
+//   down    : y[r,n] = h_r . down_n, in fp32 or rounded to bf16
 //
 // Both operands go to the scaled matrix instruction as they are, codes and
 // scales: v_mfma_scale_f32_16x16x128_f8f6f4, whose products are exact and whose
@@ -13,10 +13,10 @@
 //
 // The instruction adds groups of eight products, each cut to 2^-13 of the largest
 // one's binade, and the groups in fp32: about 4e-6 of an output's size, far below the codes'.
-// Rounded to fewer bits are h (8-bit rows, from the unrounded product: what its down
-// product takes) and each expert's row of y (bf16, as the other grouped kernels leave it to
-// the merge, which sums in fp32 and rounds once more: together 2.4e-3 of an output against
-// 1.7e-3 for the last rounding alone; fp32 rows of y would be 8 to 10% of a long prompt's time).
+// Rounded to fewer bits is h (8-bit rows, from the unrounded product: what its down
+// product takes), and where the caller's y is bf16 each expert's row (as the other grouped kernels
+// leave it to the merge, which sums in fp32 and rounds once more: together 2.4e-3 of an output
+// against 1.7e-3 for the last rounding alone, more where rows cancel).  Rows in fp32 leave that one only.
 //
 // Wave tile: 64 rows of weights x BM rows of x.  Weights go from memory to registers,
 // where a wave is the only one that needs them, a step of 128 inputs ahead; x through two
@@ -50,7 +50,7 @@ struct Mx8Grouped {
     const int32_t *tile_start;
     const uint8_t *const *slots;
     int H, I;
-    uint8_t *out, *out_scales;  // gate/up: h codes and scales; down: y bf16 [rows, H], null
+    uint8_t *out, *out_scales;  // gate/up: h codes and scales; down: y [rows, H] bf16 or fp32, null
 };
 
 // Waves of a workgroup, a row group each.  Eight in the down half of BM = 32, two workgroups a CU: Qwen
@@ -62,14 +62,14 @@ template <bool GATEUP>
 constexpr int kMx8OutRow = kMx8Waves * (GATEUP ? 32 : 128) + 16;
 template <int BM>
 constexpr int kMx8Stage = BM * 128 + 256;  // codes and scales of a step's 128 inputs
-template <int BM, bool GATEUP>
-constexpr int kMx8Lds = std::max(2 * kMx8Stage<BM>, BM * kMx8OutRow<GATEUP> + (GATEUP ? BM * kMx8Waves : 0));
+template <int BM, bool GATEUP, bool Y32>
+constexpr int kMx8Lds = std::max(2 * kMx8Stage<BM>, Y32 ? 0 : BM * kMx8OutRow<GATEUP> + (GATEUP ? BM * kMx8Waves : 0));
 
 // BM rows x four groups (128 h columns or 256 y columns), K in steps of 128, two
-// stages of activations; at least OCC workgroups per CU.
-template <int BM, bool GATEUP, int OCC>
+// stages of activations; at least OCC workgroups per CU.  Y32: rows of y in fp32 (down).
+template <int BM, bool GATEUP, int OCC, bool Y32>
 __global__ __launch_bounds__(64 * kMx8Waves, OCC) void mx8_grouped_kernel(Mx8Grouped p) {
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[kMx8Lds<BM, GATEUP>];
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kMx8Lds<BM, GATEUP, Y32>];
     constexpr int TM = BM / 16, NW = kMx8Waves;
     const int H = p.H, I = p.I;
     const int K = GATEUP ? H : I, KT = K / kGroupIn;
@@ -217,6 +217,23 @@ __global__ __launch_bounds__(64 * kMx8Waves, OCC) void mx8_grouped_kernel(Mx8Gro
     if (row_end - p.offsets[e] <= BM) run(std::true_type{});
     else run(std::false_type{});
 
+    const int rows = min(BM, row_end - m0);
+    if constexpr (Y32) {
+        // four neighbouring columns a lane are 16 bytes already: out as they are, 64 bytes of a
+        // row side by side and the next 64 by the store behind, and kept for the merge (4096
+        // tokens of the DeepSeek-V2-Lite shape: 105 us and 37 in the merge, where bf16 rows take 84 and 21,
+        // the bytes' time; not kept 108 and 43; 1303 of the Qwen shape 46 and 16 against 37 and 9)
+        if (rg >= groups) return;
+#pragma unroll
+        for (int m = 0; m < TM; ++m) {
+            if (16 * m + r >= rows) continue;
+            float *y = reinterpret_cast<float *>(p.out) + (size_t)(m0 + 16 * m + r) * H + rg * kGroupRows + 4 * g;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4_t *>(y + 16 * i) = acc[i][m];
+        }
+        return;
+    }
+
     // ---- epilogue: a lane holds token row r of each tile and weight rows 4 g ..
     // + 3 of each 16-row tile; through LDS, out in whole-row 16-byte stores.  The 32
     // columns of h that a wave has of a row are one scale block, in four lanes.
@@ -248,7 +265,6 @@ __global__ __launch_bounds__(64 * kMx8Waves, OCC) void mx8_grouped_kernel(Mx8Gro
         }
     }
     __syncthreads();
-    const int rows = min(BM, row_end - m0);
     constexpr int CO = NW * (GATEUP ? 32 : 128), CH = CO / 16;  // bytes and 16-byte pieces of a row
     const int ldo = GATEUP ? I : 2 * H, bytes = min(CO, ldo - nt * CO);  // bytes % 128 == 0
     for (int c = tid; c < rows * CH; c += 64 * NW) {
@@ -278,16 +294,16 @@ struct Mx8Call {
     hipStream_t s;
 };
 
-template <int BM, int OCC>
+template <int BM, int OCC, bool Y32>
 static int mx8_grouped_launch(const Mx8Call &c, const uint8_t *x, const uint8_t *xs, const int32_t *perm, uint8_t *h,
                               uint8_t *hs, uint8_t *y) {
     constexpr int NW = kMx8Waves;
     auto grid = [&](int nt) { return (unsigned)(((size_t)c.max_tiles * nt + 7) / 8 * 8); };
-    mx8_grouped_kernel<BM, true, OCC><<<grid((c.I / 32 + NW - 1) / NW), 64 * NW, 0, c.s>>>(
+    mx8_grouped_kernel<BM, true, OCC, false><<<grid((c.I / 32 + NW - 1) / NW), 64 * NW, 0, c.s>>>(
         Mx8Grouped{x, xs, perm, c.offsets, c.sel, c.nsel, c.tile_start, c.slots, c.H, c.I, h, hs});
     const int rc = check_launch("mx8_grouped_kernel<gateup>");
     if (rc) return rc;
-    mx8_grouped_kernel<BM, false, OCC><<<grid((c.H / kGroupRows + NW - 1) / NW), 64 * NW, 0, c.s>>>(
+    mx8_grouped_kernel<BM, false, OCC, Y32><<<grid((c.H / kGroupRows + NW - 1) / NW), 64 * NW, 0, c.s>>>(
         Mx8Grouped{h, hs, nullptr, c.offsets, c.sel, c.nsel, c.tile_start, c.slots, c.H, c.I, y, nullptr});
     return check_launch("mx8_grouped_kernel<down>");
 }
@@ -300,10 +316,10 @@ using namespace pd;
 // rows, 58.3 us against 63.2 with 64; T = 400, 25 rows, 74.6 against 65.8): weights are read once a tile.
 PD_API int pdscope_grouped_mxfp8_block_m(int rows_hint) { return rows_hint <= 16 ? 32 : 64; }
 
-PD_API int pdscope_swiglu_grouped_mxfp8(const void *x, const void *x_scales, const int32_t *perm_token,
-                                        const int32_t *offsets, const int32_t *sel, int nsel, const int32_t *tile_start,
-                                        int max_tiles, int block_m, const void *const *slots, int H, int I, void *h,
-                                        void *h_scales, void *y, void *stream) {
+template <bool Y32>
+static int swiglu_grouped_mxfp8(const void *x, const void *x_scales, const int32_t *perm_token, const int32_t *offsets,
+                                const int32_t *sel, int nsel, const int32_t *tile_start, int max_tiles, int block_m,
+                                const void *const *slots, int H, int I, void *h, void *h_scales, void *y, void *stream) {
     if (!x || !x_scales || !perm_token || !offsets || !sel || !tile_start || !slots || !h || !h_scales || !y)
         return fail(kEInval, "grouped_mxfp8: null pointer");
     if (nsel < 1 || max_tiles < 1 || max_tiles > (1 << 22))
@@ -322,6 +338,23 @@ PD_API int pdscope_swiglu_grouped_mxfp8(const void *x, const void *x_scales, con
                     reinterpret_cast<hipStream_t>(stream)};
     auto *xc = (const uint8_t *)x, *xs = (const uint8_t *)x_scales;
     auto *hc = (uint8_t *)h, *hs = (uint8_t *)h_scales, *out = (uint8_t *)y;
-    if (block_m == 32) return mx8_grouped_launch<32, 4>(c, xc, xs, perm_token, hc, hs, out);
-    return mx8_grouped_launch<64, 2>(c, xc, xs, perm_token, hc, hs, out);
+    if (block_m == 32) return mx8_grouped_launch<32, 4, Y32>(c, xc, xs, perm_token, hc, hs, out);
+    return mx8_grouped_launch<64, 2, Y32>(c, xc, xs, perm_token, hc, hs, out);
+}
+
+PD_API int pdscope_swiglu_grouped_mxfp8(const void *x, const void *x_scales, const int32_t *perm_token,
+                                        const int32_t *offsets, const int32_t *sel, int nsel, const int32_t *tile_start,
+                                        int max_tiles, int block_m, const void *const *slots, int H, int I, void *h,
+                                        void *h_scales, void *y, void *stream) {
+    return swiglu_grouped_mxfp8<false>(x, x_scales, perm_token, offsets, sel, nsel, tile_start, max_tiles, block_m, slots, H,
+                                       I, h, h_scales, y, stream);
+}
+
+PD_API int pdscope_swiglu_grouped_mxfp8_y32(const void *x, const void *x_scales, const int32_t *perm_token,
+                                            const int32_t *offsets, const int32_t *sel, int nsel,
+                                            const int32_t *tile_start, int max_tiles, int block_m,
+                                            const void *const *slots, int H, int I, void *h, void *h_scales, void *y,
+                                            void *stream) {
+    return swiglu_grouped_mxfp8<true>(x, x_scales, perm_token, offsets, sel, nsel, tile_start, max_tiles, block_m, slots, H, I,
+                                      h, h_scales, y, stream);
 }

@@ -3,7 +3,8 @@
 //   merge       restates the fused index_add_ merge of
 //               expertbench/pdscope_runtime.py:450-469 as a gather: each
 //               thread owns 8 output columns of one token and sums its k
-//               rows in fp32, slot order, rounding once (no atomics).
+//               rows in fp32, slot order, rounding once (no atomics); the
+//               rows are bf16, or fp32 (merge_y32).
 //   merge_ordered restates the default per-expert merge of
 //               pdscope_runtime.py:466-468 (merge='reference'): a token's k
 //               rows are added in ascending expert id, each product rounded
@@ -15,6 +16,8 @@
 //   stage_merge restates native/native_layer_dispatch.cpp:83-88 (copy the
 //               CPU block to device scratch, then index_add_ of
 //               scratch * weights into out) in bf16 arithmetic, rows in order.
+#include <type_traits>
+
 #include "common.h"
 
 namespace pd {
@@ -50,6 +53,12 @@ struct MergeAcc {
             }
         }
     }
+    // columns 4 half .. + 3, of an fp32 row
+    __device__ __forceinline__ void add32(float w, int half, uint4 v) {
+        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) a[4 * half + q] = __builtin_fmaf(w, __uint_as_float(x[q]), a[4 * half + q]);
+    }
     __device__ __forceinline__ void add_last(uint4 v) {
         round_add(0, lo_bf(v.x), hi_bf(v.x));
         round_add(2, lo_bf(v.y), hi_bf(v.y));
@@ -73,8 +82,9 @@ struct MergeAcc {
 // over all k for each next row in every thread took 71 us at T=4096, k=8,
 // H=2048, 27 now (25 for the fp32 sum), and the roundings in integer
 // arithmetic more than the loads (now the hardware's pair conversion).
-template <int KM, bool ORDERED>
-__global__ __launch_bounds__(256) void merge_kernel(const uint16_t *__restrict__ y,
+// Y32: rows of y in fp32 (not ORDERED), YT its type.
+template <int KM, bool ORDERED, bool Y32 = false, typename YT = std::conditional_t<Y32, float, uint16_t>>
+__global__ __launch_bounds__(256) void merge_kernel(const YT *__restrict__ y,
                                                     const int32_t *__restrict__ row_of,
                                                     const uint16_t *__restrict__ w, int T, int k, int H,
                                                     const uint16_t *__restrict__ add_in,
@@ -112,14 +122,26 @@ __global__ __launch_bounds__(256) void merge_kernel(const uint16_t *__restrict__
         else acc.zero();
 #pragma unroll 1
         for (int b = 0; b < (KM > 8 ? k : 1); b += 8) {
-            uint4 v[8];
+            constexpr int P = Y32 ? 2 : 1;  // 16-byte pieces of a row's eight columns
+            uint4 v[8][P];
 #pragma unroll
             for (int s = 0; s < 8; ++s)
-                if (b + s < k)
-                    v[s] = reinterpret_cast<const uint4 *>(y + (size_t)__builtin_amdgcn_readlane(row, b + s) * H)[cc];
+                if (b + s < k) {
+                    const uint4 *at = reinterpret_cast<const uint4 *>(y + (size_t)__builtin_amdgcn_readlane(row, b + s) * H);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) v[s][i] = at[cc * P + i];
+                }
 #pragma unroll
             for (int s = 0; s < 8; ++s)
-                if (b + s < k) acc.add(bf2f((uint32_t)__builtin_amdgcn_readlane(wb, b + s)), v[s]);
+                if (b + s < k) {
+                    const float ws = bf2f((uint32_t)__builtin_amdgcn_readlane(wb, b + s));
+                    if constexpr (Y32) {
+                        acc.add32(ws, 0, v[s][0]);
+                        acc.add32(ws, 1, v[s][P - 1]);
+                    } else {
+                        acc.add(ws, v[s][0]);
+                    }
+                }
         }
         if (ORDERED && add_in) acc.add_last(addv);
         if (live) reinterpret_cast<uint4 *>(out + (size_t)t * H)[c] = acc.result();
@@ -127,8 +149,8 @@ __global__ __launch_bounds__(256) void merge_kernel(const uint16_t *__restrict__
 }
 
 // any k, one thread per chunk, one slot at a time
-template <bool ORDERED>
-__global__ __launch_bounds__(256) void merge_any_kernel(const uint16_t *__restrict__ y,
+template <bool ORDERED, bool Y32 = false, typename YT = std::conditional_t<Y32, float, uint16_t>>
+__global__ __launch_bounds__(256) void merge_any_kernel(const YT *__restrict__ y,
                                                         const int32_t *__restrict__ row_of,
                                                         const uint16_t *__restrict__ w, int T, int k, int H,
                                                         const uint16_t *__restrict__ add_in,
@@ -159,7 +181,14 @@ __global__ __launch_bounds__(256) void merge_any_kernel(const uint16_t *__restri
         } else {
             for (int s = 0; s < k; ++s) {
                 const int r = row_of[(size_t)t * k + s];
-                acc.add(bf2f(w[(size_t)t * k + s]), reinterpret_cast<const uint4 *>(y + (size_t)r * H)[c]);
+                const float ws = bf2f(w[(size_t)t * k + s]);
+                const uint4 *at = reinterpret_cast<const uint4 *>(y + (size_t)r * H);
+                if constexpr (Y32) {
+                    acc.add32(ws, 0, at[2 * c]);
+                    acc.add32(ws, 1, at[2 * c + 1]);
+                } else {
+                    acc.add(ws, at[c]);
+                }
             }
         }
         if (ORDERED && add_in) acc.add_last(reinterpret_cast<const uint4 *>(add_in + (size_t)t * H)[c]);
@@ -187,24 +216,25 @@ __global__ __launch_bounds__(256) void stage_merge_kernel(const uint16_t *__rest
 
 using namespace pd;
 
-template <bool ORDERED>
+template <bool ORDERED, bool Y32 = false>
 static int launch_merge(const void *y, const int32_t *row_of, const void *w, int T, int k, int H,
                         const void *add_in, void *out, void *stream) {
     if (!y || !row_of || !w || !out) return fail(kEInval, "merge: null pointer");
     if (T < 1 || k < 1 || H < 8 || H % 8) return fail(kEInval, "merge: need T,k >= 1 and H % 8 == 0");
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const uint16_t *yy = (const uint16_t *)y, *ww = (const uint16_t *)w, *aa = (const uint16_t *)add_in;
+    const auto *yy = (const std::conditional_t<Y32, float, uint16_t> *)y;
+    const uint16_t *ww = (const uint16_t *)w, *aa = (const uint16_t *)add_in;
     if (k <= 16) {
         const int64_t waves = (int64_t)T * ((H / 8 + 63) / 64);
         const int blocks = (int)std::min<int64_t>((waves + 3) / 4, 65536);
         if (k <= 8)
-            merge_kernel<8, ORDERED><<<blocks, 256, 0, s>>>(yy, row_of, ww, T, k, H, aa, (uint16_t *)out);
+            merge_kernel<8, ORDERED, Y32><<<blocks, 256, 0, s>>>(yy, row_of, ww, T, k, H, aa, (uint16_t *)out);
         else
-            merge_kernel<16, ORDERED><<<blocks, 256, 0, s>>>(yy, row_of, ww, T, k, H, aa, (uint16_t *)out);
+            merge_kernel<16, ORDERED, Y32><<<blocks, 256, 0, s>>>(yy, row_of, ww, T, k, H, aa, (uint16_t *)out);
     } else {
         const int64_t total = (int64_t)T * (H / 8);
         const int blocks = (int)std::min<int64_t>((total + 255) / 256, 65536);
-        merge_any_kernel<ORDERED><<<blocks, 256, 0, s>>>(yy, row_of, ww, T, k, H, aa, (uint16_t *)out);
+        merge_any_kernel<ORDERED, Y32><<<blocks, 256, 0, s>>>(yy, row_of, ww, T, k, H, aa, (uint16_t *)out);
     }
     return check_launch("merge_kernel");
 }
@@ -212,6 +242,11 @@ static int launch_merge(const void *y, const int32_t *row_of, const void *w, int
 PD_API int pdscope_merge(const void *y, const int32_t *row_of, const void *w, int T, int k, int H,
                          const void *add_in, void *out, void *stream) {
     return launch_merge<false>(y, row_of, w, T, k, H, add_in, out, stream);
+}
+
+PD_API int pdscope_merge_y32(const void *y, const int32_t *row_of, const void *w, int T, int k, int H,
+                             const void *add_in, void *out, void *stream) {
+    return launch_merge<false, true>(y, row_of, w, T, k, H, add_in, out, stream);
 }
 
 PD_API int pdscope_merge_ordered(const void *y, const int32_t *row_of, const void *w, int T, int k, int H,

@@ -29,11 +29,11 @@
 namespace pd {
 
 struct NormArgs {
-    const uint16_t *block;  // [T, H], or (k > 0) the experts' rows [y_rows, H]
+    const uint16_t *block;  // [T, H], or (k > 0) the experts' rows [y_rows, H], which may be fp32
     const int32_t *row_of;
     const uint16_t *w, *add_in;
     int64_t y_rows;
-    int k;
+    int k, y_f32;
     const void *resid;
     const void *post_w, *gate, *pre_w;
     int gate_rows, gate_cols;  // gate has a value per token / per channel
@@ -60,7 +60,8 @@ template <bool VEC, bool F32, bool NT = false>
 __device__ __forceinline__ void load8(const void *base, const Eight<VEC> &e, int H, float (&v)[8]) {
     if (VEC) {
         if (F32) {
-            const uint4 a = ld_g((const float *)base + e.at), b = ld_g((const float *)base + e.at + 4);
+            const float *p = (const float *)base + e.at;
+            const uint4 a = NT ? ld_nt(p) : ld_g(p), b = NT ? ld_nt(p + 4) : ld_g(p + 4);
             const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]);
@@ -135,8 +136,8 @@ __device__ __forceinline__ void narrow8(const float (&v)[8], float (&o)[8]) {
 }
 __device__ __forceinline__ void narrow8(const double (&v)[8], float (&o)[8]) { round_to_odd8(v, o); }
 
-// NV: eights of a row per thread; MX: 8-bit rows as well.
-template <bool VEC, bool R32, bool P32, int NV, bool MX>
+// NV: eights of a row per thread; MX: 8-bit rows as well; Y32: the experts' rows in fp32.
+template <bool VEC, bool R32, bool P32, int NV, bool MX, bool Y32>
 __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
     using F = std::conditional_t<MX, double, float>;
     __shared__ F s_sum[16];
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
         // slot order; a row outside y (an expert computed elsewhere) adds nothing
         const int32_t *rows = a.row_of + (size_t)t * a.k;
         const uint16_t *ws = a.w + (size_t)t * a.k;
-#pragma unroll 8
+#pragma unroll (Y32 ? 4 : 8)
         for (int s = 0; s < a.k; ++s) {
             const int32_t row = rows[s];
             const F w = bf2f(ws[s]);
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
             for (int j = 0; j < NV; ++j) {
                 if (!on[j]) continue;
                 float y[8];
-                load8<VEC, false, true>(a.block + (size_t)row * H, at[j], H, y);
+                load8<VEC, Y32, true>((const char *)a.block + (size_t)row * H * (Y32 ? 4 : 2), at[j], H, y);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[j][i] = fma(w, (F)y[i], v[j][i]);
             }
@@ -257,17 +258,17 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a) {
 
 constexpr int kNormMaxH = 16384;
 
-template <bool VEC, bool R32, bool P32, bool MX>
+template <bool VEC, bool R32, bool P32, bool MX, bool Y32>
 static void norm_launch(const NormArgs &a, int T, hipStream_t s) {
     const int n = (a.H + 511) / 512 * 64;  // eight values a thread
-    if (n <= 1024) norm_kernel<VEC, R32, P32, 1, MX><<<T, n, 0, s>>>(a);
-    else norm_kernel<VEC, R32, P32, 2, MX><<<T, (n / 2 + 63) / 64 * 64, 0, s>>>(a);
+    if (n <= 1024) norm_kernel<VEC, R32, P32, 1, MX, Y32><<<T, n, 0, s>>>(a);
+    else norm_kernel<VEC, R32, P32, 2, MX, Y32><<<T, (n / 2 + 63) / 64 * 64, 0, s>>>(a);
 }
 
 template <bool VEC, bool R32, bool P32>
 static void norm_launch(const NormArgs &a, int T, hipStream_t s) {
-    if (a.out_codes) norm_launch<VEC, R32, P32, true>(a, T, s);
-    else norm_launch<VEC, R32, P32, false>(a, T, s);
+    if (a.out_codes) a.y_f32 ? norm_launch<VEC, R32, P32, true, true>(a, T, s) : norm_launch<VEC, R32, P32, true, false>(a, T, s);
+    else a.y_f32 ? norm_launch<VEC, R32, P32, false, true>(a, T, s) : norm_launch<VEC, R32, P32, false, false>(a, T, s);
 }
 
 static int norm_call(const char *what, const NormArgs &a, int resid_f32, int params_f32, int T, void *stream) {
@@ -305,7 +306,7 @@ PD_API int pdscope_norm_residual(const void *block, const void *resid, int resid
                                  const void *gate, int gate_rows, int gate_cols, float scale, const void *pre_w,
                                  int params_f32, float eps, int T, int H, void *out_resid, void *out_norm,
                                  void *stream) {
-    const NormArgs a{(const uint16_t *)block, nullptr, nullptr, nullptr, 0, 0, resid, post_w, gate, pre_w,
+    const NormArgs a{(const uint16_t *)block, nullptr, nullptr, nullptr, 0, 0, 0, resid, post_w, gate, pre_w,
                      gate_rows, gate_cols, scale, eps, H, out_resid, (uint16_t *)out_norm, nullptr, nullptr};
     return norm_call("norm_residual", a, resid_f32, params_f32, T, stream);
 }
@@ -317,7 +318,7 @@ PD_API int pdscope_merge_norm_residual(const void *y, int64_t y_rows, const int3
                                        void *stream) {
     if (!row_of || !w) return fail(kEInval, "merge_norm_residual: null pointer");
     if (k < 1 || y_rows < 1) return fail(kEInval, "merge_norm_residual: need k >= 1 and y_rows >= 1");
-    const NormArgs a{(const uint16_t *)y, row_of, (const uint16_t *)w, (const uint16_t *)add_in, y_rows, k, resid, post_w,
+    const NormArgs a{(const uint16_t *)y, row_of, (const uint16_t *)w, (const uint16_t *)add_in, y_rows, k, 0, resid, post_w,
                      gate, pre_w, gate_rows, gate_cols, scale, eps, H, out_resid, (uint16_t *)out_norm, nullptr, nullptr};
     return norm_call("merge_norm_residual", a, resid_f32, params_f32, T, stream);
 }
@@ -327,7 +328,7 @@ PD_API int pdscope_norm_residual_mxfp8(const void *block, const void *resid, int
                                        int params_f32, float eps, int T, int H, void *out_resid, void *out_norm,
                                        void *out_codes, void *out_scales, void *stream) {
     if (!out_codes || !out_scales) return fail(kEInval, "norm_residual_mxfp8: null pointer");
-    const NormArgs a{(const uint16_t *)block, nullptr, nullptr, nullptr, 0, 0, resid, post_w, gate, pre_w,
+    const NormArgs a{(const uint16_t *)block, nullptr, nullptr, nullptr, 0, 0, 0, resid, post_w, gate, pre_w,
                      gate_rows, gate_cols, scale, eps, H, out_resid, (uint16_t *)out_norm, (uint8_t *)out_codes,
                      (uint8_t *)out_scales};
     return norm_call("norm_residual_mxfp8", a, resid_f32, params_f32, T, stream);
@@ -341,8 +342,21 @@ PD_API int pdscope_merge_norm_residual_mxfp8(const void *y, int64_t y_rows, cons
                                              void *stream) {
     if (!row_of || !w || !out_codes || !out_scales) return fail(kEInval, "merge_norm_residual_mxfp8: null pointer");
     if (k < 1 || y_rows < 1) return fail(kEInval, "merge_norm_residual_mxfp8: need k >= 1 and y_rows >= 1");
-    const NormArgs a{(const uint16_t *)y, row_of, (const uint16_t *)w, (const uint16_t *)add_in, y_rows, k, resid, post_w,
+    const NormArgs a{(const uint16_t *)y, row_of, (const uint16_t *)w, (const uint16_t *)add_in, y_rows, k, 0, resid, post_w,
                      gate, pre_w, gate_rows, gate_cols, scale, eps, H, out_resid, (uint16_t *)out_norm,
                      (uint8_t *)out_codes, (uint8_t *)out_scales};
     return norm_call("merge_norm_residual_mxfp8", a, resid_f32, params_f32, T, stream);
+}
+
+PD_API int pdscope_merge_norm_residual_y32(const void *y, int64_t y_rows, const int32_t *row_of, const void *w, int k,
+                                           const void *add_in, const void *resid, int resid_f32, const void *post_w,
+                                           const void *gate, int gate_rows, int gate_cols, float scale,
+                                           const void *pre_w, int params_f32, float eps, int T, int H, void *out_resid,
+                                           void *out_norm, void *out_codes, void *out_scales, void *stream) {
+    if (!row_of || !w || !out_codes != !out_scales) return fail(kEInval, "merge_norm_residual_y32: null pointer");
+    if (k < 1 || y_rows < 1) return fail(kEInval, "merge_norm_residual_y32: need k >= 1 and y_rows >= 1");
+    const NormArgs a{(const uint16_t *)y, row_of, (const uint16_t *)w, (const uint16_t *)add_in, y_rows, k, 1, resid, post_w,
+                     gate, pre_w, gate_rows, gate_cols, scale, eps, H, out_resid, (uint16_t *)out_norm,
+                     (uint8_t *)out_codes, (uint8_t *)out_scales};
+    return norm_call("merge_norm_residual_y32", a, resid_f32, params_f32, T, stream);
 }

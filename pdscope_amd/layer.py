@@ -18,10 +18,13 @@ ACTIVATIONS = ("bf16", "mxfp8")
 
 
 class MoEWorkspace:
-    """Device buffers for up to ``max_tokens`` tokens of one layer shape."""
+    """Device buffers for up to ``max_tokens`` tokens of one layer shape.  y_dtype: type
+    of the experts' rows y before the merge, bf16 or (experts over 8-bit rows only) fp32."""
 
     def __init__(self, max_tokens: int, H: int, I: int, E: int, k: int, device, *, route_only: bool = False,
-                 shared_I: int | None = None, few_tokens: bool = False, mxfp8: bool = False):
+                 shared_I: int | None = None, few_tokens: bool = False, mxfp8: bool = False, y_dtype=BF16):
+        if y_dtype not in (BF16, torch.float32):
+            raise ValueError(f"y_dtype must be bf16 or fp32, got {y_dtype}")
         device = torch.device(device)
         n = max_tokens * k
         i32 = dict(dtype=torch.int32, device=device)
@@ -40,7 +43,7 @@ class MoEWorkspace:
         self.sel_all = torch.arange(E, **i32)
         rows = 1 if route_only else max(n, 1)
         self.h_ws = torch.empty(rows * I, dtype=BF16, device=device)
-        self.y = torch.empty(rows * H, dtype=BF16, device=device)
+        self.y = torch.empty(rows * H, dtype=y_dtype, device=device)
         self.out = torch.empty((1 if route_only else max_tokens, H), dtype=BF16, device=device)
         self.hist = torch.empty(E, **i32)
         self.route_ws = ops.new_route_workspace(max_tokens, H, E, device)
@@ -182,13 +185,16 @@ def experts_resident(x, ids, weights, slots, ws: MoEWorkspace, out=None, *, bloc
     representation: what `slots` addresses, "bf16" or "mxfp4" blocks (4-bit, any
     T: K2, their grouped launches, K5; shared experts' output comes through add_in).
     x: bf16 rows, or 8-bit ones (ops.MxRows) for 4-bit experts, whose products then
-    run on 8-bit rows throughout."""
+    run on 8-bit rows throughout; with a workspace of y_dtype=torch.float32 the experts'
+    rows are not rounded before the merge."""
     mx8 = isinstance(x, ops.MxRows)
     T = x.codes.shape[0] if mx8 else x.shape[0]
     H, I, E, k = ws.H, ws.I, ws.E, ws.k
     out = ws.out[:T] if out is None else out
     if mx8 and not ops.is_mxfp4(representation):
         raise ValueError('8-bit rows need 4-bit experts (representation="mxfp4")')
+    if ws.y.dtype is not BF16 and (not mx8 or ops.merge_mode(merge)):
+        raise ValueError("fp32 rows of y are those of experts over 8-bit rows, with merge='fused'")
     if ops.is_mxfp4(representation):
         if shared_slot is not None:
             raise ValueError("shared experts join 4-bit routed experts through add_in")

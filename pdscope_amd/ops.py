@@ -692,10 +692,13 @@ class DecodeBinding:
 # --------------------------------------------------------------------- A8/A9
 
 def merge(y, row_of, w, out, add_in=None, *, mode="fused"):
+    """Weighted sum of each token's rows of y, bf16 or in mode "fused" fp32 (see pdscope_merge and, for mode
+    "reference", pdscope_merge_ordered)."""
     _need(w, "weights", BF16, 2)
     dev = w.device
+    y32 = isinstance(y, torch.Tensor) and y.dtype is torch.float32
     if not _line(y, BF16, dev):
-        _need(y, "y", BF16, None, dev)
+        _need(y, "y", torch.float32 if y32 else BF16, None, dev)
     if not _line(row_of, torch.int32, dev):
         _need(row_of, "row_of", torch.int32, 1, dev)
     _need(out, "out", BF16, 2, dev)
@@ -704,6 +707,10 @@ def merge(y, row_of, w, out, add_in=None, *, mode="fused"):
     if add_in is not None:
         _need(add_in, "add_in", BF16, 2, dev)
     name = "pdscope_merge_ordered" if merge_mode(mode) else "pdscope_merge"
+    if y32:
+        if merge_mode(mode):
+            raise ValueError("fp32 rows are merged in mode 'fused'")
+        name = "pdscope_merge_y32"
     _call_on(dev, name, _p(y), _p(row_of), _p(w), T, k, H, _p(add_in), _p(out))
     return out
 
@@ -896,7 +903,8 @@ def grouped_mxfp8_block_m(rows_hint: int) -> int:
 def swiglu_grouped_mxfp8(x: MxRows, perm_token, offsets, sel, tile_start, max_tiles, block_m, slots, H, I,
                          h_ws: MxRows, y):
     """swiglu_grouped_mxfp4 over 8-bit rows x; the experts' hidden rows go through h_ws
-    [rows, I] as 8-bit rows too (see pdscope_swiglu_grouped_mxfp8); block_m 32 or 64."""
+    [rows, I] as 8-bit rows too (see pdscope_swiglu_grouped_mxfp8); block_m 32 or 64.  y: bf16,
+    or fp32 for rows that are not rounded."""
     _need_rows(x, "inputs", None, H, None)
     dev = x.codes.device
     for t, n in ((perm_token, "perm_token"), (offsets, "offsets"), (sel, "sel"), (tile_start, "tile_start")):
@@ -905,8 +913,9 @@ def swiglu_grouped_mxfp8(x: MxRows, perm_token, offsets, sel, tile_start, max_ti
     if not _line(slots, torch.int64, dev):
         _need(slots, "slots", torch.int64, 1, dev)
     _need_rows(h_ws, "h_ws", None, I, dev)
+    y32 = isinstance(y, torch.Tensor) and y.dtype is torch.float32
     if not _line(y, BF16, dev):
-        _need(y, "y", BF16, None, dev)
+        _need(y, "y", torch.float32 if y32 else BF16, None, dev)
     check_slots(slots, H, I, "mxfp4")
     rows, nsel = perm_token.shape[0], sel.shape[0]
     if h_ws.codes.shape[0] < rows or y.numel() < rows * H:
@@ -917,7 +926,7 @@ def swiglu_grouped_mxfp8(x: MxRows, perm_token, offsets, sel, tile_start, max_ti
         raise ValueError("slots must hold one entry per expert")
     if max(x.codes.shape[0] * H, rows * I) >= 1 << 36:
         raise ValueError("swiglu_grouped_mxfp8 addresses fewer than 2^36 activations")
-    _call_on(dev, "pdscope_swiglu_grouped_mxfp8", x.codes.data_ptr(), x.scales.data_ptr(), perm_token.data_ptr(),
+    _call_on(dev, "pdscope_swiglu_grouped_mxfp8_y32" if y32 else "pdscope_swiglu_grouped_mxfp8", x.codes.data_ptr(), x.scales.data_ptr(), perm_token.data_ptr(),
              offsets.data_ptr(), sel.data_ptr(), nsel, tile_start.data_ptr(), int(max_tiles), int(block_m),
              slots.data_ptr(), H, I, h_ws.codes.data_ptr(), h_ws.scales.data_ptr(), y.data_ptr())
     return y
@@ -1187,14 +1196,15 @@ def merge_norm_residual(y, row_of, w, resid, *, add_in=None, post_weight=None, g
                         out_mxfp8=None):
     """norm_residual of the experts' weighted merge, which is summed in the same
     launch (as merge(y, row_of, w, add_in=add_in) in mode 'fused', and not rounded):
-    y [rows, H] grouped expert rows, row_of [T*k] int32 (an entry outside
+    y [rows, H] grouped expert rows, bf16 or fp32, row_of [T*k] int32 (an entry outside
     [0, rows) adds nothing), w [T, k] bf16, add_in [T, H] bf16 or None."""
     _need(w, "weights", BF16, 2)
     dev = w.device
     T, k = w.shape
     _need(resid, "resid", None, 2, dev)
     H = resid.shape[1]
-    _need(y, "y", BF16, None, dev)
+    y32 = isinstance(y, torch.Tensor) and y.dtype is torch.float32
+    _need(y, "y", torch.float32 if y32 else BF16, None, dev)
     _need(row_of, "row_of", torch.int32, 1, dev)
     if row_of.numel() != T * k:
         raise ValueError(f"row_of must hold T*k = {T * k} entries, got {row_of.numel()}")
@@ -1210,10 +1220,14 @@ def merge_norm_residual(y, row_of, w, resid, *, add_in=None, post_weight=None, g
     args = (_p(y), y.numel() // H, _p(row_of), _p(w), k, _p(add_in), _p(resid), f32, _p(post_weight), _p(gate), rows,
             cols, float(scale), _p(pre_weight), p32, float(eps), T, H, _p(out_resid), _p(out_norm))
     if not mx:
-        _call_on(dev, "pdscope_merge_norm_residual", *args)
+        if y32:
+            _call_on(dev, "pdscope_merge_norm_residual_y32", *args, None, None)
+        else:
+            _call_on(dev, "pdscope_merge_norm_residual", *args)
         return out_resid, out_norm
     out = _mx_out(out_mxfp8, T, H, dev)
-    _call_on(dev, "pdscope_merge_norm_residual_mxfp8", *args, _p(out.codes), _p(out.scales))
+    _call_on(dev, "pdscope_merge_norm_residual_y32" if y32 else "pdscope_merge_norm_residual_mxfp8", *args, _p(out.codes),
+             _p(out.scales))
     return out_resid, out_norm, out
 
 
