@@ -174,7 +174,8 @@ class _Experts:
             from pdscope_amd import layer, ops
             self.experts = ops.mxfp4_pack(self.codes, self.scales, H, I)
             self.slots = ops.slot_table([self.experts[e] for e in range(E)], DEV)
-            self.ws = layer.MoEWorkspace(T, H, I, E, k, DEV)
+            # rows of the experts as they are summed, so that the output is rounded once
+            self.ws = layer.MoEWorkspace(T, H, I, E, k, DEV, y_dtype=torch.float32)
 
 
 class _Linear:
