@@ -4,7 +4,7 @@
 //
 // One wave per unit, lane l = r + 16 g on the words that it owns: row r, inputs 32 j
 // + 8 g .. + 7.  Bound by memory: 2 bytes a value on the bf16 side, a little over half
-// a byte on the other.  4096 x 4096, G = 128: pack 8.1 us (2.1 TB/s), quantize 15.4 (2.7), dequantize
+// a byte on the other.  4096 x 4096, G = 128: pack 7.9 us (2.2 TB/s), quantize 14.9 (2.8), dequantize
 // 11.2 (3.8); done once a model.
 #include "int4.h"
 

@@ -12,7 +12,7 @@
 // (i4_rows_kernel), few rows with the K axis split over the waves of a workgroup
 // (i4_split_kernel), many in tiles through LDS (i4_gemm_kernel).  The first two are
 // bound by W's bytes or, for small matrices, by a launch's start, one load and one join: N = 151936, K
-// = 2048, G = 64 with zero points, one row 36 us (4.7 TB/s); K = 4096, G = 128 64 us (5.3); N = 2048,
+// = 2048, G = 64 with zero points, one row 36 us (4.7 TB/s); K = 4096, G = 128 64 us (5.0); N = 2048,
 // K = 4096 4.8 us (0.9).  With 16 rows x's bytes cost as much, read again by every workgroup: N = 4096, K
 // = 2048 5.1 us, N = 151936, K = 4096 82.
 #include <algorithm>
@@ -269,8 +269,8 @@ constexpr int kI4GemmStage = kI4GemmX + 4 * 512;  // 128 bytes at most for each 
 //
 // A step of RT = 4 issues 64 products and 4 for the sums, and some 220 other vector
 // instructions (112 decode, 64 scale) through the same port, so two waves take about 3100 cycles
-// where the products alone need 2200.  N = 4096, K = 2048, G = 128, T = 2048 37.3 us,
-// 0.92 PFLOP/s (G = 64 43, G = 32 56: more scalings), of which the loop 26, what is before and behind it
+// where the products alone need 2200.  N = 4096, K = 2048, G = 128, T = 2048 37 to
+// 38 us in a row of launches (42 traced one by one), 0.90 PFLOP/s (G = 64 43, G = 32 56), of which the loop 26, what is before and behind it
 // 4.3; without the loop's loads 33.6, without decoding 35.8, without reading x from LDS 30.4.  T = 4096 and
 // K = 4096 1.0 PFLOP/s.  Held back by neither alone; reading x 32 inputs ahead of the products or
 // another order of them changed nothing.  RT = 2 without parts has 168 registers, for three workgroups a
@@ -557,7 +557,7 @@ static I4Plan i4_plan(int T, int N, int K, int G) {
     // of its loads, and small ones that share the K axis have fewer steps: N = 4096,
     // K = 2048, tiles of 64 tokens x 64 rows in four parts / in two / x 128 in two / x 256: T = 256 11.1 / 12.0
     // / 15.6 / 24.7 us, T = 512 - / 22.4 / 15.7 / 24.6, T = 1024 - / 42 / 29 / 25.5, T = 2048 - / 83 / 57 /
-    // 37.3; K = 4096, N = 2048, T = 512 16.9 / 19.4 / 24.9 / 44.6.  Tiles of 128 rows without
+    // 37 to 38; K = 4096, N = 2048, T = 512 16.9 / 19.4 / 24.9 / 44.6.  Tiles of 128 rows without
     // parts go by up to three a CU, those of 256 by two; a round of 256 of the former counts as 10, one
     // of 256 of the latter as 24, of 512 as 34 (against 256 rows, G = 128 / 32: T = 640 23.5 / 33.6 us
     // and 24.8 / 38.2, T = 1300 32.3 / 45.0 and 36.0 / 55.0, T = 1600 42.7 / 58.4 and 35.9 / 55.7, N = 4097,

@@ -3,8 +3,8 @@
 // activations are bf16 only.
 //
 // A thread has eight channels, four neighbours a scale block.  Bound by memory: 2 bytes
-// a value on one side, 33/32 on the other.  4096 rows of 2048: 7.5 us to rows and 6.0 back,
-// 3.4 and 4.2 TB/s.
+// a value on one side, 33/32 on the other.  4096 rows of 2048: 6.1 to 6.7 us to rows and 5.2 to
+// 5.9 back, 3.8 to 4.2 and 4.3 to 4.9 TB/s.
 #include "mxfp8.h"
 
 namespace pd {
