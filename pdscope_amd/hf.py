@@ -125,7 +125,8 @@ def install_int4_linears(model, group=128, zeros=False, keep=()):
         if m.weight.dtype != torch.bfloat16 or m.weight.device.type != "cuda":
             raise ValueError(f"{name} must be bf16 on the GPU, got {m.weight.dtype} on {m.weight.device}")
         if m.bias is not None and (m.bias.dtype != m.weight.dtype or m.bias.device != m.weight.device):
-            raise ValueError(f"{name}'s bias must be as its weight, bf16 on {m.weight.device}, got {m.bias.dtype} on {m.bias.device}")
+            raise ValueError(f"{name}'s bias must be as its weight, bf16 on {m.weight.device}, got {m.bias.dtype} on "
+                             f"{m.bias.device}")
         if m.in_features % group:
             raise ValueError(f"{name} has {m.in_features} inputs, not whole groups of {group}: keep it or take smaller groups")
     forms = {}

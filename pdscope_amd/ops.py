@@ -926,9 +926,9 @@ def swiglu_grouped_mxfp8(x: MxRows, perm_token, offsets, sel, tile_start, max_ti
         raise ValueError("slots must hold one entry per expert")
     if max(x.codes.shape[0] * H, rows * I) >= 1 << 36:
         raise ValueError("swiglu_grouped_mxfp8 addresses fewer than 2^36 activations")
-    _call_on(dev, "pdscope_swiglu_grouped_mxfp8_y32" if y32 else "pdscope_swiglu_grouped_mxfp8", x.codes.data_ptr(), x.scales.data_ptr(), perm_token.data_ptr(),
-             offsets.data_ptr(), sel.data_ptr(), nsel, tile_start.data_ptr(), int(max_tiles), int(block_m),
-             slots.data_ptr(), H, I, h_ws.codes.data_ptr(), h_ws.scales.data_ptr(), y.data_ptr())
+    _call_on(dev, "pdscope_swiglu_grouped_mxfp8_y32" if y32 else "pdscope_swiglu_grouped_mxfp8", x.codes.data_ptr(),
+             x.scales.data_ptr(), perm_token.data_ptr(), offsets.data_ptr(), sel.data_ptr(), nsel, tile_start.data_ptr(),
+             int(max_tiles), int(block_m), slots.data_ptr(), H, I, h_ws.codes.data_ptr(), h_ws.scales.data_ptr(), y.data_ptr())
     return y
 
 
